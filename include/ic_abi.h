@@ -466,6 +466,76 @@ int ic_piso_scales(const float* W, int64_t rows, int64_t cols, int64_t ld, const
                    const float* coarse, int num_coarse, const float* fine, int num_fine, float* scales,
                    int8_t* zp, void* stream);
 
+/* ---------------------------------------------------------------- running quantised layers
+ *
+ * No counterpart in the reference: the operators that a program needs to run
+ * the layers that the entry points above quantised.  dtype: IC_DTYPE_*. */
+
+/* The leading dimension of 8-bit activations of `cols` columns (a multiple
+ * of 128 bytes). */
+int64_t ic_activation_pitch(int64_t cols);
+
+/* Rows of activations as 8-bit codes:
+ *   h = x + residual; y = h * (mean(h^2) + eps)^-1/2 * weight;
+ *   z = R pad(y) (the rotation of ic_rotate_rows; rot 1, 4, 16, 64 or 256);
+ *   s = max(max|z|, 1e-30) / 127;  q = clamp(rhaz(z / s), -127, 127)
+ * in fp32.  x [rows, cols] (ld_x) and residual / residual_out (ld_r, ld_ro;
+ * both NULL = no residual; residual_out, h in x's dtype, may be residual
+ * itself) of `dtype`; weight [cols] of weight_dtype (x's, or fp32), NULL =
+ * no norm.  codes [rows, ld_q] with ld_q = ic_activation_pitch(cols padded
+ * to rot), 16-byte aligned, zeros behind the last column; scales fp32 [rows];
+ * sums int32 [rows] = the codes' row sums.  A row with Inf or NaN gets the
+ * scale NaN and codes 0.  At most 65536 padded columns. */
+int ic_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void* residual,
+                     int64_t ld_r, const void* weight, int weight_dtype, float eps, int rot, int8_t* codes,
+                     int64_t ld_q, float* scales, int32_t* sums, void* residual_out, int64_t ld_ro, void* stream);
+
+/* out[r, c] = codes[r, c] * scales[r] in `dtype`. */
+int ic_dequantize_rows(const int8_t* codes, int64_t rows, int64_t cols, int64_t ld_q, const float* scales, void* out,
+                       int dtype, int64_t ld_out, void* stream);
+
+/* sums[r] = sum of row r's codes (for codes made elsewhere). */
+int ic_row_sums_i8(const int8_t* codes, int64_t rows, int64_t cols, int64_t ld_q, int32_t* sums, void* stream);
+
+/* A stored weight (int8 [N, K], or INT4 bytes [N, ceil(K/2)], pitch ld
+ * bytes) laid out once for ic_quantized_linear; ic_linear_weight_bytes()
+ * bytes, 16-byte aligned. */
+int64_t ic_linear_weight_bytes(int64_t N, int64_t K, int bits);
+int ic_linear_pack_weight(const void* stored, int bits, int64_t N, int64_t K, int64_t ld, void* tiles, void* stream);
+
+/* out[m, n] = sa[m] sw[n] (sum_k a q - zp[n] sum_k a) + bias[n], the sums
+ * exact in int32.  a [M, K] int8 (ld_a as ic_activation_pitch or more, zeros
+ * or any codes behind column K: the weight's are zero), sa [M], sums [M]
+ * (may be NULL without zero-points); tiles from ic_linear_pack_weight; sw [N] fp16 bits (sw_kind
+ * 0) or fp32 (1); zp int8 [N] or NULL; bias [N] of bias_dtype or NULL; out
+ * [M, N] (ld_out) of out_dtype.  K <= 65536; M, N <= 1048560. */
+int ic_quantized_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t M,
+                        const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,
+                        int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out, void* stream);
+
+/* Microscaled 4-bit floating point (OCP MX): E2M1 elements, one E8M0 scale
+ * for 32 consecutive columns, 2^(floor(log2(max|x|)) - 2); elements to the
+ * nearest, ties to even, at most 6.  A block with Inf or NaN: scale byte 255,
+ * codes 0.  Operands are kept in tiles of 16 rows x 128 columns (csrc/
+ * lowbit.hpp): ic_mxfp4_code_bytes() of codes and ic_mxfp4_scale_bytes() of
+ * scales, 16-byte aligned. */
+int64_t ic_mxfp4_code_bytes(int64_t rows, int64_t cols);
+int64_t ic_mxfp4_scale_bytes(int64_t rows, int64_t cols);
+int ic_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, void* codes, void* scales,
+                      void* stream);
+int ic_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, void* out, int dtype,
+                        int64_t ld_out, void* stream);
+
+/* Row-major codes [rows, ceil(cols/2)] (even column in the low nibble) and
+ * scales [rows, ceil(cols/32)] to tiles (to_tiles 1), or back (0). */
+int ic_mxfp4_relayout(void* flat_codes, int64_t ld_codes, void* flat_scales, int64_t ld_scales, int64_t rows,
+                      int64_t cols, void* codes, void* scales, int to_tiles, void* stream);
+
+/* out = A W^T + bias, A [M, K] and W [N, K] in tiles, summed in fp32. */
+int ic_mxfp4_linear(const void* a, const void* a_scales, int64_t M, const void* w, const void* w_scales,
+                    const void* bias, int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out,
+                    void* stream);
+
 /* ---------------------------------------------------------------- profiling */
 
 /* HBM ceiling probes (measurement only; no counterpart in the reference):

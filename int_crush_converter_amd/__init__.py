@@ -2,7 +2,10 @@
 
 Public names mirror the reference package ``converter`` (its ``__init__.py``)
 for the hot path: rotation, RTN scales, PiSO scales, packing, DLR Hessians,
-GPTQ / LDLQ layers, the pipeline and the value types.  The reference's
+GPTQ / LDLQ layers, the pipeline and the value types.  Beside them stand the
+operators that run what it produced (no counterpart in the reference): norm
+and quantisation of activations, products with the stored weights, and the
+microscaled 4-bit format.  The reference's
 SmoothQuant / SmoothRot / SVD helpers are outside this path and not
 exported.  All arithmetic runs in the gfx950 HIP library
 ``libicq.so`` (see ``include/ic_abi.h``); there is no CPU fallback.
@@ -40,6 +43,9 @@ from .gptq import gptq_quantize_layer, gptq_quantize_layer_rtn
 from .ldlq import ldlq_quantize_layer
 from .calibration_io import load_calibration, build_name_map, get_hessian, get_per_channel_amax
 from .pipeline import quantize_model, should_skip
+from .activations import QuantizedActivations, rms_norm_quantize, quantize_activations
+from .linear import QuantizedWeight, quantized_linear
+from .mxfp4 import Mxfp4Tensor, mxfp4_quantize, mxfp4_linear
 from .types import QuantizationResult, QuantizeConfig, ProgressInfo, ProgressSummary, ProgressCallback
 
 __all__ = [
@@ -57,4 +63,6 @@ __all__ = [
     "QuantizationResult", "QuantizeConfig", "ProgressInfo", "ProgressSummary", "ProgressCallback",
     "compute_piso_scales_int8", "compute_piso_scales_int8_asymmetric",
     "compute_piso_scales_int4", "compute_piso_scales_int4_asymmetric",
+    "QuantizedActivations", "rms_norm_quantize", "quantize_activations", "QuantizedWeight", "quantized_linear",
+    "Mxfp4Tensor", "mxfp4_quantize", "mxfp4_linear",
 ]

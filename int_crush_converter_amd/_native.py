@@ -94,6 +94,21 @@ _SIGS = {
     "ic_woodbury_workspace_bytes": (_i64, [_i64, _i64]),
     "ic_woodbury_inverse": (_i32, [_vp, _vp, _i64, _i64, _i64, _f32, _vp, _i32, _vp, _i64, _vp, _vp, _vp, _vp]),
     "ic_dlr_to_dense": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "ic_activation_pitch": (_i64, [_i64]),
+    "ic_quantize_rows": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _vp, _i64, _vp, _vp, _vp,
+                                _i64, _vp]),
+    "ic_dequantize_rows": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _vp]),
+    "ic_row_sums_i8": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp]),
+    "ic_linear_weight_bytes": (_i64, [_i64, _i64, _i32]),
+    "ic_linear_pack_weight": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp]),
+    "ic_quantized_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp,
+                                   _i32, _i64, _vp]),
+    "ic_mxfp4_code_bytes": (_i64, [_i64, _i64]),
+    "ic_mxfp4_scale_bytes": (_i64, [_i64, _i64]),
+    "ic_mxfp4_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "ic_mxfp4_dequantize": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp]),
+    "ic_mxfp4_relayout": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _vp]),
+    "ic_mxfp4_linear": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _vp]),
     "ic_piso_scales": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp]),
 }
 

@@ -1,0 +1,149 @@
+"""8-bit activations for layers that the converter quantised.
+
+``rms_norm_quantize`` and ``quantize_activations`` turn rows of 16- or 32-bit
+activations into int8 codes with one fp32 scale a row (``q * s``, ``s`` the
+largest magnitude / 127, halves rounded away from zero like the weights'
+codes), after the regular-Hadamard rotation that the weights had
+(``rotate_weights``): ``W x = (W R^T)(R x)``.  One pass of the HIP library
+(``ic_quantize_rows``) adds the residual, normalises, rotates and quantises.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+
+ROT_SIZES = (1, 4, 16, 64, 256)
+MAX_FEATURES = 65536
+_PAD = 128                       # ic_activation_pitch
+
+
+def check_gpu(name: str, t: torch.Tensor) -> torch.Tensor:
+    """A tensor in GPU memory, on the current device."""
+    t = nat.to_gpu(t)
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return t
+
+
+def as_rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., K] as 2-D rows whose columns are contiguous (a copy only where the strides ask for one)."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.stride(1) != 1 and t.shape[1] > 1 or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        t = t.contiguous()
+    return t
+
+
+class QuantizedActivations:
+    """int8 codes of shape ``[*lead, in_features]``, their fp32 scales and the int32 sums of each row's codes.
+    On the GPU; rows are stored at a pitch of whole 128 bytes, zeros behind the last column."""
+
+    __slots__ = ("data", "scales", "sums", "in_features", "lead")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, sums: torch.Tensor, in_features: int, lead):
+        self.data, self.scales, self.sums = data, scales, sums
+        self.in_features, self.lead = in_features, tuple(lead)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "QuantizedActivations":
+        """Codes [..., K] (int8) and scales [...] from elsewhere.  The codes are copied unless their rows already
+        have the stored layout."""
+        if codes.dim() < 1 or codes.dtype != torch.int8:
+            raise ValueError(f"expected int8 codes [..., K], got {codes.dtype} {tuple(codes.shape)}")
+        lead, K = codes.shape[:-1], codes.shape[-1]
+        if not 1 <= K <= MAX_FEATURES:
+            raise ValueError(f"in_features must be in [1, {MAX_FEATURES}], got {K}")
+        codes = as_rows(check_gpu("codes", codes)) if codes.numel() else check_gpu("codes", codes).reshape(-1, K)
+        rows = codes.shape[0]
+        if scales.numel() != rows:
+            raise ValueError(f"{scales.numel()} scales for {rows} rows of codes")
+        scales = check_gpu("scales", scales).reshape(-1).to(torch.float32).contiguous()
+        if K % _PAD or codes.stride(0) != K or codes.data_ptr() % 16:
+            data = torch.zeros(rows, -(-K // _PAD) * _PAD, dtype=torch.int8, device=codes.device)
+            data[:, :K] = codes
+        else:
+            data = codes
+        sums = torch.empty(rows, dtype=torch.int32, device=codes.device)
+        nat.check(nat.lib().ic_row_sums_i8(data, rows, K, data.shape[1], sums, nat.stream()), "ic_row_sums_i8")
+        return cls(data, scales, sums, K, lead)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """The int8 codes [*lead, in_features] (a view for 2-D activations)."""
+        c = self.data[:, : self.in_features]
+        return c if len(self.lead) == 1 else c.reshape(*self.lead, self.in_features)
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values ``q * s`` [*lead, in_features], rounded once to ``dtype``."""
+        K, data = self.in_features, self.data
+        out = torch.empty((*self.lead, K), dtype=dtype, device=data.device)
+        code = nat.dtype_code(out)
+        nat.check(nat.lib().ic_dequantize_rows(data.data_ptr(), data.shape[0], K, data.shape[1],
+                                               self.scales.data_ptr(), out.data_ptr(), code, K, nat.stream()),
+                  "ic_dequantize_rows")
+        return out
+
+
+def _quantize(x, weight, residual, eps, rot_size):
+    if rot_size not in ROT_SIZES and rot_size != 0:
+        raise ValueError(f"rot_size must be 0 or one of {ROT_SIZES}, got {rot_size}: rotate_activations serves others")
+    if x.dim() < 1:
+        raise ValueError("expected activations [..., K]")
+    lead, K = x.shape[:-1], x.shape[-1]
+    rot = rot_size or 1
+    Kp = -(-K // rot) * rot
+    if not 1 <= K or Kp > MAX_FEATURES:
+        raise ValueError(f"in_features (padded to the rotation) must be in [1, {MAX_FEATURES}], got {K}")
+    xg = check_gpu("x", x)
+    code = nat.dtype_code(xg)
+    dev, rows = xg.device, x.numel() // K
+    xr = as_rows(xg) if rows else xg.reshape(0, K)
+    rr = out = w = None
+    wcode = code
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} does not match x {tuple(x.shape)} {x.dtype}")
+        rg = check_gpu("residual", residual)
+        rr = as_rows(rg) if rows else rg.reshape(0, K)
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if weight is not None:
+        if weight.shape != (K,):
+            raise ValueError(f"the norm's weight has shape {tuple(weight.shape)}, expected ({K},)")
+        w = check_gpu("weight", weight)
+        if w.dtype != x.dtype:
+            if w.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+                raise TypeError(f"unsupported dtype {w.dtype}")
+            w, wcode = w.float(), nat.DT_F32
+        w = w.contiguous()
+    pitch = -(-Kp // _PAD) * _PAD
+    data = torch.empty((rows, pitch), dtype=torch.int8, device=dev)
+    scales = torch.empty(rows, dtype=torch.float32, device=dev)
+    sums = torch.empty(rows, dtype=torch.int32, device=dev)
+    ld = lambda t: t.stride(0) if rows > 1 else K                # noqa: E731
+    nat.check(nat.lib().ic_quantize_rows(
+        xr.data_ptr(), code, rows, K, ld(xr), None if rr is None else rr.data_ptr(), 0 if rr is None else ld(rr),
+        None if w is None else w.data_ptr(), wcode, eps, rot, data.data_ptr(), pitch, scales.data_ptr(),
+        sums.data_ptr(), None if out is None else out.data_ptr(), K, nat.stream()), "ic_quantize_rows")
+    if out is not None and x.device.type != "cuda":
+        out = out.to(x.device)
+    return QuantizedActivations(data, scales, sums, Kp, lead), out
+
+
+def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
+                      eps: float = 1e-6, rot_size: int = 0) -> tuple[QuantizedActivations, torch.Tensor | None]:
+    """``h = x + residual``; 8-bit codes of ``rotate(h * rsqrt(mean(h^2) + eps) * weight)``.
+
+    x: [..., K] float32 / bfloat16 / float16; residual: like x or None; weight: [K].  rot_size: 0 (none), 4, 16, 64
+    or 256, the size the weights were rotated with; rows are zero-padded to a multiple of it.  Returns the activations
+    and ``h`` in x's dtype (None without a residual).  The norm sees the fp32 sum, not its rounding.  A row that
+    holds Inf or NaN gets the scale NaN and codes 0, and leaves the other rows as they are."""
+    if weight is None:
+        raise ValueError("rms_norm_quantize needs the norm's weight; quantize_activations is the form without a norm")
+    return _quantize(x, weight, residual, float(eps), rot_size)
+
+
+def quantize_activations(x: torch.Tensor, *, rot_size: int = 0) -> QuantizedActivations:
+    """8-bit codes of the (rotated) rows of x [..., K], as rms_norm_quantize without residual and norm."""
+    return _quantize(x, None, None, 0.0, rot_size)[0]

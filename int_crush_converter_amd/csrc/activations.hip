@@ -1,0 +1,304 @@
+// 8-bit activations for a quantised layer: residual addition, root-mean-square
+// norm, group-wise Hadamard rotation and quantisation of a row in one pass.
+//
+//   h = x + r,  y = h rsqrt(mean(h^2) + eps) g,  z = R pad(y),
+//   s = max(|z|_max, 1e-30) / 127,  q = clamp(rhaz(z / s), -127, 127)
+//
+// A row stays in registers from its load to its codes, so HBM sees each
+// input and each output once.
+#include "common.hpp"
+#include "prof.hpp"
+#include "lowbit.hpp"
+
+namespace icq {
+namespace {
+
+constexpr float kTinyMax = 1e-30f;   // the smallest row maximum that a scale stands for
+
+__device__ __forceinline__ void bfly4(float& a, float& b, float& c, float& d) {
+    const float s = (a + b) + (c + d);
+    const float na = __builtin_fmaf(s, 0.5f, -d), nb = __builtin_fmaf(s, 0.5f, -c);
+    const float nc = __builtin_fmaf(s, 0.5f, -b), nd = __builtin_fmaf(s, 0.5f, -a);
+    a = na; b = nb; c = nc; d = nd;
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dppf(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kXor3 = 0x1B;     // quad permutations
+constexpr int kRor4 = 0x124, kRor8 = 0x128;                 // rotations within 16 lanes
+constexpr int kMirror = 0x140;                              // lane i -> 15 - i within 16 lanes
+
+// One base-4 digit across the lanes of a quad, and one across lane bits 2, 3
+// of a row of 16: y_d = S / 2 - x_(3 - d).
+__device__ __forceinline__ float digit_quad(float v) {
+    const float a = v + dppf<kXor1>(v);
+    return __builtin_fmaf(a + dppf<kXor2>(a), 0.5f, -dppf<kXor3>(v));
+}
+__device__ __forceinline__ float digit_row16(float v) {
+    const float a = v + dppf<kRor8>(v);          // lanes i, i ^ 8
+    const float s = a + dppf<kRor4>(a);          // a has period 8: a rotation by 4 is i ^ 4
+    return __builtin_fmaf(s, 0.5f, -dppf<kXor3>(dppf<kMirror>(v)));   // i ^ 15 ^ 3 = i ^ 12
+}
+
+// R of order rot in {4, 16, 64, 256} on chunks of 16 consecutive columns, 16
+// consecutive lanes holding 256 columns.
+__device__ __forceinline__ void rotate16(float (&v)[16], int rot) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) bfly4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    if (rot >= 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bfly4(v[i], v[i + 4], v[i + 8], v[i + 12]);
+    }
+    if (rot >= 64) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = digit_quad(v[i]);
+    }
+    if (rot >= 256) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = digit_row16(v[i]);
+    }
+}
+
+template <int WAVES, typename T, typename F>
+__device__ __forceinline__ T row_reduce(T v, T* lds, F op) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+    if (WAVES > 1) {
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) lds[w] = v;
+        __syncthreads();
+        v = lds[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) v = op(v, lds[i]);
+        __syncthreads();
+    }
+    return v;
+}
+
+// WAVES waves hold one row, NC chunks of 16 columns a lane; for WAVES = 1 a
+// work-group of 4 waves holds 4 rows.
+template <int DT, int WAVES, int NC, bool FAST>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_kernel(
+    const void* __restrict__ x, int64_t rows, int64_t cols, int64_t ld_x, const void* residual, int64_t ld_r,
+    const void* __restrict__ weight, int weight_f32, float eps, int rot, int8_t* __restrict__ codes,
+    int64_t ld_q, float* __restrict__ scales, int32_t* __restrict__ sums, void* residual_out,
+    int64_t ld_ro) {
+    __shared__ float red_f[WAVES];
+    __shared__ unsigned red_u[WAVES];
+    __shared__ int red_i[WAVES];
+    const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= rows) return;
+    constexpr int SPAN = 64 * WAVES * 16;
+
+    float v[NC][16];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) load16<DT, FAST>(x, row * ld_x, c * SPAN + lane * 16, cols, v[c]);
+    if (residual) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float r[16];
+            load16<DT, FAST>(residual, row * ld_r, c * SPAN + lane * 16, cols, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[c][i] += r[i];
+            store16<DT, FAST>(residual_out, row * ld_ro, c * SPAN + lane * 16, cols, v[c]);
+        }
+    }
+    if (weight) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ss = __builtin_fmaf(v[c][i], v[c][i], ss);
+        ss = row_reduce<WAVES>(ss, red_f, [](float a, float b) { return a + b; });
+        const float rs = 1.0f / sqrtf(ss / (float)cols + eps);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float g[16];
+            if (weight_f32) load16<IC_DTYPE_F32, FAST>(weight, 0, c * SPAN + lane * 16, cols, g);
+            else load16<DT, FAST>(weight, 0, c * SPAN + lane * 16, cols, g);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * rs * g[i];
+        }
+    }
+    if (rot > 1) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) rotate16(v[c], rot);
+    }
+    // the maximum of the magnitudes' bits: Inf and NaN compare above every finite value
+    unsigned top = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[c][i]) & 0x7fffffffu);
+    top = row_reduce<WAVES>(top, red_u, [](unsigned a, unsigned b) { return max(a, b); });
+    const bool bad = top >= 0x7f800000u;
+    const float peak = bad ? 1.0f : fmaxf(__uint_as_float(top), kTinyMax);
+    const float inv = bad ? 0.0f : 127.0f / peak;
+    int sum = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int64_t c0 = c * SPAN + lane * 16;
+        lb_u32x4 word;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            unsigned p = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float z = bad ? 0.0f : v[c][4 * w + k] * inv;
+                const int q = (int)__builtin_amdgcn_fmed3f(rhaz_trunc(z), -127.0f, 127.0f);
+                p |= (unsigned)(q & 255) << (8 * k);
+            }
+            word[w] = p;
+            sum = __builtin_amdgcn_sdot4(p, 0x01010101, sum, false);
+        }
+        if (c0 < ld_q) *reinterpret_cast<lb_u32x4*>(codes + row * ld_q + c0) = word;
+    }
+    sum = row_reduce<WAVES>(sum, red_i, [](int a, int b) { return a + b; });
+    if (lane == 0) {
+        scales[row] = bad ? __uint_as_float(0x7fc00000u) : peak / 127.0f;
+        sums[row] = sum;
+    }
+}
+
+// q * s back as values: one lane per 16 codes.
+template <int DT>
+__global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* __restrict__ codes, int64_t rows,
+                                                              int64_t cols, int64_t ld_q,
+                                                              const float* __restrict__ scales, void* __restrict__ out,
+                                                              int64_t ld_out, bool fast) {
+    const int64_t upr = cdiv(cols, 16), total = rows * upr, stride = (int64_t)gridDim.x * 256;
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += stride) {
+        const int64_t r = u / upr, c0 = (u - r * upr) * 16;
+        const lb_u32x4 w = *reinterpret_cast<const lb_u32x4*>(codes + r * ld_q + c0);
+        const float s = scales[r];
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * s;
+        if (fast) store16<DT, true>(out, r * ld_out, c0, cols, v);
+        else store16<DT, false>(out, r * ld_out, c0, cols, v);
+    }
+}
+
+// Row sums of 8-bit codes: one wave a row.
+__global__ __launch_bounds__(256) void row_sums_kernel(const int8_t* __restrict__ codes, int64_t rows, int64_t cols,
+                                                       int64_t ld_q, int32_t* __restrict__ sums) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    int sum = 0;
+    for (int64_t c = threadIdx.x & 63; c < cols; c += 64) sum += codes[row * ld_q + c];
+    sum = wave_sum(sum);
+    if ((threadIdx.x & 63) == 0) sums[row] = sum;
+}
+
+struct RowArgs {
+    const void* x; int64_t rows, cols, ld_x; const void* residual; int64_t ld_r; const void* weight;
+    int weight_f32; float eps; int rot; int8_t* codes; int64_t ld_q; float* scales; int32_t* sums; void* residual_out;
+    int64_t ld_ro; hipStream_t st;
+};
+
+template <int DT, int WAVES, int NC>
+void launch_rows(const RowArgs& a, bool fast) {
+    const dim3 grid((unsigned)(WAVES == 1 ? cdiv(a.rows, 4) : a.rows)), block(WAVES == 1 ? 256 : 64 * WAVES);
+    if (fast)
+        hipLaunchKernelGGL((quantize_rows_kernel<DT, WAVES, NC, true>), grid, block, 0, a.st, a.x, a.rows, a.cols,
+                           a.ld_x, a.residual, a.ld_r, a.weight, a.weight_f32, a.eps, a.rot, a.codes, a.ld_q, a.scales,
+                           a.sums, a.residual_out, a.ld_ro);
+    else
+        hipLaunchKernelGGL((quantize_rows_kernel<DT, WAVES, NC, false>), grid, block, 0, a.st, a.x, a.rows, a.cols,
+                           a.ld_x, a.residual, a.ld_r, a.weight, a.weight_f32, a.eps, a.rot, a.codes, a.ld_q, a.scales,
+                           a.sums, a.residual_out, a.ld_ro);
+}
+
+template <int DT, int WAVES>
+void launch_chunks(const RowArgs& a, bool fast) {
+    const int64_t nc = cdiv(a.ld_q, (int64_t)64 * WAVES * 16);
+    if (nc <= 1) launch_rows<DT, WAVES, 1>(a, fast);
+    else if (nc <= 2) launch_rows<DT, WAVES, 2>(a, fast);
+    else if (nc <= 3) launch_rows<DT, WAVES, 3>(a, fast);
+    else launch_rows<DT, WAVES, 4>(a, fast);
+}
+
+template <int DT>
+void launch_waves(const RowArgs& a, bool fast) {
+    if (a.ld_q <= 1024) launch_chunks<DT, 1>(a, fast);
+    else if (a.ld_q <= 16384) launch_chunks<DT, 4>(a, fast);
+    else launch_chunks<DT, 16>(a, fast);
+}
+
+}  // namespace
+}  // namespace icq
+
+using namespace icq;
+
+extern "C" int64_t ic_activation_pitch(int64_t cols) { return cols < 0 ? 0 : cdiv(cols, kActPad) * kActPad; }
+
+extern "C" int ic_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld_x,
+                                const void* residual, int64_t ld_r, const void* weight, int weight_dtype,
+                                float eps, int rot, int8_t* codes, int64_t ld_q, float* scales, int32_t* sums, void* residual_out,
+                                int64_t ld_ro, void* stream) {
+    IC_REQUIRE(rows >= 0 && cols >= 1, "ic_quantize_rows: rows must be >= 0 and cols >= 1");
+    IC_REQUIRE(dtype >= 0 && dtype <= 2, "ic_quantize_rows: unknown dtype");
+    IC_REQUIRE(!weight || weight_dtype == dtype || weight_dtype == IC_DTYPE_F32,
+               "ic_quantize_rows: the norm's weight is of x's dtype or fp32");
+    IC_REQUIRE(rot == 1 || rot == 4 || rot == 16 || rot == 64 || rot == 256,
+               "ic_quantize_rows: rot must be 1, 4, 16, 64 or 256");
+    if (rows == 0) return IC_OK;
+    IC_REQUIRE(x && codes && scales && sums, "ic_quantize_rows: null pointer");
+    IC_REQUIRE(!residual == !residual_out, "ic_quantize_rows: residual and residual_out go together");
+    const int64_t cols_pad = cdiv(cols, rot) * rot;
+    if (cols_pad > 65536 || rows > 0x7fffffff) return fail(IC_ERR_RANGE, "ic_quantize_rows: at most 65536 columns and 2^31 - 1 rows");
+    IC_REQUIRE(ld_x >= cols && (!residual || (ld_r >= cols && ld_ro >= cols)), "ic_quantize_rows: leading dimension below cols");
+    IC_REQUIRE(ld_q == ic_activation_pitch(cols_pad) && aligned16(codes),
+               "ic_quantize_rows: codes need ic_activation_pitch columns and 16-byte alignment");
+    const int64_t es = dtype == IC_DTYPE_F32 ? 4 : 2;
+    auto whole = [&](const void* p, int64_t ld) { return !p || (aligned16(p) && ld * es % 16 == 0); };
+    const bool fast = cols % 16 == 0 && whole(x, ld_x) && whole(residual, ld_r) && whole(residual_out, ld_ro) &&
+                      whole(weight, 16);
+    RowArgs a{x, rows, cols, ld_x, residual, ld_r, weight, weight && weight_dtype == IC_DTYPE_F32, eps, rot, codes, ld_q, scales, sums,
+              residual_out, ld_ro, as_stream(stream)};
+    ProfScope prof(a.st, PT_OTHER, 0.0, (double)rows * cols * (es * (residual ? 3 : 1) + 1));
+    if (dtype == IC_DTYPE_F32) launch_waves<IC_DTYPE_F32>(a, fast);
+    else if (dtype == IC_DTYPE_BF16) launch_waves<IC_DTYPE_BF16>(a, fast);
+    else launch_waves<IC_DTYPE_F16>(a, fast);
+    IC_CHECK_LAUNCH();
+    return IC_OK;
+}
+
+extern "C" int ic_dequantize_rows(const int8_t* codes, int64_t rows, int64_t cols, int64_t ld_q, const float* scales,
+                                  void* out, int dtype, int64_t ld_out, void* stream) {
+    IC_REQUIRE(rows >= 0 && cols >= 1, "ic_dequantize_rows: rows must be >= 0 and cols >= 1");
+    IC_REQUIRE(dtype >= 0 && dtype <= 2, "ic_dequantize_rows: unknown dtype");
+    if (rows == 0) return IC_OK;
+    IC_REQUIRE(codes && scales && out, "ic_dequantize_rows: null pointer");
+    IC_REQUIRE(ld_q >= cdiv(cols, 16) * 16 && ld_q % 16 == 0 && aligned16(codes) && ld_out >= cols,
+               "ic_dequantize_rows: rows of codes need a pitch of whole 16-byte words");
+    const int64_t es = dtype == IC_DTYPE_F32 ? 4 : 2;
+    const bool fast = cols % 16 == 0 && aligned16(out) && ld_out * es % 16 == 0;
+    const int64_t grid = cdiv(rows * cdiv(cols, 16), 256);
+    const dim3 g((unsigned)(grid < 65536 ? grid : 65536)), b(256);
+    hipStream_t st = as_stream(stream);
+    ProfScope prof(st, PT_OTHER, 0.0, (double)rows * cols * (es + 1));
+    if (dtype == IC_DTYPE_F32)
+        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_F32>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out, fast);
+    else if (dtype == IC_DTYPE_BF16)
+        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_BF16>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out, fast);
+    else
+        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_F16>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out, fast);
+    IC_CHECK_LAUNCH();
+    return IC_OK;
+}
+
+extern "C" int ic_row_sums_i8(const int8_t* codes, int64_t rows, int64_t cols, int64_t ld_q, int32_t* sums,
+                              void* stream) {
+    IC_REQUIRE(rows >= 0 && cols >= 1 && ld_q >= cols, "ic_row_sums_i8: bad sizes");
+    if (rows == 0) return IC_OK;
+    IC_REQUIRE(codes && sums, "ic_row_sums_i8: null pointer");
+    if (cols > 65536 || rows > 0x7fffffff) return fail(IC_ERR_RANGE, "ic_row_sums_i8: at most 65536 columns and 2^31 - 1 rows");
+    hipLaunchKernelGGL(row_sums_kernel, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, as_stream(stream), codes, rows,
+                       cols, ld_q, sums);
+    IC_CHECK_LAUNCH();
+    return IC_OK;
+}
