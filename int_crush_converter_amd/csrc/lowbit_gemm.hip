@@ -41,49 +41,82 @@ struct Operands {
 template <int KIND> struct Acc { typedef i32x4 T; };
 template <> struct Acc<kMx> { typedef lb_f32x4 T; };
 
-// y for four consecutive n from n0 of row m, from the accumulated sums.
+// What the outputs of four consecutive columns from n0 need (columns past the
+// last repeat the last).
 template <int KIND>
-__device__ __forceinline__ void finish4(const Operands& p, typename Acc<KIND>::T acc, int64_t m, int64_t n0) {
-    if (m >= p.M || n0 >= p.N) return;
-    float v[4];
-    float sa = 1.0f;
-    int sum = 0;
-    if (KIND != kMx) {
-        sa = p.sa[m];
-        if (p.zp) sum = p.sums[m];
-    }
+struct Columns {
+    float sw[4], bias[4];
+    int zp[4];
+    __device__ __forceinline__ void load(const Operands& p, int64_t n0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t n = n0 + i < p.N ? n0 + i : p.N - 1;
-        if constexpr (KIND == kMx) {
-            v[i] = acc[i];
-        } else {
-            // INT4 operands are held as 16 q; the shift is exact.  |sum_k a (q - zp)| < 2^31 for K <= 65536, so the
-            // difference is right even where a term has wrapped
-            int d = KIND == kInt4 ? acc[i] >> 4 : acc[i];
-            if (p.zp) d = (int)((unsigned)d - (unsigned)((int)p.zp[n] * sum));
-            const float sw = p.sw_f32 ? static_cast<const float*>(p.sw)[n]
-                                      : f16_bits_to_f32(static_cast<const uint16_t*>(p.sw)[n]);
-            v[i] = (float)d * (sa * sw);
+        for (int i = 0; i < 4; ++i) {
+            const int64_t n = n0 + i < p.N ? n0 + i : p.N - 1;
+            if (KIND != kMx) {
+                sw[i] = p.sw_f32 ? static_cast<const float*>(p.sw)[n] : f16_bits_to_f32(static_cast<const uint16_t*>(p.sw)[n]);
+                zp[i] = p.zp ? p.zp[n] : 0;
+            }
+            bias[i] = p.bias ? load_as_f32(p.bias, p.bias_dtype, n) : 0.0f;
         }
-        if (p.bias) v[i] += load_as_f32(p.bias, p.bias_dtype, n);
     }
-    const int64_t at = m * p.ld_out + n0;
-    if (p.wide && n0 + 4 <= p.N) {
+    // y from the accumulated sums of a row with scale sa and code sum `sum`
+    __device__ __forceinline__ lb_f32x4 finish(typename Acc<KIND>::T acc, float sa, int sum) const {
+        lb_f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (KIND == kMx) {
+                v[i] = acc[i] + bias[i];
+            } else {
+                // INT4 operands are held as 16 q; the shift is exact.  |sum_k a (q - zp)| < 2^31 for K <= 65536, so
+                // the difference is right even where a term has wrapped
+                const int d = (int)((unsigned)(KIND == kInt4 ? acc[i] >> 4 : acc[i]) - (unsigned)zp[i] * (unsigned)sum);
+                v[i] = (float)d * (sa * sw[i]) + bias[i];
+            }
+        }
+        return v;
+    }
+};
+
+// A wave's 16 rows x 64 (16 COLS) columns of y from its area of LDS: a lane
+// writes 4 COLS consecutive columns of one row, so that 4 lanes write whole
+// lines.  Rows of `area` hold 16 COLS + 4 values: 16-byte reads and writes
+// then spread over the banks.
+template <int COLS>
+__device__ __forceinline__ void store_rows(const Operands& p, const float* area, int lane, int64_t m0, int64_t n0) {
+    const int64_t m = m0 + (lane >> 2);
+    const float* row = area + (lane >> 2) * (16 * COLS + 4) + (lane & 3) * 4 * COLS;
+    const int64_t c0 = n0 + (lane & 3) * 4 * COLS;
+    if (m >= p.M || c0 >= p.N) return;
+    float v[4 * COLS];
+#pragma unroll
+    for (int i = 0; i < COLS; ++i) *reinterpret_cast<lb_f32x4*>(v + 4 * i) = *reinterpret_cast<const lb_f32x4*>(row + 4 * i);
+    const int64_t at = m * p.ld_out + c0;
+    if (p.wide && c0 + 4 * COLS <= p.N) {
         if (p.out_dtype == IC_DTYPE_F32) {
-            *reinterpret_cast<lb_f32x4*>(static_cast<float*>(p.out) + at) = lb_f32x4{v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int i = 0; i < COLS; ++i)
+                *reinterpret_cast<lb_f32x4*>(static_cast<float*>(p.out) + at + 4 * i) = lb_f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
         } else {
-            lb_u32x2 w;
-            if (p.out_dtype == IC_DTYPE_BF16)
-                w = lb_u32x2{pack_half_words<IC_DTYPE_BF16>(v[0], v[1]), pack_half_words<IC_DTYPE_BF16>(v[2], v[3])};
-            else
-                w = lb_u32x2{pack_half_words<IC_DTYPE_F16>(v[0], v[1]), pack_half_words<IC_DTYPE_F16>(v[2], v[3])};
-            *reinterpret_cast<lb_u32x2*>(static_cast<uint16_t*>(p.out) + at) = w;
+            uint32_t w[2 * COLS];
+            if (p.out_dtype == IC_DTYPE_BF16) {
+#pragma unroll
+                for (int i = 0; i < 2 * COLS; ++i) w[i] = pack_half_words<IC_DTYPE_BF16>(v[2 * i], v[2 * i + 1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2 * COLS; ++i) w[i] = pack_half_words<IC_DTYPE_F16>(v[2 * i], v[2 * i + 1]);
+            }
+            uint16_t* q = static_cast<uint16_t*>(p.out) + at;
+            if constexpr (COLS % 2 == 0) {
+#pragma unroll
+                for (int i = 0; i < COLS / 2; ++i)
+                    *reinterpret_cast<lb_u32x4*>(q + 8 * i) = lb_u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+            } else {
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) *reinterpret_cast<lb_u32x2*>(q + 4 * i) = lb_u32x2{w[2 * i], w[2 * i + 1]};
+            }
         }
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n0 + i < p.N) store_from_f32(p.out, p.out_dtype, at + i, v[i]);
+#pragma unroll 1
+        for (int i = 0; i < 4 * COLS && c0 + i < p.N; ++i) store_from_f32(p.out, p.out_dtype, at + i, row[i]);
     }
 }
 
@@ -91,10 +124,12 @@ __device__ __forceinline__ void finish4(const Operands& p, typename Acc<KIND>::T
 __device__ __forceinline__ i32x4 mma_i8(lb_u32x4 w, lb_u32x4 x, i32x4 acc) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), acc, 0, 0, 0);
 }
+// (byte B of each scale word)
+template <int B>
 __device__ __forceinline__ lb_f32x4 mma_mx(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc, int sw, int sx) {
     const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, sw, 0, sx);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, B, sw, B, sx);
 }
 // 32 INT4 values of a lane as two operands of 16 bytes, each value times 16.
 __device__ __forceinline__ lb_u32x4 low_nibbles(lb_u32x4 p) { return (p << 4) & 0xf0f0f0f0u; }
@@ -106,6 +141,7 @@ template <int KIND, int MT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
     typedef typename Acc<KIND>::T acc_t;
     __shared__ acc_t part[WAVES][MT][64];
+    __shared__ float rows[MT][16 * 20];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
     const int64_t nt = blockIdx.x, mt0 = (int64_t)blockIdx.y * MT;
     const int64_t tiles = cdiv(p.K, 128), words = cdiv(p.K, 512);
@@ -135,7 +171,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
             const int sw = (int)(ws[(t >> 2) * 64] >> (8 * (t & 3)));
 #pragma unroll
             for (int i = 0; i < MT; ++i)
-                acc[i] = mma_mx(w, xt[i][t * 64], acc[i], sw & 255, (int)(xs[i][(t >> 2) * 64] >> (8 * (t & 3))) & 255);
+                acc[i] = mma_mx<0>(w, xt[i][t * 64], acc[i], sw & 255, (int)(xs[i][(t >> 2) * 64] >> (8 * (t & 3))) & 255);
         } else {
             lb_u32x4 w0, w1;
             if (KIND == kInt8) {
@@ -157,11 +193,220 @@ __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
+    Columns<KIND> cols;
+    cols.load(p, nt * 16 + g * 4);
     for (int i = wave; i < MT; i += WAVES) {
         acc_t s = part[0][i][lane];
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) s += part[k][i][lane];
-        finish4<KIND>(p, s, (mt0 + i) * 16 + r, nt * 16 + g * 4);
+        const int64_t m = (mt0 + i) * 16 + r < p.M ? (mt0 + i) * 16 + r : p.M - 1;
+        const lb_f32x4 v = cols.finish(s, KIND == kMx ? 1.0f : p.sa[m], KIND != kMx && p.zp ? p.sums[m] : 0);
+        float* area = rows[i];
+        *reinterpret_cast<lb_f32x4*>(area + r * 20 + g * 4) = v;
+        lds_wave_fence();
+        store_rows<1>(p, area, lane, (mt0 + i) * 16, nt * 16);
+    }
+}
+
+// Copies 16 bytes a lane from global memory straight to LDS: lane i's bytes
+// land at dst + 16 i.
+__device__ __forceinline__ void load_to_lds(const void* src, void* dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+
+// Waits until at most N of this wave's global loads (copies to LDS among
+// them) are outstanding and all its LDS reads are done, then meets the other
+// waves of the work-group.  (A fence before a plain barrier would wait for
+// every copy in flight.)
+template <int N>
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Many rows: a work-group of WM x WN waves takes WM FM 16 rows of y and
+// WN FN 16 columns, each wave FM x FN instruction tiles.  K advances by 128
+// columns a step through BUF buffers in LDS, filled straight from global
+// memory BUF - 1 steps ahead.
+template <int KIND, int WM, int WN, int FM, int FN, int BUF>
+__global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
+    typedef typename Acc<KIND>::T acc_t;
+    constexpr int WAVES = WM * WN, BM = WM * FM * 16, BN = WN * FN * 16;
+    constexpr int X_KB = BM / 16 * (KIND == kMx ? 1 : 2), W_KB = BN / 16 * (KIND == kInt8 ? 2 : 1);   // a stage's KB
+    constexpr int LOADS = (X_KB + W_KB) / WAVES;
+    static_assert((X_KB + W_KB) % WAVES == 0 && X_KB % WAVES == 0, "each wave copies the same number of KB");
+    __shared__ lb_u32x4 lds[BUF][(X_KB + W_KB) * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    const int wm = wave / WN, wn = wave % WN;
+
+    // work-groups are dealt to the 8 XCDs in turn: give each XCD one run of tiles, and walk a run in blocks of
+    // 8 tile rows so that what its L2 holds is used again
+    const int total = grid_m * grid_n, per = total / 8, extra = total % 8, xcd = blockIdx.x % 8;
+    const int id = xcd * per + (xcd < extra ? xcd : extra) + blockIdx.x / 8;
+    const int band = id / (8 * grid_n), rows_in = grid_m - band * 8 < 8 ? grid_m - band * 8 : 8;
+    const int in_band = id - band * 8 * grid_n;
+    const int bm = band * 8 + in_band % rows_in, bn = in_band / rows_in;
+
+    const int64_t tiles = cdiv(p.K, 128), words = cdiv(p.K, 512);
+    const int64_t n_tiles = cdiv(p.N, 16), m_tiles = cdiv(p.M, 16);
+
+    // where this wave's copies come from; rows and tiles past the last repeat the last, and are dropped at the end
+    const uint8_t* src[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int kb = i * WAVES + wave;
+        if (kb < X_KB) {
+            if (KIND == kMx) {
+                const int64_t mt = (int64_t)bm * (BM / 16) + kb;
+                src[i] = p.a + (mt < m_tiles ? mt : m_tiles - 1) * tiles * 1024 + lane * 16;
+            } else {
+                // 8 rows of 128 bytes; 16-byte chunk c of row r lies in slot c ^ (r & 7), so that 8 lanes reading
+                // one chunk of 8 rows touch 8 different groups of banks
+                const int64_t m = (int64_t)bm * BM + kb * 8 + (lane >> 3);
+                src[i] = p.a + (m < p.M ? m : p.M - 1) * p.ld_a + ((lane & 7) ^ (lane >> 3)) * 16;
+            }
+        } else {
+            const int64_t nt = (int64_t)bn * (BN / 16) + (KIND == kInt8 ? (kb - X_KB) / 2 : kb - X_KB);
+            src[i] = p.w + ((nt < n_tiles ? nt : n_tiles - 1) * tiles * (KIND == kInt8 ? 2 : 1) +
+                            (KIND == kInt8 ? (kb - X_KB) % 2 : 0)) * 1024 + lane * 16;
+        }
+    }
+    auto fetch = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            load_to_lds(src[i], &lds[buf][(i * WAVES + wave) * 64]);
+            src[i] += i * WAVES < X_KB ? (KIND == kMx ? 1024 : 128) : (KIND == kInt8 ? 2048 : 1024);
+        }
+    };
+
+    acc_t acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+
+    // the scale words of four steps, BM / 16 + BN / 16 tiles of 256 bytes: 16 lanes copy a tile's
+    constexpr int S_TILES = (BM + BN) / 16, S_WAVES = S_TILES / 4;
+    static_assert(KIND != kMx || (BM % 64 == 0 && BN % 64 == 0 && S_WAVES <= WAVES), "a wave copies the scales of four tiles");
+    __shared__ uint32_t lds_s[KIND == kMx ? 2 : 1][KIND == kMx ? S_TILES * 64 : 1];
+    const uint32_t* s_src = nullptr;
+    if (KIND == kMx && wave < S_WAVES) {
+        const int tile = wave * 4 + (lane >> 4);
+        if (tile < BM / 16) {
+            const int64_t mt = (int64_t)bm * (BM / 16) + tile;
+            s_src = p.a_scale + (mt < m_tiles ? mt : m_tiles - 1) * words * 64 + (lane & 15) * 4;
+        } else {
+            const int64_t nt = (int64_t)bn * (BN / 16) + tile - BM / 16;
+            s_src = p.w_scale + (nt < n_tiles ? nt : n_tiles - 1) * words * 64 + (lane & 15) * 4;
+        }
+    }
+    auto fetch_scales = [&](int half) {
+        if (KIND == kMx && wave < S_WAVES) {
+            load_to_lds(s_src, &lds_s[half][wave * 256]);
+            s_src += 64;
+        }
+    };
+    int xs[KIND == kMx ? FM : 1], ws[KIND == kMx ? FN : 1];
+    auto read_scales = [&](int half) {
+        if constexpr (KIND == kMx) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i) xs[i] = (int)lds_s[half][(wm * FM + i) * 64 + lane];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) ws[j] = (int)lds_s[half][(BM / 16 + wn * FN + j) * 64 + lane];
+        }
+    };
+
+    auto step = [&](const lb_u32x4* s, auto byte) {
+        constexpr int B = decltype(byte)::value;
+        const lb_u32x4* x = s + wm * FM * (KIND == kMx ? 64 : 128);
+        const lb_u32x4* w = s + X_KB * 64 + wn * FN * (KIND == kInt8 ? 128 : 64) + lane;
+        if constexpr (KIND == kMx) {
+            lb_u32x4 wv[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) wv[j] = w[j * 64];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const lb_u32x4 xv = x[i * 64 + lane];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma_mx<B>(wv[j], xv, acc[i][j], ws[j], xs[i]);
+            }
+        } else {
+            lb_u32x4 wv[2][FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                if (KIND == kInt4) {
+                    const lb_u32x4 q = w[j * 64];
+                    wv[0][j] = low_nibbles(q);
+                    wv[1][j] = high_nibbles(q);
+                } else {
+                    wv[0][j] = w[j * 128];
+                    wv[1][j] = w[j * 128 + 64];
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+                    const lb_u32x4 xv = x[(i * 16 + r) * 8 + ((h * 4 + g) ^ (r & 7))];
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = mma_i8(wv[h][j], xv, acc[i][j]);
+                }
+        }
+    };
+
+    // one step: wait for this wave's own copies of it, meet the others (whose copies have then landed too, and who
+    // are done with the buffer of the step before), fill that buffer, multiply.  The scales of four steps are copied
+    // just before the first of them, into the half that the last four did not use.
+    const int steps = (int)tiles;
+    auto turn = [&](int t, int buf, int half, auto byte) {
+        constexpr int B = decltype(byte)::value;
+        if (t + BUF - 2 < steps) meet<LOADS * (BUF - 2)>();
+        else meet<0>();
+        if (t + BUF - 1 < steps) {
+            if (KIND == kMx && B == 1) fetch_scales(half ^ 1);         // (of step t + 3, the first of its word)
+            fetch((buf + BUF - 1) % BUF);
+        }
+        if (KIND == kMx && B == 0) read_scales(half);
+        step(lds[buf], byte);
+    };
+    if (KIND == kMx) fetch_scales(0);
+#pragma unroll
+    for (int b = 0; b < BUF - 1; ++b)
+        if (b < steps) fetch(b);
+    if constexpr (KIND == kMx) {
+        static_assert(KIND != kMx || BUF == 4, "a word of scales holds four steps");
+        for (int t = 0, half = 0; t < steps; t += 4, half ^= 1) {
+            turn(t, 0, half, std::integral_constant<int, 0>{});
+            if (t + 1 < steps) turn(t + 1, 1, half, std::integral_constant<int, 1>{});
+            if (t + 2 < steps) turn(t + 2, 2, half, std::integral_constant<int, 2>{});
+            if (t + 3 < steps) turn(t + 3, 3, half, std::integral_constant<int, 3>{});
+        }
+    } else {
+        for (int t = 0; t < steps; t += BUF) {
+#pragma unroll
+            for (int b = 0; b < BUF; ++b)
+                if (t + b < steps) turn(t + b, b, 0, std::integral_constant<int, 0>{});
+        }
+    }
+    static_assert(FN == 2 || FN == 4, "store_rows takes 32 or 64 columns");
+    static_assert(sizeof(lds) >= WAVES * 16 * (16 * FN + 4) * 4, "the areas of the epilogue lie in the buffers");
+    Columns<KIND> cols[FN];
+    const int64_t m0 = (int64_t)bm * BM + wm * FM * 16, n0 = (int64_t)bn * BN + wn * FN * 16;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) cols[j].load(p, n0 + j * 16 + g * 4);
+    meet<0>();                                               // the buffers are free
+    float* area = reinterpret_cast<float*>(&lds[0][0]) + wave * 16 * (16 * FN + 4);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int64_t m = m0 + i * 16 + r < p.M ? m0 + i * 16 + r : p.M - 1;
+        const float sa = KIND == kMx ? 1.0f : p.sa[m];
+        const int sum = KIND != kMx && p.zp ? p.sums[m] : 0;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            *reinterpret_cast<lb_f32x4*>(area + r * (16 * FN + 4) + j * 16 + g * 4) = cols[j].finish(acc[i][j], sa, sum);
+        lds_wave_fence();
+        store_rows<FN>(p, area, lane, m0 + i * 16, n0);
+        lds_wave_fence();
     }
 }
 
@@ -198,11 +443,18 @@ void launch_direct(const Operands& p, hipStream_t st) {
     hipLaunchKernelGGL((linear_direct_kernel<KIND, MT, WAVES>), grid, dim3(64 * WAVES), 0, st, p);
 }
 
+template <int KIND, int WM, int WN, int FM, int FN, int BUF>
+void launch_tiled(const Operands& p, hipStream_t st) {
+    const int gm = (int)cdiv(p.M, WM * FM * 16), gn = (int)cdiv(p.N, WN * FN * 16);
+    hipLaunchKernelGGL((linear_tiled_kernel<KIND, WM, WN, FM, FN, BUF>), dim3((unsigned)gm * gn), dim3(64 * WM * WN), 0, st, p, gm, gn);
+}
+
 template <int KIND>
 int launch_linear(const Operands& p, hipStream_t st) {
     if (p.M <= 16) launch_direct<KIND, 1, 8>(p, st);
     else if (p.M <= 32) launch_direct<KIND, 2, 8>(p, st);
-    else launch_direct<KIND, 4, 8>(p, st);
+    else if (p.M <= 64) launch_direct<KIND, 4, 8>(p, st);
+    else launch_tiled<KIND, 2, 4, 8, 4, KIND == kMx ? 4 : KIND == kInt4 ? 3 : 2>(p, st);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
