@@ -35,7 +35,7 @@ struct Operands {
     void* out;
     int out_dtype;
     int64_t ld_out;
-    int wide;                // four outputs may be stored at once
+    int wide;                // rows of out are 16-byte aligned and whole groups of 8 values
 };
 
 template <int KIND> struct Acc { typedef i32x4 T; };
@@ -76,47 +76,39 @@ struct Columns {
     }
 };
 
-// A wave's 16 rows x 64 (16 COLS) columns of y from its area of LDS: a lane
-// writes 4 COLS consecutive columns of one row, so that 4 lanes write whole
-// lines.  Rows of `area` hold 16 COLS + 4 values: 16-byte reads and writes
-// then spread over the banks.
-template <int COLS>
-__device__ __forceinline__ void store_rows(const Operands& p, const float* area, int lane, int64_t m0, int64_t n0) {
-    const int64_t m = m0 + (lane >> 2);
-    const float* row = area + (lane >> 2) * (16 * COLS + 4) + (lane & 3) * 4 * COLS;
-    const int64_t c0 = n0 + (lane & 3) * 4 * COLS;
-    if (m >= p.M || c0 >= p.N) return;
-    float v[4 * COLS];
-#pragma unroll
-    for (int i = 0; i < COLS; ++i) *reinterpret_cast<lb_f32x4*>(v + 4 * i) = *reinterpret_cast<const lb_f32x4*>(row + 4 * i);
-    const int64_t at = m * p.ld_out + c0;
-    if (p.wide && c0 + 4 * COLS <= p.N) {
-        if (p.out_dtype == IC_DTYPE_F32) {
-#pragma unroll
-            for (int i = 0; i < COLS; ++i)
-                *reinterpret_cast<lb_f32x4*>(static_cast<float*>(p.out) + at + 4 * i) = lb_f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-        } else {
-            uint32_t w[2 * COLS];
-            if (p.out_dtype == IC_DTYPE_BF16) {
-#pragma unroll
-                for (int i = 0; i < 2 * COLS; ++i) w[i] = pack_half_words<IC_DTYPE_BF16>(v[2 * i], v[2 * i + 1]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2 * COLS; ++i) w[i] = pack_half_words<IC_DTYPE_F16>(v[2 * i], v[2 * i + 1]);
-            }
-            uint16_t* q = static_cast<uint16_t*>(p.out) + at;
-            if constexpr (COLS % 2 == 0) {
-#pragma unroll
-                for (int i = 0; i < COLS / 2; ++i)
-                    *reinterpret_cast<lb_u32x4*>(q + 8 * i) = lb_u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
-            } else {
-#pragma unroll
-                for (int i = 0; i < COLS; ++i) *reinterpret_cast<lb_u32x2*>(q + 4 * i) = lb_u32x2{w[2 * i], w[2 * i + 1]};
-            }
-        }
+// Eight consecutive outputs at element `at` of out, 16-byte aligned.
+__device__ __forceinline__ void store8(const Operands& p, lb_f32x4 a, lb_f32x4 b, int64_t at) {
+    if (p.out_dtype == IC_DTYPE_F32) {
+        *reinterpret_cast<lb_f32x4*>(static_cast<float*>(p.out) + at) = a;
+        *reinterpret_cast<lb_f32x4*>(static_cast<float*>(p.out) + at + 4) = b;
     } else {
-#pragma unroll 1
-        for (int i = 0; i < 4 * COLS && c0 + i < p.N; ++i) store_from_f32(p.out, p.out_dtype, at + i, row[i]);
+        lb_u32x4 w;
+        if (p.out_dtype == IC_DTYPE_BF16)
+            w = lb_u32x4{pack_half_words<IC_DTYPE_BF16>(a[0], a[1]), pack_half_words<IC_DTYPE_BF16>(a[2], a[3]),
+                         pack_half_words<IC_DTYPE_BF16>(b[0], b[1]), pack_half_words<IC_DTYPE_BF16>(b[2], b[3])};
+        else
+            w = lb_u32x4{pack_half_words<IC_DTYPE_F16>(a[0], a[1]), pack_half_words<IC_DTYPE_F16>(a[2], a[3]),
+                         pack_half_words<IC_DTYPE_F16>(b[0], b[1]), pack_half_words<IC_DTYPE_F16>(b[2], b[3])};
+        *reinterpret_cast<lb_u32x4*>(static_cast<uint16_t*>(p.out) + at) = w;
+    }
+}
+// Four consecutive outputs of row m from column n.
+__device__ __forceinline__ void store4(const Operands& p, lb_f32x4 v, int64_t m, int64_t n) {
+    if (m >= p.M || n >= p.N) return;
+    const int64_t at = m * p.ld_out + n;
+    if (p.wide && n + 4 <= p.N) {
+        if (p.out_dtype == IC_DTYPE_F32)
+            *reinterpret_cast<lb_f32x4*>(static_cast<float*>(p.out) + at) = v;
+        else if (p.out_dtype == IC_DTYPE_BF16)
+            *reinterpret_cast<lb_u32x2*>(static_cast<uint16_t*>(p.out) + at) =
+                lb_u32x2{pack_half_words<IC_DTYPE_BF16>(v[0], v[1]), pack_half_words<IC_DTYPE_BF16>(v[2], v[3])};
+        else
+            *reinterpret_cast<lb_u32x2*>(static_cast<uint16_t*>(p.out) + at) =
+                lb_u32x2{pack_half_words<IC_DTYPE_F16>(v[0], v[1]), pack_half_words<IC_DTYPE_F16>(v[2], v[3])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < p.N) store_from_f32(p.out, p.out_dtype, at + i, v[i]);
     }
 }
 
@@ -131,6 +123,22 @@ __device__ __forceinline__ lb_f32x4 mma_mx(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc,
     const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, B, sw, B, sx);
 }
+// The same products of 32 rows and 32 columns, with twice the operations an
+// instruction (a wave alone on its SIMD reaches 4.7 POP/s and 8.9 PFLOP/s with
+// these over the card, 2.9 and 5.1 with the smaller ones).
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <int KIND> struct Acc32 { typedef i32x16 T; };
+template <> struct Acc32<kMx> { typedef f32x16 T; };
+__device__ __forceinline__ i32x16 mma32_i8(lb_u32x4 w, lb_u32x4 x, i32x16 acc) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), acc, 0, 0, 0);
+}
+template <int B>
+__device__ __forceinline__ f32x16 mma32_mx(lb_u32x4 w, lb_u32x4 x, f32x16 acc, int sw, int sx) {
+    const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, 4, B, sw, B, sx);
+}
 // 32 INT4 values of a lane as two operands of 16 bytes, each value times 16.
 __device__ __forceinline__ lb_u32x4 low_nibbles(lb_u32x4 p) { return (p << 4) & 0xf0f0f0f0u; }
 __device__ __forceinline__ lb_u32x4 high_nibbles(lb_u32x4 p) { return p & 0xf0f0f0f0u; }
@@ -141,7 +149,6 @@ template <int KIND, int MT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
     typedef typename Acc<KIND>::T acc_t;
     __shared__ acc_t part[WAVES][MT][64];
-    __shared__ float rows[MT][16 * 20];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
     const int64_t nt = blockIdx.x, mt0 = (int64_t)blockIdx.y * MT;
     const int64_t tiles = cdiv(p.K, 128), words = cdiv(p.K, 512);
@@ -200,19 +207,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) s += part[k][i][lane];
         const int64_t m = (mt0 + i) * 16 + r < p.M ? (mt0 + i) * 16 + r : p.M - 1;
-        const lb_f32x4 v = cols.finish(s, KIND == kMx ? 1.0f : p.sa[m], KIND != kMx && p.zp ? p.sums[m] : 0);
-        float* area = rows[i];
-        *reinterpret_cast<lb_f32x4*>(area + r * 20 + g * 4) = v;
-        lds_wave_fence();
-        store_rows<1>(p, area, lane, (mt0 + i) * 16, nt * 16);
+        store4(p, cols.finish(s, KIND == kMx ? 1.0f : p.sa[m], KIND != kMx && p.zp ? p.sums[m] : 0), (mt0 + i) * 16 + r,
+               nt * 16 + g * 4);
     }
-}
-
-// Copies 16 bytes a lane from global memory straight to LDS: lane i's bytes
-// land at dst + 16 i.
-__device__ __forceinline__ void load_to_lds(const void* src, void* dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
 // Waits until at most N of this wave's global loads (copies to LDS among
@@ -224,189 +221,398 @@ __device__ __forceinline__ void meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// Many rows: a work-group of WM x WN waves takes WM FM 16 rows of y and
-// WN FN 16 columns, each wave FM x FN instruction tiles.  K advances by 128
-// columns a step through BUF buffers in LDS, filled straight from global
-// memory BUF - 1 steps ahead.
+// Many rows.  A work-group of WM x WN waves takes tiles of y of 32 WM FM rows
+// and 32 WN FN columns one after another, a wave FM x FN blocks of 32 x 32 of
+// each.  K advances in stages (128 columns of 4-bit weights, 64 of INT8)
+// through BUF buffers in LDS that are filled straight from global memory,
+// BUF - 1 stages ahead of the products; a tile's first stages are on their way
+// while the outputs of the tile before are stored.  Operands go from LDS to
+// registers one set (32 bytes of each row) ahead of their products, between
+// matrix instructions, so a wave waits neither for LDS nor long at the one
+// barrier that a stage has: when it gets there, what is left of the stage is
+// in registers, and its buffer is filled again.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
-    typedef typename Acc<KIND>::T acc_t;
-    constexpr int WAVES = WM * WN, BM = WM * FM * 16, BN = WN * FN * 16;
-    constexpr int X_KB = BM / 16 * (KIND == kMx ? 1 : 2), W_KB = BN / 16 * (KIND == kInt8 ? 2 : 1);   // a stage's KB
-    constexpr int LOADS = (X_KB + W_KB) / WAVES;
-    static_assert((X_KB + W_KB) % WAVES == 0 && X_KB % WAVES == 0, "each wave copies the same number of KB");
-    __shared__ lb_u32x4 lds[BUF][(X_KB + W_KB) * 64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    typedef typename Acc32<KIND>::T acc_t;
+    constexpr int WAVES = WM * WN, BM = 32 * WM * FM, BN = 32 * WN * FN;
+    constexpr int X_KB = BM / 16 * (KIND == kInt4 ? 2 : 1), W_KB = BN / 16;      // a stage's KB
+    constexpr int X_LOADS = X_KB / WAVES, W_LOADS = W_KB / WAVES, LOADS = X_LOADS + W_LOADS;   // a wave's copies of 1 KB a stage
+    constexpr int STAGE = (X_KB + W_KB) * 64;                                     // in 16-byte words
+    constexpr int S_TILES = KIND == kMx ? (BM + BN) / 16 : 0, S_LOADS = S_TILES / (4 * WAVES), S_WORDS = S_TILES * 16;
+    static_assert(X_KB % WAVES == 0 && W_KB % WAVES == 0 && S_TILES % (4 * WAVES) == 0, "each wave copies the same share");
+    static_assert(FN == 2 && W_KB + X_KB >= WAVES * 4, "the epilogue stores 64 columns a wave, through one buffer");
+    static_assert(BM <= 64 * WAVES && BN <= 64 * WAVES, "a thread holds one row's and one column's scale");
+    constexpr int STORES = FM * 4;                                                // a lane's stores of a whole 16-bit tile
+    // one array for all of it: the compiler guards reads of a second one with waits for every copy in flight.
+    // BUF stages; two sets of scale words; a column's bias, scale and zero-point; a row's scale and code sum
+    constexpr int SCALES = BUF * STAGE, COLS = SCALES + 2 * S_WORDS, ROWS = COLS + BN * 3 / 4;
+    __shared__ lb_u32x4 lds[ROWS + (KIND == kMx ? 0 : BM / 2)];
+    float* const col = reinterpret_cast<float*>(lds + COLS);
+    float* const row = reinterpret_cast<float*>(lds + ROWS);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, r = lane & 31;
     const int wm = wave / WN, wn = wave % WN;
+    const int lane16 = lane * 16;
 
-    // work-groups are dealt to the 8 XCDs in turn: give each XCD one run of tiles, and walk a run in blocks of
-    // 8 tile rows so that what its L2 holds is used again
-    const int total = grid_m * grid_n, per = total / 8, extra = total % 8, xcd = blockIdx.x % 8;
-    const int id = xcd * per + (xcd < extra ? xcd : extra) + blockIdx.x / 8;
-    const int band = id / (8 * grid_n), rows_in = grid_m - band * 8 < 8 ? grid_m - band * 8 : 8;
-    const int in_band = id - band * 8 * grid_n;
-    const int bm = band * 8 + in_band % rows_in, bn = in_band / rows_in;
+    // work-groups are dealt to the 8 XCDs in turn: each XCD gets one run of tiles, walked in bands of 8 tile rows so
+    // that what its L2 holds is used again
+    const int total = grid_m * grid_n, xcd = blockIdx.x & 7, per = total >> 3, extra = total & 7;
+    const int first = xcd * per + (xcd < extra ? xcd : extra), last = first + per + (xcd < extra ? 1 : 0);
+    int tile = first + (blockIdx.x >> 3);
+    if (tile >= last) return;
 
-    const int64_t tiles = cdiv(p.K, 128), words = cdiv(p.K, 512);
-    const int64_t n_tiles = cdiv(p.N, 16), m_tiles = cdiv(p.M, 16);
+    const int k_tiles = (int)cdiv(p.K, 128), words = (int)cdiv(p.K, 512);
+    const int n_tiles = (int)cdiv(p.N, 16), m_tiles = (int)cdiv(p.M, 16);
+    const int stages = KIND == kInt8 ? (int)cdiv(p.K, 64) : k_tiles;
+    constexpr int W_STEP = 1024, X_STEP = KIND == kMx ? 1024 : KIND == kInt4 ? 128 : 64;
+    const int w_pitch = k_tiles * (KIND == kInt8 ? 2048 : 1024);                  // bytes of a row of tiles
 
-    // where this wave's copies come from; rows and tiles past the last repeat the last, and are dropped at the end
-    const uint8_t* src[LOADS];
+    // ---- copies.  Rows and tiles past the last repeat the last; their outputs are dropped.
+    int bm = 0, bn = 0;
+    __amdgpu_buffer_rsrc_t x_buf, w_buf, xs_buf, ws_buf;
+    int x_row[KIND == kMx ? X_LOADS : 1], w_row[W_LOADS], x_off[KIND == kMx ? 1 : X_LOADS], s_off[S_LOADS + 1];
+    auto buffer = [](const void* base) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
+    };
+    auto aim = [&]() {
+        const int band = tile / (8 * grid_n), rows_in = grid_m - band * 8 < 8 ? grid_m - band * 8 : 8;
+        const int in_band = tile - band * 8 * grid_n;
+        bm = band * 8 + in_band % rows_in;
+        bn = in_band / rows_in;
+        const int nt = bn * (BN / 16), nl = n_tiles - 1 - nt;
+        w_buf = buffer(p.w + (int64_t)nt * w_pitch);
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int kb = i * WAVES + wave;
-        if (kb < X_KB) {
-            if (KIND == kMx) {
-                const int64_t mt = (int64_t)bm * (BM / 16) + kb;
-                src[i] = p.a + (mt < m_tiles ? mt : m_tiles - 1) * tiles * 1024 + lane * 16;
-            } else {
-                // 8 rows of 128 bytes; 16-byte chunk c of row r lies in slot c ^ (r & 7), so that 8 lanes reading
-                // one chunk of 8 rows touch 8 different groups of banks
-                const int64_t m = (int64_t)bm * BM + kb * 8 + (lane >> 3);
-                src[i] = p.a + (m < p.M ? m : p.M - 1) * p.ld_a + ((lane & 7) ^ (lane >> 3)) * 16;
+        for (int i = 0; i < W_LOADS; ++i) w_row[i] = (i * WAVES + wave < nl ? i * WAVES + wave : nl) * w_pitch;
+        if constexpr (KIND == kMx) {
+            const int mt = bm * (BM / 16), ml = m_tiles - 1 - mt;
+            x_buf = buffer(p.a + (int64_t)mt * w_pitch);
+#pragma unroll
+            for (int i = 0; i < X_LOADS; ++i) x_row[i] = (i * WAVES + wave < ml ? i * WAVES + wave : ml) * w_pitch;
+            // 16 lanes copy the 256 bytes of a tile's word of scales; a copy takes four tiles of one operand
+            xs_buf = buffer(p.a_scale + (int64_t)mt * words * 64);
+            ws_buf = buffer(p.w_scale + (int64_t)nt * words * 64);
+#pragma unroll
+            for (int i = 0; i < S_LOADS; ++i) {
+                const int t = (i * WAVES + wave) * 4, u = (t < BM / 16 ? t : t - BM / 16) + (lane >> 4), l = t < BM / 16 ? ml : nl;
+                s_off[i] = (u < l ? u : l) * words * 256 + (lane & 15) * 16;
             }
         } else {
-            const int64_t nt = (int64_t)bn * (BN / 16) + (KIND == kInt8 ? (kb - X_KB) / 2 : kb - X_KB);
-            src[i] = p.w + ((nt < n_tiles ? nt : n_tiles - 1) * tiles * (KIND == kInt8 ? 2 : 1) +
-                            (KIND == kInt8 ? (kb - X_KB) % 2 : 0)) * 1024 + lane * 16;
-        }
-    }
-    auto fetch = [&](int buf) {
+            // INT4: 8 rows of 128 bytes a copy, chunk c of row r in slot c ^ (r & 7); INT8: 16 rows of 64 bytes, chunk
+            // c in slot c ^ (r >> 2 & 3).  Lanes that read one chunk of several rows then touch different banks.
+            const int row0 = KIND == kInt4 ? lane >> 3 : lane >> 2;
+            const int chunk = KIND == kInt4 ? (lane & 7) ^ row0 : (lane & 3) ^ (row0 >> 2 & 3);
+            const int ml = (int)p.M - 1 - bm * BM;
+            x_buf = buffer(p.a + (int64_t)bm * BM * p.ld_a);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            load_to_lds(src[i], &lds[buf][(i * WAVES + wave) * 64]);
-            src[i] += i * WAVES < X_KB ? (KIND == kMx ? 1024 : 128) : (KIND == kInt8 ? 2048 : 1024);
+            for (int i = 0; i < X_LOADS; ++i) {
+                const int row = (i * WAVES + wave) * (KIND == kInt4 ? 8 : 16) + row0;
+                x_off[i] = (row < ml ? row : ml) * (int)p.ld_a + chunk * 16;
+            }
+        }
+    };
+    auto copy = [&](__amdgpu_buffer_rsrc_t from, int lane_off, int off, lb_u32x4* to) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, lane_off, off, 0, 0);
+    };
+    auto fetch = [&](int t, int buf) {
+        lb_u32x4* to = lds + buf * STAGE + wave * 64;
+        if constexpr (KIND == kMx) {
+            if ((t & 3) == 0) {
+                lb_u32x4* set = lds + SCALES + (t >> 2 & 1) * S_WORDS + wave * 64;
+#pragma unroll
+                for (int i = 0; i < S_LOADS; ++i) {
+                    if ((i * WAVES + wave) * 4 < BM / 16) copy(xs_buf, s_off[i], (t >> 2) * 256, set + i * WAVES * 64);
+                    else copy(ws_buf, s_off[i], (t >> 2) * 256, set + i * WAVES * 64);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < X_LOADS; ++i) {
+            if constexpr (KIND == kMx) copy(x_buf, lane16, x_row[i] + t * X_STEP, to + i * WAVES * 64);
+            else copy(x_buf, x_off[i], t * X_STEP, to + i * WAVES * 64);
+        }
+#pragma unroll
+        for (int i = 0; i < W_LOADS; ++i) copy(w_buf, lane16, w_row[i] + t * W_STEP, to + (X_LOADS + i) * WAVES * 64);
+    };
+
+    // ---- operands in registers: of a block of 32 rows, chunk 2 c + h of row r for set c.  Row r of a column block is
+    // column (r / 16) 16 + (r / 4 & 1) 8 + (r / 8 & 1) 4 + r % 4 of the block's outputs, so that a lane ends with groups
+    // of 8 consecutive outputs.
+    lb_u32x4 xv[2][FM], wv[2][FN];
+    int xs[KIND == kMx ? FM : 1][2], ws[KIND == kMx ? FN : 1][2];
+    const int w_lane = (r >> 4) * 64 + h * 16 + (r >> 2 & 1) * 8 + (r >> 3 & 1) * 4 + (r & 3);
+    auto read_x = [&](const lb_u32x4* s, lb_u32x4 (&to)[FM], int c) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int block = wm * FM + i;
+            if (KIND == kMx) to[i] = s[block * 128 + (r >> 4) * 64 + (c * 2 + h) * 16 + (r & 15)];
+            else if (KIND == kInt8) to[i] = s[(block * 32 + r) * 4 + ((c * 2 + h) ^ (r >> 2 & 3))];
+            else to[i] = s[(block * 32 + r) * 8 + ((c * 2 + h) ^ (r & 7))];
+        }
+    };
+    auto read_w = [&](const lb_u32x4* s, lb_u32x4 (&to)[FN], int c) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) to[j] = s[X_KB * 64 + (wn * FN + j) * 128 + c * 32 + w_lane];
+    };
+    auto read_scales = [&](int t, int c) {
+        if constexpr (KIND == kMx) {
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(lds + SCALES + (t >> 2 & 1) * S_WORDS);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) xs[i][c] = (int)q[(wm * FM + i) * 128 + (r >> 4) * 64 + (c * 2 + h) * 16 + (r & 15)];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) ws[j][c] = (int)q[BM * 4 + (wn * FN + j) * 128 + c * 32 + w_lane];
         }
     };
 
     acc_t acc[FM][FN];
+    int buf = 0;
+    float c_scale = 1.0f, c_bias = 0.0f, r_scale = 1.0f;   // of the thread's column and row
+    int c_zero = 0, r_sum = 0;
+    auto start = [&]() {                                   // a tile's first copies
+        aim();
+        const int tid = threadIdx.x;
+        const int64_t n = bn * BN + tid < p.N ? bn * BN + tid : p.N - 1, m = bm * BM + tid < p.M ? bm * BM + tid : p.M - 1;
+        if (KIND != kMx) {
+            c_scale = p.sw_f32 ? static_cast<const float*>(p.sw)[n] : f16_bits_to_f32(static_cast<const uint16_t*>(p.sw)[n]);
+            r_scale = p.sa[m];
+            if (p.zp) {
+                c_zero = p.zp[n];
+                r_sum = p.sums[m];
+            }
+        }
+        if (p.bias) c_bias = load_as_f32(p.bias, p.bias_dtype, n);
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
+        for (int b = 0; b < BUF - 1; ++b)
+            if (b < stages) fetch(b, b);
+    };
+    // in stage t, when this wave has read the last of it: stage t + 1 has landed, and all waves are done with stage t's
+    // buffer.  Behind the last stage whatever the next buffer holds is read, and not used: no branch parts the reads
+    // from the products.
+    auto advance = [&](int t) {
+        if (t + 2 < BUF) meet<63>();                       // the first BUF - 1 had landed at the tile's start
+        else if (t + BUF <= stages) meet<(BUF - 2) * LOADS>();
+        else meet<0>();
+        if (t + BUF < stages) fetch(t + BUF, buf);
+        buf = buf + 1 == BUF ? 0 : buf + 1;
+        return lds + buf * STAGE;
+    };
+    // a read from LDS, then its share of the matrix instructions
+    auto interleave = [](auto reads_) {
+        constexpr int READS = decltype(reads_)::value;
+        auto one = [](auto i_) {
+            constexpr int i = decltype(i_)::value, share = FM * FN * (i + 1) / READS - FM * FN * i / READS;
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, share, 0);
+        };
+        static_for<0, READS>(one);
+    };
 
-    // the scale words of four steps, BM / 16 + BN / 16 tiles of 256 bytes: 16 lanes copy a tile's
-    constexpr int S_TILES = (BM + BN) / 16, S_WAVES = S_TILES / 4;
-    static_assert(KIND != kMx || (BM % 64 == 0 && BN % 64 == 0 && S_WAVES <= WAVES), "a wave copies the scales of four tiles");
-    __shared__ uint32_t lds_s[KIND == kMx ? 2 : 1][KIND == kMx ? S_TILES * 64 : 1];
-    const uint32_t* s_src = nullptr;
-    if (KIND == kMx && wave < S_WAVES) {
-        const int tile = wave * 4 + (lane >> 4);
-        if (tile < BM / 16) {
-            const int64_t mt = (int64_t)bm * (BM / 16) + tile;
-            s_src = p.a_scale + (mt < m_tiles ? mt : m_tiles - 1) * words * 64 + (lane & 15) * 4;
+    start();
+    meet<0>();
+    for (;;) {
+        if (threadIdx.x < BN) {
+            col[threadIdx.x] = c_bias;
+            if (KIND != kMx) {
+                col[BN + threadIdx.x] = c_scale;
+                col[2 * BN + threadIdx.x] = __int_as_float(c_zero);
+            }
+        }
+        if (KIND != kMx && threadIdx.x < BM) {
+            row[threadIdx.x] = r_scale;
+            row[BM + threadIdx.x] = __int_as_float(r_sum);
+        }
+        if (BUF <= stages) fetch(BUF - 1, BUF - 1);
+        read_x(lds, xv[0], 0);
+        read_w(lds, wv[0], 0);
+        read_scales(0, 0);
+        buf = 0;
+        if constexpr (KIND == kInt4) {
+            // four sets a stage: the low nibbles of both words of weights, then the high ones
+            auto stage = [&](int t, auto first_) {
+                constexpr bool FIRST = decltype(first_)::value;
+                auto products = [&](int word, bool high, const lb_u32x4 (&x)[FM], bool fresh) {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) {
+                        const lb_u32x4 w = high ? high_nibbles(wv[word][j]) : low_nibbles(wv[word][j]);
+#pragma unroll
+                        for (int i = 0; i < FM; ++i) acc[i][j] = mma32_i8(w, x[i], fresh ? acc_t{} : acc[i][j]);
+                    }
+                };
+                const lb_u32x4* here = lds + buf * STAGE;
+                read_x(here, xv[1], 1);
+                read_w(here, wv[1], 1);
+                products(0, false, xv[0], FIRST);
+                interleave(std::integral_constant<int, FM + FN>{});
+                __builtin_amdgcn_sched_barrier(0);
+                read_x(here, xv[0], 2);
+                products(1, false, xv[1], false);
+                interleave(std::integral_constant<int, FM>{});
+                __builtin_amdgcn_sched_barrier(0);
+                read_x(here, xv[1], 3);
+                products(0, true, xv[0], false);
+                interleave(std::integral_constant<int, FM>{});
+                const lb_u32x4* s = advance(t);
+                read_x(s, xv[0], 0);
+                read_w(s, wv[0], 0);
+                products(1, true, xv[1], false);
+                interleave(std::integral_constant<int, FM + FN>{});
+            };
+            stage(0, std::true_type{});
+#pragma unroll 1
+            for (int t = 1; t < stages; ++t) stage(t, std::false_type{});
         } else {
-            const int64_t nt = (int64_t)bn * (BN / 16) + tile - BM / 16;
-            s_src = p.w_scale + (nt < n_tiles ? nt : n_tiles - 1) * words * 64 + (lane & 15) * 4;
-        }
-    }
-    auto fetch_scales = [&](int half) {
-        if (KIND == kMx && wave < S_WAVES) {
-            load_to_lds(s_src, &lds_s[half][wave * 256]);
-            s_src += 64;
-        }
-    };
-    int xs[KIND == kMx ? FM : 1], ws[KIND == kMx ? FN : 1];
-    auto read_scales = [&](int half) {
-        if constexpr (KIND == kMx) {
+            // (stage t with t % 4 = B: the byte of its scales)
+            auto stage = [&](int t, auto byte, auto first_) {
+                constexpr int B = decltype(byte)::value;
+                constexpr bool FIRST = decltype(first_)::value;
+                auto products = [&](auto set, bool fresh) {
+                    constexpr int C = decltype(set)::value;
 #pragma unroll
-            for (int i = 0; i < FM; ++i) xs[i] = (int)lds_s[half][(wm * FM + i) * 64 + lane];
+                    for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) ws[j] = (int)lds_s[half][(BM / 16 + wn * FN + j) * 64 + lane];
+                        for (int i = 0; i < FM; ++i) {
+                            const acc_t a = fresh ? acc_t{} : acc[i][j];
+                            if constexpr (KIND == kMx) acc[i][j] = mma32_mx<B>(wv[C][j], xv[C][i], a, ws[j][C], xs[i][C]);
+                            else acc[i][j] = mma32_i8(wv[C][j], xv[C][i], a);
+                        }
+                };
+                const lb_u32x4* here = lds + buf * STAGE;
+                read_x(here, xv[1], 1);
+                read_w(here, wv[1], 1);
+                if (B == 0) read_scales(t, 1);
+                products(std::integral_constant<int, 0>{}, FIRST);
+                interleave(std::integral_constant<int, FM + FN>{});
+                const lb_u32x4* s = advance(t);
+                read_x(s, xv[0], 0);
+                read_w(s, wv[0], 0);
+                if (B == 3) read_scales(t + 1, 0);
+                products(std::integral_constant<int, 1>{}, false);
+                interleave(std::integral_constant<int, FM + FN>{});
+            };
+            stage(0, std::integral_constant<int, 0>{}, std::true_type{});
+            if constexpr (KIND == kMx) {
+#pragma unroll 1
+                for (int t = 1; t < stages; t += 4) {
+                    stage(t, std::integral_constant<int, 1>{}, std::false_type{});
+                    if (t + 1 < stages) stage(t + 1, std::integral_constant<int, 2>{}, std::false_type{});
+                    if (t + 2 < stages) stage(t + 2, std::integral_constant<int, 3>{}, std::false_type{});
+                    if (t + 3 < stages) stage(t + 3, std::integral_constant<int, 0>{}, std::false_type{});
+                }
+            } else {
+#pragma unroll 1
+                for (int t = 1; t < stages; ++t) stage(t, std::integral_constant<int, 1>{}, std::false_type{});
+            }
         }
-    };
 
-    auto step = [&](const lb_u32x4* s, auto byte) {
-        constexpr int B = decltype(byte)::value;
-        const lb_u32x4* x = s + wm * FM * (KIND == kMx ? 64 : 128);
-        const lb_u32x4* w = s + X_KB * 64 + wn * FN * (KIND == kInt8 ? 128 : 64) + lane;
-        if constexpr (KIND == kMx) {
-            lb_u32x4 wv[FN];
+        // ---- outputs, after the next tile's first copies
+        const int m0 = bm * BM + wm * FM * 32, n0 = bn * BN + wn * FN * 32;
+        const bool whole = p.wide && p.out_dtype != IC_DTYPE_F32 && (bm + 1) * BM <= p.M && (bn + 1) * BN <= p.N;
+        tile += gridDim.x >> 3;
+        const bool more = tile < last;                     // (all waves are done with the buffers)
+        // y from the accumulated sum: INT4 operands are held as 16 q, and the shift is exact.  |zp| <= 2^7 and
+        // |sum| <= 2^23 for K <= 65536, so the 24-bit product is exact, and |sum_k a (q - zp)| < 2^31, so the
+        // difference is right even where a term has wrapped.
+        auto value = [&](auto s, float sw, float zero, float bias, float sa, float sum) {
+            if constexpr (KIND == kMx) return s + bias;
+            else {
+                const unsigned d = (unsigned)(KIND == kInt4 ? s >> 4 : s) - (unsigned)__mul24(__float_as_int(zero), __float_as_int(sum));
+                return (float)(int)d * (sa * sw) + bias;
+            }
+        };
+        if (p.wide) {
+            if (more) start();
+            // 32 rows of 128 bytes at a time through the wave's part of the last buffer, so that 8 lanes store a line;
+            // chunk c of row r lies in slot c ^ (r & 7)
+            lb_u32x4* area = lds + (BUF - 1) * STAGE + wave * 256;
+            const int chunk = (lane & 7) ^ (lane >> 3), m1 = m0 + (lane >> 3);
+            auto flush = [&](int i, int n) {
+                lds_wave_fence();
+                const int64_t at = m1 * p.ld_out + n;
+                lb_u32x4 v[4];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) wv[j] = w[j * 64];
+                for (int k = 0; k < 4; ++k) v[k] = area[k * 64 + lane];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int m = i * 32 + k * 8;
+                    if (m1 + m >= p.M || n >= p.N) continue;
+                    if (p.out_dtype == IC_DTYPE_F32) *reinterpret_cast<lb_u32x4*>(static_cast<float*>(p.out) + at + m * p.ld_out) = v[k];
+                    else *reinterpret_cast<lb_u32x4*>(static_cast<uint16_t*>(p.out) + at + m * p.ld_out) = v[k];
+                }
+                lds_wave_fence();
+            };
+            const int cw = wn * FN * 32, rw = wm * FM * 32;
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const lb_u32x4 xv = x[i * 64 + lane];
+                const float sa = KIND == kMx ? 0.0f : row[rw + i * 32 + r], sum = KIND == kMx ? 0.0f : row[BM + rw + i * 32 + r];
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mma_mx<B>(wv[j], xv, acc[i][j], ws[j], xs[i]);
+                for (int j = 0; j < FN; ++j) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        lb_f32x4 v[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int c = cw + j * 32 + q * 16 + h * 8 + k * 4;
+                            const lb_f32x4 bias = *reinterpret_cast<const lb_f32x4*>(col + c);
+                            lb_f32x4 sw = {}, zero = {};
+                            if (KIND != kMx) {
+                                sw = *reinterpret_cast<const lb_f32x4*>(col + BN + c);
+                                zero = *reinterpret_cast<const lb_f32x4*>(col + 2 * BN + c);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[k][e] = value(acc[i][j][8 * q + 4 * k + e], sw[e], zero[e], bias[e], sa, sum);
+                        }
+                        if (p.out_dtype == IC_DTYPE_F32) {
+                            area[r * 8 + ((q * 4 + h * 2) ^ (r & 7))] = __builtin_bit_cast(lb_u32x4, v[0]);
+                            area[r * 8 + ((q * 4 + h * 2 + 1) ^ (r & 7))] = __builtin_bit_cast(lb_u32x4, v[1]);
+                        } else {
+                            lb_u32x4 w;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = p.out_dtype == IC_DTYPE_BF16 ? pack_half_words<IC_DTYPE_BF16>(v[e >> 1][2 * (e & 1)], v[e >> 1][2 * (e & 1) + 1])
+                                                                    : pack_half_words<IC_DTYPE_F16>(v[e >> 1][2 * (e & 1)], v[e >> 1][2 * (e & 1) + 1]);
+                            area[r * 8 + ((j * 4 + q * 2 + h) ^ (r & 7))] = w;
+                        }
+                    }
+                    if (p.out_dtype == IC_DTYPE_F32) flush(i, n0 + j * 32 + chunk * 4);
+                }
+                if (p.out_dtype != IC_DTYPE_F32) flush(i, n0 + chunk * 8);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (!more) break;
+            if (whole) meet<STORES>();                     // the copies were issued before the stores
+            else meet<0>();
         } else {
-            lb_u32x4 wv[2][FN];
+            // rows of y at any alignment: 32 rows at a time through LDS, then value by value
+            constexpr int PITCH = FN * 32 + 4;
+            static_assert(WAVES * 32 * PITCH * 4 <= SCALES * 16, "the waves' areas lie in the buffers");
+            typedef std::conditional_t<KIND == kMx, float, int> sum_t;
+            typedef sum_t sum4_t __attribute__((ext_vector_type(4)));
+            sum_t* area = reinterpret_cast<sum_t*>(lds) + wave * 32 * PITCH;
 #pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                if (KIND == kInt4) {
-                    const lb_u32x4 q = w[j * 64];
-                    wv[0][j] = low_nibbles(q);
-                    wv[1][j] = high_nibbles(q);
-                } else {
-                    wv[0][j] = w[j * 128];
-                    wv[1][j] = w[j * 128 + 64];
+            for (int i = 0; i < FM; ++i) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<sum4_t*>(area + r * PITCH + j * 32 + (k >> 1) * 16 + h * 8 + (k & 1) * 4) =
+                            sum4_t{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+                lds_wave_fence();
+                const int rows = (int)p.M - (m0 + i * 32) < 32 ? (int)p.M - (m0 + i * 32) : 32;
+#pragma unroll 1
+                for (int e = lane; e < rows * FN * 32; e += 64) {
+                    const int m = e / (FN * 32), n = e % (FN * 32);
+                    if (n0 + n >= p.N) continue;
+                    const sum_t s = area[m * PITCH + n];
+                    const int c = wn * FN * 32 + n, o = wm * FM * 32 + i * 32 + m;
+                    const float v = KIND == kMx ? value(s, 0.0f, 0.0f, col[c], 0.0f, 0.0f)
+                                                : value(s, col[BN + c], col[2 * BN + c], col[c], row[o], row[BM + o]);
+                    store_from_f32(p.out, p.out_dtype, (m0 + i * 32 + m) * p.ld_out + n0 + n, v);
                 }
+                lds_wave_fence();
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    const lb_u32x4 xv = x[(i * 16 + r) * 8 + ((h * 4 + g) ^ (r & 7))];
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i][j] = mma_i8(wv[h][j], xv, acc[i][j]);
-                }
+            if (!more) break;
+            meet<0>();
+            start();
+            meet<0>();
         }
-    };
-
-    // one step: wait for this wave's own copies of it, meet the others (whose copies have then landed too, and who
-    // are done with the buffer of the step before), fill that buffer, multiply.  The scales of four steps are copied
-    // just before the first of them, into the half that the last four did not use.
-    const int steps = (int)tiles;
-    auto turn = [&](int t, int buf, int half, auto byte) {
-        constexpr int B = decltype(byte)::value;
-        if (t + BUF - 2 < steps) meet<LOADS * (BUF - 2)>();
-        else meet<0>();
-        if (t + BUF - 1 < steps) {
-            if (KIND == kMx && B == 1) fetch_scales(half ^ 1);         // (of step t + 3, the first of its word)
-            fetch((buf + BUF - 1) % BUF);
-        }
-        if (KIND == kMx && B == 0) read_scales(half);
-        step(lds[buf], byte);
-    };
-    if (KIND == kMx) fetch_scales(0);
-#pragma unroll
-    for (int b = 0; b < BUF - 1; ++b)
-        if (b < steps) fetch(b);
-    if constexpr (KIND == kMx) {
-        static_assert(KIND != kMx || BUF == 4, "a word of scales holds four steps");
-        for (int t = 0, half = 0; t < steps; t += 4, half ^= 1) {
-            turn(t, 0, half, std::integral_constant<int, 0>{});
-            if (t + 1 < steps) turn(t + 1, 1, half, std::integral_constant<int, 1>{});
-            if (t + 2 < steps) turn(t + 2, 2, half, std::integral_constant<int, 2>{});
-            if (t + 3 < steps) turn(t + 3, 3, half, std::integral_constant<int, 3>{});
-        }
-    } else {
-        for (int t = 0; t < steps; t += BUF) {
-#pragma unroll
-            for (int b = 0; b < BUF; ++b)
-                if (t + b < steps) turn(t + b, b, 0, std::integral_constant<int, 0>{});
-        }
-    }
-    static_assert(FN == 2 || FN == 4, "store_rows takes 32 or 64 columns");
-    static_assert(sizeof(lds) >= WAVES * 16 * (16 * FN + 4) * 4, "the areas of the epilogue lie in the buffers");
-    Columns<KIND> cols[FN];
-    const int64_t m0 = (int64_t)bm * BM + wm * FM * 16, n0 = (int64_t)bn * BN + wn * FN * 16;
-#pragma unroll
-    for (int j = 0; j < FN; ++j) cols[j].load(p, n0 + j * 16 + g * 4);
-    meet<0>();                                               // the buffers are free
-    float* area = reinterpret_cast<float*>(&lds[0][0]) + wave * 16 * (16 * FN + 4);
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int64_t m = m0 + i * 16 + r < p.M ? m0 + i * 16 + r : p.M - 1;
-        const float sa = KIND == kMx ? 1.0f : p.sa[m];
-        const int sum = KIND != kMx && p.zp ? p.sums[m] : 0;
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-            *reinterpret_cast<lb_f32x4*>(area + r * (16 * FN + 4) + j * 16 + g * 4) = cols[j].finish(acc[i][j], sa, sum);
-        lds_wave_fence();
-        store_rows<FN>(p, area, lane, m0 + i * 16, n0);
-        lds_wave_fence();
     }
 }
 
@@ -443,10 +649,13 @@ void launch_direct(const Operands& p, hipStream_t st) {
     hipLaunchKernelGGL((linear_direct_kernel<KIND, MT, WAVES>), grid, dim3(64 * WAVES), 0, st, p);
 }
 
+// One work-group a CU (256 of them), each of which walks its XCD's tiles.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF>
 void launch_tiled(const Operands& p, hipStream_t st) {
-    const int gm = (int)cdiv(p.M, WM * FM * 16), gn = (int)cdiv(p.N, WN * FN * 16);
-    hipLaunchKernelGGL((linear_tiled_kernel<KIND, WM, WN, FM, FN, BUF>), dim3((unsigned)gm * gn), dim3(64 * WM * WN), 0, st, p, gm, gn);
+    const int gm = (int)cdiv(p.M, 32 * WM * FM), gn = (int)cdiv(p.N, 32 * WN * FN);
+    const int64_t tiles = (int64_t)gm * gn;
+    const unsigned grid = (unsigned)(tiles < 256 ? cdiv(tiles, 8) * 8 : 256);
+    hipLaunchKernelGGL((linear_tiled_kernel<KIND, WM, WN, FM, FN, BUF>), dim3(grid), dim3(64 * WM * WN), 0, st, p, gm, gn);
 }
 
 template <int KIND>
@@ -454,7 +663,7 @@ int launch_linear(const Operands& p, hipStream_t st) {
     if (p.M <= 16) launch_direct<KIND, 1, 8>(p, st);
     else if (p.M <= 32) launch_direct<KIND, 2, 8>(p, st);
     else if (p.M <= 64) launch_direct<KIND, 4, 8>(p, st);
-    else launch_tiled<KIND, 2, 4, 8, 4, KIND == kMx ? 4 : KIND == kInt4 ? 3 : 2>(p, st);
+    else launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
@@ -512,7 +721,7 @@ extern "C" int ic_quantized_linear(const int8_t* a, int64_t ld_a, const float* s
     IC_REQUIRE(ld_a >= cdiv(K, kActPad) * kActPad && ld_a % 16 == 0 && aligned16(a) && aligned16(tiles),
                "ic_quantized_linear: activations need rows of ic_activation_pitch codes, 16-byte aligned");
     IC_REQUIRE(ld_out >= N, "ic_quantized_linear: ld_out below N");
-    p.wide = aligned16(out) && ld_out % 4 == 0;
+    p.wide = aligned16(out) && ld_out % (out_dtype == IC_DTYPE_F32 ? 4 : 8) == 0 && N % 8 == 0;
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 2.0 * M * N * K, (double)M * K + (double)N * K * bits / 8);
     return bits == 8 ? launch_linear<kInt8>(p, st) : launch_linear<kInt4>(p, st);
@@ -531,7 +740,7 @@ extern "C" int ic_mxfp4_linear(const void* a, const void* a_scales, int64_t M, c
     IC_REQUIRE(a && a_scales && w && w_scales && out, "ic_mxfp4_linear: null pointer");
     IC_REQUIRE(aligned16(a) && aligned16(w) && aligned16(a_scales) && aligned16(w_scales) && ld_out >= N,
                "ic_mxfp4_linear: operands need 16-byte alignment and ld_out at least N");
-    p.wide = aligned16(out) && ld_out % 4 == 0;
+    p.wide = aligned16(out) && ld_out % (out_dtype == IC_DTYPE_F32 ? 4 : 8) == 0 && N % 8 == 0;
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 2.0 * M * N * K, ((double)M * K + (double)N * K) * 17 / 32);
     return launch_linear<kMx>(p, st);
