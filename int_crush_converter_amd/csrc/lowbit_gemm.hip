@@ -296,10 +296,11 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
                 s_off[i] = (u < l ? u : l) * words * 256 + (lane & 15) * 16;
             }
         } else {
-            // INT4: 8 rows of 128 bytes a copy, chunk c of row r in slot c ^ (r & 7); INT8: 16 rows of 64 bytes, chunk
-            // c in slot c ^ (r >> 2 & 3).  Lanes that read one chunk of several rows then touch different banks.
+            // INT4: 8 rows of 128 bytes a copy, chunk c of row r in slot c ^ (r >> 1 & 7); INT8: 16 rows of 64 bytes, chunk
+            // c in slot c ^ (r >> 2 & 3).  16 lanes that read one chunk of 16 rows then touch all 64 banks once.
             const int row0 = KIND == kInt4 ? lane >> 3 : lane >> 2;
-            const int chunk = KIND == kInt4 ? (lane & 7) ^ row0 : (lane & 3) ^ (row0 >> 2 & 3);
+            const int chunk = KIND == kInt4 ? (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4)) : (lane & 3) ^ (lane >> 4);
+            static_assert(WAVES % 2 == 0, "a wave's copies begin at rows of one parity of 8");
             const int ml = (int)p.M - 1 - bm * BM;
             x_buf = buffer(p.a + (int64_t)bm * BM * p.ld_a);
 #pragma unroll
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
             const int block = wm * FM + i;
             if (KIND == kMx) to[i] = s[block * 128 + (r >> 4) * 64 + (c * 2 + h) * 16 + (r & 15)];
             else if (KIND == kInt8) to[i] = s[(block * 32 + r) * 4 + ((c * 2 + h) ^ (r >> 2 & 3))];
-            else to[i] = s[(block * 32 + r) * 8 + ((c * 2 + h) ^ (r & 7))];
+            else to[i] = s[(block * 32 + r) * 8 + ((c * 2 + h) ^ (r >> 1 & 7))];
         }
     };
     auto read_w = [&](const lb_u32x4* s, lb_u32x4 (&to)[FN], int c) {
@@ -520,21 +521,20 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
         if (p.wide) {
             if (more) start();
             // 32 rows of 128 bytes at a time through the wave's part of the last buffer, so that 8 lanes store a line;
-            // chunk c of row r lies in slot c ^ (r & 7)
+            // chunk c of row r lies in slot c ^ (r >> 1 & 7)
             lb_u32x4* area = lds + (BUF - 1) * STAGE + wave * 256;
-            const int chunk = (lane & 7) ^ (lane >> 3), m1 = m0 + (lane >> 3);
-            auto flush = [&](int i, int n) {
+            const int chunk = (lane & 7) ^ (lane >> 4), m1 = m0 + (lane >> 3);     // (of rows k 8 + lane / 8, k even)
+            auto flush = [&](int i, int n0, int width) {
                 lds_wave_fence();
-                const int64_t at = m1 * p.ld_out + n;
                 lb_u32x4 v[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] = area[k * 64 + lane];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int m = i * 32 + k * 8;
-                    if (m1 + m >= p.M || n >= p.N) continue;
-                    if (p.out_dtype == IC_DTYPE_F32) *reinterpret_cast<lb_u32x4*>(static_cast<float*>(p.out) + at + m * p.ld_out) = v[k];
-                    else *reinterpret_cast<lb_u32x4*>(static_cast<uint16_t*>(p.out) + at + m * p.ld_out) = v[k];
+                    const int m = m1 + i * 32 + k * 8, n = n0 + (chunk ^ (k & 1) * 4) * width;
+                    if (m >= p.M || n >= p.N) continue;
+                    if (p.out_dtype == IC_DTYPE_F32) *reinterpret_cast<lb_u32x4*>(static_cast<float*>(p.out) + m * p.ld_out + n) = v[k];
+                    else *reinterpret_cast<lb_u32x4*>(static_cast<uint16_t*>(p.out) + m * p.ld_out + n) = v[k];
                 }
                 lds_wave_fence();
             };
@@ -560,20 +560,20 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
                             for (int e = 0; e < 4; ++e) v[k][e] = value(acc[i][j][8 * q + 4 * k + e], sw[e], zero[e], bias[e], sa, sum);
                         }
                         if (p.out_dtype == IC_DTYPE_F32) {
-                            area[r * 8 + ((q * 4 + h * 2) ^ (r & 7))] = __builtin_bit_cast(lb_u32x4, v[0]);
-                            area[r * 8 + ((q * 4 + h * 2 + 1) ^ (r & 7))] = __builtin_bit_cast(lb_u32x4, v[1]);
+                            area[r * 8 + ((q * 4 + h * 2) ^ (r >> 1 & 7))] = __builtin_bit_cast(lb_u32x4, v[0]);
+                            area[r * 8 + ((q * 4 + h * 2 + 1) ^ (r >> 1 & 7))] = __builtin_bit_cast(lb_u32x4, v[1]);
                         } else {
                             lb_u32x4 w;
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 w[e] = p.out_dtype == IC_DTYPE_BF16 ? pack_half_words<IC_DTYPE_BF16>(v[e >> 1][2 * (e & 1)], v[e >> 1][2 * (e & 1) + 1])
                                                                     : pack_half_words<IC_DTYPE_F16>(v[e >> 1][2 * (e & 1)], v[e >> 1][2 * (e & 1) + 1]);
-                            area[r * 8 + ((j * 4 + q * 2 + h) ^ (r & 7))] = w;
+                            area[r * 8 + ((j * 4 + q * 2 + h) ^ (r >> 1 & 7))] = w;
                         }
                     }
-                    if (p.out_dtype == IC_DTYPE_F32) flush(i, n0 + j * 32 + chunk * 4);
+                    if (p.out_dtype == IC_DTYPE_F32) flush(i, n0 + j * 32, 4);
                 }
-                if (p.out_dtype != IC_DTYPE_F32) flush(i, n0 + chunk * 8);
+                if (p.out_dtype != IC_DTYPE_F32) flush(i, n0, 8);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (!more) break;
@@ -596,7 +596,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
                             sum4_t{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
                 lds_wave_fence();
                 const int rows = (int)p.M - (m0 + i * 32) < 32 ? (int)p.M - (m0 + i * 32) : 32;
-#pragma unroll 1
+#pragma unroll 4
                 for (int e = lane; e < rows * FN * 32; e += 64) {
                     const int m = e / (FN * 32), n = e % (FN * 32);
                     if (n0 + n >= p.N) continue;
@@ -649,21 +649,37 @@ void launch_direct(const Operands& p, hipStream_t st) {
     hipLaunchKernelGGL((linear_direct_kernel<KIND, MT, WAVES>), grid, dim3(64 * WAVES), 0, st, p);
 }
 
-// One work-group a CU (256 of them), each of which walks its XCD's tiles.
+// As many work-groups as run at once (one a CU with tiles of 256 x 256, whose
+// buffers take most of its LDS, two with 128 x 128), each of which walks its
+// XCD's tiles.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF>
 void launch_tiled(const Operands& p, hipStream_t st) {
     const int gm = (int)cdiv(p.M, 32 * WM * FM), gn = (int)cdiv(p.N, 32 * WN * FN);
     const int64_t tiles = (int64_t)gm * gn;
-    const unsigned grid = (unsigned)(tiles < 256 ? cdiv(tiles, 8) * 8 : 256);
+    constexpr int64_t at_once = WM * WN == 4 ? 512 : 256;
+    const unsigned grid = (unsigned)(tiles < at_once ? cdiv(tiles, 8) * 8 : at_once);
     hipLaunchKernelGGL((linear_tiled_kernel<KIND, WM, WN, FM, FN, BUF>), dim3(grid), dim3(64 * WM * WN), 0, st, p, gm, gn);
 }
 
+// Which form: the direct one while it has few work-groups (of 64 rows x 16
+// columns each), since a tile of 128 x 128 takes its K steps one after another
+// and leaves CUs idle when there are few; then tiles of 256 x 256 where they
+// fill at least three quarters of their rounds over the 256 CUs, else of
+// 128 x 128.  Measured, us (direct / 128 / 256):
+//   INT4 M 128 4096x4096 (512 work-groups)  19 / 23 / 49;  M 200 (1024)  30 / 23 / 49
+//   INT4 M 2048 4096x4096 (256-tiles fill 1/2)  245 / 43 / 54;  M 3000 (3/4)  - / 60 / 59
+//   INT4 M 4096 12288x4096 (all)  - / 215 / 189
+//   MXFP4 M 200 4096x4096 (1024)  14 / 15 / 29;  M 333 (1536)  20 / 16 / 30
+//   MXFP4 M 2048 4096x4096 (1/2)  81 / 27 / 34;  M 4096 12288x4096 (all)  - / 131 / 118
 template <int KIND>
 int launch_linear(const Operands& p, hipStream_t st) {
+    const int64_t groups = cdiv(p.N, 16) * cdiv(p.M, 64);
+    const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256);
     if (p.M <= 16) launch_direct<KIND, 1, 8>(p, st);
     else if (p.M <= 32) launch_direct<KIND, 2, 8>(p, st);
-    else if (p.M <= 64) launch_direct<KIND, 4, 8>(p, st);
-    else launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
+    else if (p.M <= 64 || groups < (KIND == kMx ? 1100 : 700)) launch_direct<KIND, 4, 8>(p, st);
+    else if (tiles * 4 >= cdiv(tiles, 256) * 256 * 3) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
+    else launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4>(p, st);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
