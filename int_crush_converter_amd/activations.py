@@ -19,14 +19,6 @@ MAX_FEATURES = 65536
 _PAD = 128                       # ic_activation_pitch
 
 
-def check_gpu(name: str, t: torch.Tensor) -> torch.Tensor:
-    """A tensor in GPU memory, on the current device."""
-    t = nat.to_gpu(t)
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return t
-
-
 def as_rows(t: torch.Tensor) -> torch.Tensor:
     """[..., K] as 2-D rows whose columns are contiguous (a copy only where the strides ask for one)."""
     if t.dim() != 2:
@@ -36,15 +28,39 @@ def as_rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+_entries: dict[str, object] = {}
+
+
+def call(name: str, *args) -> None:
+    """A library call with device addresses, checked tensors behind them."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = nat.entry(name)
+    rc = fn(*args)
+    if rc:
+        nat.check(rc, name)
+
+
 class QuantizedActivations:
     """int8 codes of shape ``[*lead, in_features]``, their fp32 scales and the int32 sums of each row's codes.
     On the GPU; rows are stored at a pitch of whole 128 bytes, zeros behind the last column."""
 
-    __slots__ = ("data", "scales", "sums", "in_features", "lead")
+    __slots__ = ("data", "meta", "in_features", "lead")
 
-    def __init__(self, data: torch.Tensor, scales: torch.Tensor, sums: torch.Tensor, in_features: int, lead):
-        self.data, self.scales, self.sums = data, scales, sums
+    def __init__(self, data: torch.Tensor, meta: torch.Tensor, in_features: int, lead):
+        self.data = data                     # int8 [rows, pitch]
+        self.meta = meta                     # fp32 [2, rows]: the scales; the sums' bits
         self.in_features, self.lead = in_features, tuple(lead)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """fp32 [rows]."""
+        return self.meta[0]
+
+    @property
+    def sums(self) -> torch.Tensor:
+        """int32 [rows]: the sum of each row's codes."""
+        return self.meta[1].view(torch.int32)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "QuantizedActivations":
@@ -55,19 +71,19 @@ class QuantizedActivations:
         lead, K = codes.shape[:-1], codes.shape[-1]
         if not 1 <= K <= MAX_FEATURES:
             raise ValueError(f"in_features must be in [1, {MAX_FEATURES}], got {K}")
-        codes = as_rows(check_gpu("codes", codes)) if codes.numel() else check_gpu("codes", codes).reshape(-1, K)
+        codes = as_rows(nat.on_gpu("codes", codes)) if codes.numel() else nat.on_gpu("codes", codes).reshape(-1, K)
         rows = codes.shape[0]
         if scales.numel() != rows:
             raise ValueError(f"{scales.numel()} scales for {rows} rows of codes")
-        scales = check_gpu("scales", scales).reshape(-1).to(torch.float32).contiguous()
+        meta = torch.empty((2, rows), dtype=torch.float32, device=codes.device)
+        meta[0] = nat.on_gpu("scales", scales).reshape(-1)
         if K % _PAD or codes.stride(0) != K or codes.data_ptr() % 16:
             data = torch.zeros(rows, -(-K // _PAD) * _PAD, dtype=torch.int8, device=codes.device)
             data[:, :K] = codes
         else:
             data = codes
-        sums = torch.empty(rows, dtype=torch.int32, device=codes.device)
-        nat.check(nat.lib().ic_row_sums_i8(data, rows, K, data.shape[1], sums, nat.stream()), "ic_row_sums_i8")
-        return cls(data, scales, sums, K, lead)
+        call("ic_row_sums_i8", data.data_ptr(), rows, K, data.shape[1], meta.data_ptr() + 4 * rows, nat.raw_stream())
+        return cls(data, meta, K, lead)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -79,10 +95,8 @@ class QuantizedActivations:
         """The values ``q * s`` [*lead, in_features], rounded once to ``dtype``."""
         K, data = self.in_features, self.data
         out = torch.empty((*self.lead, K), dtype=dtype, device=data.device)
-        code = nat.dtype_code(out)
-        nat.check(nat.lib().ic_dequantize_rows(data.data_ptr(), data.shape[0], K, data.shape[1],
-                                               self.scales.data_ptr(), out.data_ptr(), code, K, nat.stream()),
-                  "ic_dequantize_rows")
+        call("ic_dequantize_rows", data.data_ptr(), data.shape[0], K, data.shape[1], self.meta.data_ptr(),
+             out.data_ptr(), nat.dtype_code(out), K, nat.raw_stream())
         return out
 
 
@@ -96,7 +110,7 @@ def _quantize(x, weight, residual, eps, rot_size):
     Kp = -(-K // rot) * rot
     if not 1 <= K or Kp > MAX_FEATURES:
         raise ValueError(f"in_features (padded to the rotation) must be in [1, {MAX_FEATURES}], got {K}")
-    xg = check_gpu("x", x)
+    xg = nat.on_gpu("x", x)
     code = nat.dtype_code(xg)
     dev, rows = xg.device, x.numel() // K
     xr = as_rows(xg) if rows else xg.reshape(0, K)
@@ -105,13 +119,13 @@ def _quantize(x, weight, residual, eps, rot_size):
     if residual is not None:
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} does not match x {tuple(x.shape)} {x.dtype}")
-        rg = check_gpu("residual", residual)
+        rg = nat.on_gpu("residual", residual)
         rr = as_rows(rg) if rows else rg.reshape(0, K)
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
     if weight is not None:
         if weight.shape != (K,):
             raise ValueError(f"the norm's weight has shape {tuple(weight.shape)}, expected ({K},)")
-        w = check_gpu("weight", weight)
+        w = nat.on_gpu("weight", weight)
         if w.dtype != x.dtype:
             if w.dtype not in (torch.float32, torch.bfloat16, torch.float16):
                 raise TypeError(f"unsupported dtype {w.dtype}")
@@ -119,16 +133,15 @@ def _quantize(x, weight, residual, eps, rot_size):
         w = w.contiguous()
     pitch = -(-Kp // _PAD) * _PAD
     data = torch.empty((rows, pitch), dtype=torch.int8, device=dev)
-    scales = torch.empty(rows, dtype=torch.float32, device=dev)
-    sums = torch.empty(rows, dtype=torch.int32, device=dev)
-    ld = lambda t: t.stride(0) if rows > 1 else K                # noqa: E731
-    nat.check(nat.lib().ic_quantize_rows(
-        xr.data_ptr(), code, rows, K, ld(xr), None if rr is None else rr.data_ptr(), 0 if rr is None else ld(rr),
-        None if w is None else w.data_ptr(), wcode, eps, rot, data.data_ptr(), pitch, scales.data_ptr(),
-        sums.data_ptr(), None if out is None else out.data_ptr(), K, nat.stream()), "ic_quantize_rows")
+    meta = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    m = meta.data_ptr()
+    call("ic_quantize_rows", xr.data_ptr(), code, rows, K, xr.stride(0) if rows > 1 else K,
+         None if rr is None else rr.data_ptr(), 0 if rr is None else rr.stride(0) if rows > 1 else K,
+         None if w is None else w.data_ptr(), wcode, eps, rot, data.data_ptr(), pitch, m, m + 4 * rows,
+         None if out is None else out.data_ptr(), K, nat.raw_stream())
     if out is not None and x.device.type != "cuda":
         out = out.to(x.device)
-    return QuantizedActivations(data, scales, sums, Kp, lead), out
+    return QuantizedActivations(data, meta, Kp, lead), out
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,

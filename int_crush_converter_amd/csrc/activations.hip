@@ -26,25 +26,28 @@ template <int CTRL>
 __device__ __forceinline__ float dppf(float v) {
     return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
 }
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kXor3 = 0x1B;     // quad permutations
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E;                   // quad permutations
 constexpr int kRor4 = 0x124, kRor8 = 0x128;                 // rotations within 16 lanes
-constexpr int kMirror = 0x140;                              // lane i -> 15 - i within 16 lanes
 
-// One base-4 digit across the lanes of a quad, and one across lane bits 2, 3
-// of a row of 16: y_d = S / 2 - x_(3 - d).
+// One base-4 digit across lanes, twice its value: with the digits' values
+// x_0 .. x_3 in four lanes, 2 y_d = (x_d + x_(d^1)) + (x_(d^2) - x_(d^3)), a
+// sum, a difference and one exchange of the difference.  Across a quad:
 __device__ __forceinline__ float digit_quad(float v) {
-    const float a = v + dppf<kXor1>(v);
-    return __builtin_fmaf(a + dppf<kXor2>(a), 0.5f, -dppf<kXor3>(v));
+    const float p = v + dppf<kXor1>(v), q = v - dppf<kXor1>(v);
+    return p + dppf<kXor2>(q);
 }
-__device__ __forceinline__ float digit_row16(float v) {
-    const float a = v + dppf<kRor8>(v);          // lanes i, i ^ 8
-    const float s = a + dppf<kRor4>(a);          // a has period 8: a rotation by 4 is i ^ 4
-    return __builtin_fmaf(s, 0.5f, -dppf<kXor3>(dppf<kMirror>(v)));   // i ^ 15 ^ 3 = i ^ 12
+// and across lane bits 2 and 3 of a row of 16 (d ^ 2: 8 lanes on).  A rotation
+// by 4 brings lane i the difference of lane i - 4: that of d ^ 1 where bit 2 is
+// set, else that 8 lanes from it, which is its negative.
+__device__ __forceinline__ float digit_row16(float v, float sign) {
+    const float p = v + dppf<kRor8>(v), q = v - dppf<kRor8>(v);
+    return __builtin_fmaf(dppf<kRor4>(q), sign, p);
 }
 
 // R of order rot in {4, 16, 64, 256} on chunks of 16 consecutive columns, 16
-// consecutive lanes holding 256 columns.
-__device__ __forceinline__ void rotate16(float (&v)[16], int rot) {
+// consecutive lanes holding 256 columns; for 64 and 256 the result is 2 and 4
+// times the rotation's.
+__device__ __forceinline__ void rotate16(float (&v)[16], int rot, float sign) {
 #pragma unroll
     for (int i = 0; i < 16; i += 4) bfly4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     if (rot >= 16) {
@@ -57,29 +60,37 @@ __device__ __forceinline__ void rotate16(float (&v)[16], int rot) {
     }
     if (rot >= 256) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = digit_row16(v[i]);
+        for (int i = 0; i < 16; ++i) v[i] = digit_row16(v[i], sign);
     }
 }
 
+// op over the 64 lanes: within rows of 16 by DPP, between them by two exchanges.
+template <int CTRL, typename T>
+__device__ __forceinline__ T dpp_any(T v) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
 template <int WAVES, typename T, typename F>
 __device__ __forceinline__ T row_reduce(T v, T* lds, F op) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
+    v = op(v, dpp_any<kXor1>(v));
+    v = op(v, dpp_any<kXor2>(v));
+    v = op(v, dpp_any<kRor4>(v));
+    v = op(v, dpp_any<kRor8>(v));
+    v = op(v, __shfl_xor(v, 16, 64));
+    v = op(v, __shfl_xor(v, 32, 64));
     if (WAVES > 1) {
         const int w = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) lds[w] = v;
-        __syncthreads();
+        lds_barrier();                       // (each reduction has LDS of its own)
         v = lds[0];
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) v = op(v, lds[i]);
-        __syncthreads();
     }
     return v;
 }
 
 // WAVES waves hold one row, NC chunks of 16 columns a lane; for WAVES = 1 a
 // work-group of 4 waves holds 4 rows.
-template <int DT, int WAVES, int NC, bool FAST>
+template <int DT, int WAVES, int NC>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_kernel(
     const void* __restrict__ x, int64_t rows, int64_t cols, int64_t ld_x, const void* residual, int64_t ld_r,
     const void* __restrict__ weight, int weight_f32, float eps, int rot, int8_t* __restrict__ codes,
@@ -95,18 +106,24 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
 
     float v[NC][16];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) load16<DT, FAST>(x, row * ld_x, c * SPAN + lane * 16, cols, v[c]);
+    for (int c = 0; c < NC; ++c) load16<DT>(x, row * ld_x, c * SPAN + lane * 16, cols, v[c]);
     if (residual) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             float r[16];
-            load16<DT, FAST>(residual, row * ld_r, c * SPAN + lane * 16, cols, r);
+            load16<DT>(residual, row * ld_r, c * SPAN + lane * 16, cols, r);
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[c][i] += r[i];
-            store16<DT, FAST>(residual_out, row * ld_ro, c * SPAN + lane * 16, cols, v[c]);
+            store_cols<DT, 16>(residual_out, row * ld_ro, c * SPAN + lane * 16, cols, v[c]);
         }
     }
     if (weight) {
+        float g[NC][16];                     // on its way while the squares are summed
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (weight_f32) load16<IC_DTYPE_F32>(weight, 0, c * SPAN + lane * 16, cols, g[c]);
+            else load16<DT>(weight, 0, c * SPAN + lane * 16, cols, g[c]);
+        }
         float ss = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -115,17 +132,13 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
         ss = row_reduce<WAVES>(ss, red_f, [](float a, float b) { return a + b; });
         const float rs = 1.0f / sqrtf(ss / (float)cols + eps);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            float g[16];
-            if (weight_f32) load16<IC_DTYPE_F32, FAST>(weight, 0, c * SPAN + lane * 16, cols, g);
-            else load16<DT, FAST>(weight, 0, c * SPAN + lane * 16, cols, g);
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * rs * g[i];
-        }
+            for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * rs * g[c][i];
     }
     if (rot > 1) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) rotate16(v[c], rot);
+        for (int c = 0; c < NC; ++c) rotate16(v[c], rot, lane & 4 ? 1.0f : -1.0f);
     }
     // the maximum of the magnitudes' bits: Inf and NaN compare above every finite value
     unsigned top = 0;
@@ -135,8 +148,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
         for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[c][i]) & 0x7fffffffu);
     top = row_reduce<WAVES>(top, red_u, [](unsigned a, unsigned b) { return max(a, b); });
     const bool bad = top >= 0x7f800000u;
-    const float peak = bad ? 1.0f : fmaxf(__uint_as_float(top), kTinyMax);
-    const float inv = bad ? 0.0f : 127.0f / peak;
+    // z is `unit` times the values held; |z| / s <= 127 (1 + 2^-22), whose halves round to 127 at most
+    const float unit = rot >= 256 ? 0.25f : rot >= 64 ? 0.5f : 1.0f;
+    const float peak = bad ? 1.0f : fmaxf(__uint_as_float(top) * unit, kTinyMax);
+    const float inv = bad ? 0.0f : 127.0f / peak * unit;
     int sum = 0;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -144,15 +159,15 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
         lb_u32x4 word;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            unsigned p = 0;
+            int q[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float z = bad ? 0.0f : v[c][4 * w + k] * inv;
-                const int q = (int)__builtin_amdgcn_fmed3f(rhaz_trunc(z), -127.0f, 127.0f);
-                p |= (unsigned)(q & 255) << (8 * k);
+                const float z = v[c][4 * w + k];
+                q[k] = bad ? 0 : (int)__builtin_fmaf(z, inv, __builtin_copysignf(0.5f, z));    // truncates
             }
-            word[w] = p;
-            sum = __builtin_amdgcn_sdot4(p, 0x01010101, sum, false);
+            const unsigned lo = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(q[3], q[2], 0x04000c0c);
+            word[w] = lo | hi;
+            sum = __builtin_amdgcn_sdot4(word[w], 0x01010101, sum, false);
         }
         if (c0 < ld_q) *reinterpret_cast<lb_u32x4*>(codes + row * ld_q + c0) = word;
     }
@@ -168,7 +183,7 @@ template <int DT>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* __restrict__ codes, int64_t rows,
                                                               int64_t cols, int64_t ld_q,
                                                               const float* __restrict__ scales, void* __restrict__ out,
-                                                              int64_t ld_out, bool fast) {
+                                                              int64_t ld_out) {
     const int64_t upr = cdiv(cols, 16), total = rows * upr, stride = (int64_t)gridDim.x * 256;
     for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += stride) {
         const int64_t r = u / upr, c0 = (u - r * upr) * 16;
@@ -177,8 +192,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* __re
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * s;
-        if (fast) store16<DT, true>(out, r * ld_out, c0, cols, v);
-        else store16<DT, false>(out, r * ld_out, c0, cols, v);
+        store_cols<DT, 16>(out, r * ld_out, c0, cols, v);
     }
 }
 
@@ -200,32 +214,27 @@ struct RowArgs {
 };
 
 template <int DT, int WAVES, int NC>
-void launch_rows(const RowArgs& a, bool fast) {
+void launch_rows(const RowArgs& a) {
     const dim3 grid((unsigned)(WAVES == 1 ? cdiv(a.rows, 4) : a.rows)), block(WAVES == 1 ? 256 : 64 * WAVES);
-    if (fast)
-        hipLaunchKernelGGL((quantize_rows_kernel<DT, WAVES, NC, true>), grid, block, 0, a.st, a.x, a.rows, a.cols,
-                           a.ld_x, a.residual, a.ld_r, a.weight, a.weight_f32, a.eps, a.rot, a.codes, a.ld_q, a.scales,
-                           a.sums, a.residual_out, a.ld_ro);
-    else
-        hipLaunchKernelGGL((quantize_rows_kernel<DT, WAVES, NC, false>), grid, block, 0, a.st, a.x, a.rows, a.cols,
-                           a.ld_x, a.residual, a.ld_r, a.weight, a.weight_f32, a.eps, a.rot, a.codes, a.ld_q, a.scales,
-                           a.sums, a.residual_out, a.ld_ro);
+    hipLaunchKernelGGL((quantize_rows_kernel<DT, WAVES, NC>), grid, block, 0, a.st, a.x, a.rows, a.cols, a.ld_x,
+                       a.residual, a.ld_r, a.weight, a.weight_f32, a.eps, a.rot, a.codes, a.ld_q, a.scales, a.sums,
+                       a.residual_out, a.ld_ro);
 }
 
 template <int DT, int WAVES>
-void launch_chunks(const RowArgs& a, bool fast) {
+void launch_chunks(const RowArgs& a) {
     const int64_t nc = cdiv(a.ld_q, (int64_t)64 * WAVES * 16);
-    if (nc <= 1) launch_rows<DT, WAVES, 1>(a, fast);
-    else if (nc <= 2) launch_rows<DT, WAVES, 2>(a, fast);
-    else if (nc <= 3) launch_rows<DT, WAVES, 3>(a, fast);
-    else launch_rows<DT, WAVES, 4>(a, fast);
+    if (nc <= 1) launch_rows<DT, WAVES, 1>(a);
+    else if (nc <= 2) launch_rows<DT, WAVES, 2>(a);
+    else if (nc <= 3) launch_rows<DT, WAVES, 3>(a);
+    else launch_rows<DT, WAVES, 4>(a);
 }
 
 template <int DT>
-void launch_waves(const RowArgs& a, bool fast) {
-    if (a.ld_q <= 1024) launch_chunks<DT, 1>(a, fast);
-    else if (a.ld_q <= 16384) launch_chunks<DT, 4>(a, fast);
-    else launch_chunks<DT, 16>(a, fast);
+void launch_waves(const RowArgs& a) {
+    if (a.ld_q <= 1024) launch_chunks<DT, 1>(a);
+    else if (a.ld_q <= 16384) launch_chunks<DT, 4>(a);
+    else launch_chunks<DT, 16>(a);
 }
 
 }  // namespace
@@ -254,15 +263,12 @@ extern "C" int ic_quantize_rows(const void* x, int dtype, int64_t rows, int64_t 
     IC_REQUIRE(ld_q == ic_activation_pitch(cols_pad) && aligned16(codes),
                "ic_quantize_rows: codes need ic_activation_pitch columns and 16-byte alignment");
     const int64_t es = dtype == IC_DTYPE_F32 ? 4 : 2;
-    auto whole = [&](const void* p, int64_t ld) { return !p || (aligned16(p) && ld * es % 16 == 0); };
-    const bool fast = cols % 16 == 0 && whole(x, ld_x) && whole(residual, ld_r) && whole(residual_out, ld_ro) &&
-                      whole(weight, 16);
     RowArgs a{x, rows, cols, ld_x, residual, ld_r, weight, weight && weight_dtype == IC_DTYPE_F32, eps, rot, codes, ld_q, scales, sums,
               residual_out, ld_ro, as_stream(stream)};
     ProfScope prof(a.st, PT_OTHER, 0.0, (double)rows * cols * (es * (residual ? 3 : 1) + 1));
-    if (dtype == IC_DTYPE_F32) launch_waves<IC_DTYPE_F32>(a, fast);
-    else if (dtype == IC_DTYPE_BF16) launch_waves<IC_DTYPE_BF16>(a, fast);
-    else launch_waves<IC_DTYPE_F16>(a, fast);
+    if (dtype == IC_DTYPE_F32) launch_waves<IC_DTYPE_F32>(a);
+    else if (dtype == IC_DTYPE_BF16) launch_waves<IC_DTYPE_BF16>(a);
+    else launch_waves<IC_DTYPE_F16>(a);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
@@ -276,17 +282,16 @@ extern "C" int ic_dequantize_rows(const int8_t* codes, int64_t rows, int64_t col
     IC_REQUIRE(ld_q >= cdiv(cols, 16) * 16 && ld_q % 16 == 0 && aligned16(codes) && ld_out >= cols,
                "ic_dequantize_rows: rows of codes need a pitch of whole 16-byte words");
     const int64_t es = dtype == IC_DTYPE_F32 ? 4 : 2;
-    const bool fast = cols % 16 == 0 && aligned16(out) && ld_out * es % 16 == 0;
     const int64_t grid = cdiv(rows * cdiv(cols, 16), 256);
     const dim3 g((unsigned)(grid < 65536 ? grid : 65536)), b(256);
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 0.0, (double)rows * cols * (es + 1));
     if (dtype == IC_DTYPE_F32)
-        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_F32>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out, fast);
+        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_F32>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out);
     else if (dtype == IC_DTYPE_BF16)
-        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_BF16>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out, fast);
+        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_BF16>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out);
     else
-        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_F16>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out, fast);
+        hipLaunchKernelGGL(dequantize_rows_kernel<IC_DTYPE_F16>, g, b, 0, st, codes, rows, cols, ld_q, scales, out, ld_out);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }

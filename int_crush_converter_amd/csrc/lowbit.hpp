@@ -50,18 +50,17 @@ typedef float lb_f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int lb_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int lb_u32x2 __attribute__((ext_vector_type(2)));
 
-// 16 consecutive elements of a row as fp32; FAST: the row is made of whole
-// 16-element chunks at 16-byte aligned addresses.
-template <int DT, bool FAST>
+// Vectors of 16 bytes at the alignment of their elements: gfx950 loads and
+// stores them whole at any such address.
+typedef float lb_f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned int lb_u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// 16 consecutive elements of a row as fp32, zeros behind the last column.
+template <int DT>
 __device__ __forceinline__ void load16(const void* p, int64_t base, int64_t c0, int64_t cols, float (&v)[16]) {
-    if (c0 >= cols) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-        return;
-    }
-    if (FAST) {
+    if (c0 + 16 <= cols) {
         if (DT == IC_DTYPE_F32) {
-            const lb_f32x4* q = reinterpret_cast<const lb_f32x4*>(static_cast<const float*>(p) + base + c0);
+            const lb_f32x4_any* q = reinterpret_cast<const lb_f32x4_any*>(static_cast<const float*>(p) + base + c0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const lb_f32x4 t = q[i];
@@ -69,7 +68,7 @@ __device__ __forceinline__ void load16(const void* p, int64_t base, int64_t c0, 
                 for (int k = 0; k < 4; ++k) v[4 * i + k] = t[k];
             }
         } else {
-            const lb_u32x4* q = reinterpret_cast<const lb_u32x4*>(static_cast<const uint16_t*>(p) + base + c0);
+            const lb_u32x4_any* q = reinterpret_cast<const lb_u32x4_any*>(static_cast<const uint16_t*>(p) + base + c0);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const lb_u32x4 t = q[i];
@@ -86,18 +85,18 @@ __device__ __forceinline__ void load16(const void* p, int64_t base, int64_t c0, 
     }
 }
 
-template <int DT, bool FAST>
-__device__ __forceinline__ void store16(void* p, int64_t base, int64_t c0, int64_t cols, const float (&v)[16]) {
-    if (c0 >= cols) return;
-    if (FAST) {
+// N (8 or 16) consecutive elements of a row, those before the last column.
+template <int DT, int N>
+__device__ __forceinline__ void store_cols(void* p, int64_t base, int64_t c0, int64_t cols, const float (&v)[N]) {
+    if (c0 + N <= cols) {
         if (DT == IC_DTYPE_F32) {
-            lb_f32x4* q = reinterpret_cast<lb_f32x4*>(static_cast<float*>(p) + base + c0);
+            lb_f32x4_any* q = reinterpret_cast<lb_f32x4_any*>(static_cast<float*>(p) + base + c0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = lb_f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+            for (int i = 0; i < N / 4; ++i) q[i] = lb_f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
         } else {
-            lb_u32x4* q = reinterpret_cast<lb_u32x4*>(static_cast<uint16_t*>(p) + base + c0);
+            lb_u32x4_any* q = reinterpret_cast<lb_u32x4_any*>(static_cast<uint16_t*>(p) + base + c0);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < N / 8; ++i) {
                 lb_u32x4 t;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) t[k] = pack_half_words<DT>(v[8 * i + 2 * k], v[8 * i + 2 * k + 1]);
@@ -106,7 +105,7 @@ __device__ __forceinline__ void store16(void* p, int64_t base, int64_t c0, int64
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < N; ++i)
             if (c0 + i < cols) store_from_f32(p, DT, base + c0 + i, v[i]);
     }
 }

@@ -50,52 +50,46 @@ __device__ __forceinline__ lb_u32x4 quantize_block(float (&a)[16], float (&b)[16
 template <int DT>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const void* __restrict__ x, int64_t rows, int64_t cols,
                                                              int64_t ld, lb_u32x4* __restrict__ codes,
-                                                             uint8_t* __restrict__ scales, int64_t tiles, bool fast) {
+                                                             uint8_t* __restrict__ scales, int64_t tiles) {
     const int lane = threadIdx.x & 63, j = threadIdx.x >> 6;
     const int64_t row = (int64_t)blockIdx.y * 16 + (lane & 15), t = (int64_t)blockIdx.x * 4 + j;
     const int64_t c0 = t * 128 + (lane >> 4) * 32;
     float a[16], b[16];
     const int64_t n = row < rows ? cols : 0;
-    if (fast) {
-        load16<DT, true>(x, row * ld, c0, n, a);
-        load16<DT, true>(x, row * ld, c0 + 16, n, b);
-    } else {
-        load16<DT, false>(x, row * ld, c0, n, a);
-        load16<DT, false>(x, row * ld, c0 + 16, n, b);
-    }
+    load16<DT>(x, row * ld, c0, n, a);
+    load16<DT>(x, row * ld, c0 + 16, n, b);
     unsigned s;
     const lb_u32x4 w = quantize_block(a, b, s);
     if (t < tiles) codes[((int64_t)blockIdx.y * tiles + t) * 64 + lane] = w;
     scales[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 64 + lane) * 4 + j] = (uint8_t)s;
 }
 
-__device__ __forceinline__ float e2m1(unsigned nibble) {
-    const unsigned m = nibble & 7;
-    const float v = m < 2 ? 0.5f * m : __uint_as_float(((126 + (m >> 1)) << 23) | ((m & 1) << 22));
-    return nibble & 8 ? -v : v;
-}
-__device__ __forceinline__ float e8m0(unsigned s) {
-    return s == 255 ? __uint_as_float(0x7fc00000u) : s ? __uint_as_float(s << 23) : __uint_as_float(1u << 22);
-}
-
+// One wave per tile again, but a lane takes 8 columns of one row at a time, so
+// that 16 lanes write 128 consecutive values.
 template <int DT>
-__global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const lb_u32x4* __restrict__ codes,
+__global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales, int64_t rows,
                                                                int64_t cols, void* __restrict__ out, int64_t ld,
-                                                               int64_t tiles, bool fast) {
-    const int lane = threadIdx.x & 63, j = threadIdx.x >> 6;
-    const int64_t row = (int64_t)blockIdx.y * 16 + (lane & 15), t = (int64_t)blockIdx.x * 4 + j;
-    const int64_t c0 = t * 128 + (lane >> 4) * 32;
-    if (row >= rows || c0 >= cols) return;
-    const lb_u32x4 w = codes[((int64_t)blockIdx.y * tiles + t) * 64 + lane];
-    const float s = e8m0(scales[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 64 + lane) * 4 + j]);
-    float v[2][16];
+                                                               int64_t tiles) {
+    const int lane = threadIdx.x & 63, j = threadIdx.x >> 6, part = lane & 15, g = part >> 2;
+    const int64_t t = (int64_t)blockIdx.x * 4 + j, c0 = t * 128 + part * 8;
+    if (c0 >= cols) return;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i >> 4][i & 15] = e2m1((w[i >> 3] >> (4 * (i & 7))) & 15) * s;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if (fast) store16<DT, true>(out, row * ld, c0 + 16 * h, cols, v[h]);
-        else store16<DT, false>(out, row * ld, c0 + 16 * h, cols, v[h]);
+    for (int k = 0; k < 4; ++k) {
+        const int r = k * 4 + (lane >> 4);
+        const int64_t row = (int64_t)blockIdx.y * 16 + r;
+        if (row >= rows) return;
+        const uint32_t w = codes[(((int64_t)blockIdx.y * tiles + t) * 64 + g * 16 + r) * 4 + (part & 3)];
+        const unsigned e = scales[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 64 + g * 16 + r) * 4 + j];
+        // (2^-127 is no normal number: such a block is taken at 2^-126 and halved, which is exact)
+        const float s = __uint_as_float((e ? e : 1u) << 23);
+        float v[8];
+        const lb_f32x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+        const lb_f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+        const float unit = e == 255 ? __uint_as_float(0x7fc00000u) : e ? 1.0f : 0.5f;
+        v[0] = p0[0] * unit; v[1] = p0[1] * unit; v[2] = p1[0] * unit; v[3] = p1[1] * unit;
+        v[4] = p2[0] * unit; v[5] = p2[1] * unit; v[6] = p3[0] * unit; v[7] = p3[1] * unit;
+        store_cols<DT, 8>(out, row * ld, c0, cols, v);
     }
 }
 
@@ -158,7 +152,6 @@ extern "C" int ic_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t
     IC_REQUIRE(x && codes && scales, "ic_mxfp4_quantize: null pointer");
     IC_REQUIRE(ld_x >= cols && aligned16(codes), "ic_mxfp4_quantize: leading dimension below cols, or codes not 16-byte aligned");
     const int64_t es = dtype == IC_DTYPE_F32 ? 4 : 2;
-    const bool fast = cols % 16 == 0 && aligned16(x) && ld_x * es % 16 == 0;
     const dim3 g((unsigned)cdiv(cols, 512), (unsigned)cdiv(rows, 16)), b(256);
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 0.0, (double)rows * cols * (es + 17.0 / 32));
@@ -166,11 +159,11 @@ extern "C" int ic_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t
     uint8_t* s = static_cast<uint8_t*>(scales);
     const int64_t tiles = cdiv(cols, 128);
     if (dtype == IC_DTYPE_F32)
-        hipLaunchKernelGGL(mxfp4_quantize_kernel<IC_DTYPE_F32>, g, b, 0, st, x, rows, cols, ld_x, c, s, tiles, fast);
+        hipLaunchKernelGGL(mxfp4_quantize_kernel<IC_DTYPE_F32>, g, b, 0, st, x, rows, cols, ld_x, c, s, tiles);
     else if (dtype == IC_DTYPE_BF16)
-        hipLaunchKernelGGL(mxfp4_quantize_kernel<IC_DTYPE_BF16>, g, b, 0, st, x, rows, cols, ld_x, c, s, tiles, fast);
+        hipLaunchKernelGGL(mxfp4_quantize_kernel<IC_DTYPE_BF16>, g, b, 0, st, x, rows, cols, ld_x, c, s, tiles);
     else
-        hipLaunchKernelGGL(mxfp4_quantize_kernel<IC_DTYPE_F16>, g, b, 0, st, x, rows, cols, ld_x, c, s, tiles, fast);
+        hipLaunchKernelGGL(mxfp4_quantize_kernel<IC_DTYPE_F16>, g, b, 0, st, x, rows, cols, ld_x, c, s, tiles);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
@@ -183,19 +176,18 @@ extern "C" int ic_mxfp4_dequantize(const void* codes, const void* scales, int64_
     IC_REQUIRE(codes && scales && out, "ic_mxfp4_dequantize: null pointer");
     IC_REQUIRE(ld_out >= cols && aligned16(codes), "ic_mxfp4_dequantize: leading dimension below cols, or codes not 16-byte aligned");
     const int64_t es = dtype == IC_DTYPE_F32 ? 4 : 2;
-    const bool fast = cols % 16 == 0 && aligned16(out) && ld_out * es % 16 == 0;
     const dim3 g((unsigned)cdiv(cols, 512), (unsigned)cdiv(rows, 16)), b(256);
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 0.0, (double)rows * cols * (es + 17.0 / 32));
-    const lb_u32x4* c = static_cast<const lb_u32x4*>(codes);
+    const uint32_t* c = static_cast<const uint32_t*>(codes);
     const uint8_t* s = static_cast<const uint8_t*>(scales);
     const int64_t tiles = cdiv(cols, 128);
     if (dtype == IC_DTYPE_F32)
-        hipLaunchKernelGGL(mxfp4_dequantize_kernel<IC_DTYPE_F32>, g, b, 0, st, c, s, rows, cols, out, ld_out, tiles, fast);
+        hipLaunchKernelGGL(mxfp4_dequantize_kernel<IC_DTYPE_F32>, g, b, 0, st, c, s, rows, cols, out, ld_out, tiles);
     else if (dtype == IC_DTYPE_BF16)
-        hipLaunchKernelGGL(mxfp4_dequantize_kernel<IC_DTYPE_BF16>, g, b, 0, st, c, s, rows, cols, out, ld_out, tiles, fast);
+        hipLaunchKernelGGL(mxfp4_dequantize_kernel<IC_DTYPE_BF16>, g, b, 0, st, c, s, rows, cols, out, ld_out, tiles);
     else
-        hipLaunchKernelGGL(mxfp4_dequantize_kernel<IC_DTYPE_F16>, g, b, 0, st, c, s, rows, cols, out, ld_out, tiles, fast);
+        hipLaunchKernelGGL(mxfp4_dequantize_kernel<IC_DTYPE_F16>, g, b, 0, st, c, s, rows, cols, out, ld_out, tiles);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }

@@ -11,13 +11,16 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
-from .activations import MAX_FEATURES, QuantizedActivations, as_rows, check_gpu
+from .activations import MAX_FEATURES, QuantizedActivations, as_rows, call
 
 MAX_ROWS = 1048560
 
 
+_DTYPES = {torch.float32: nat.DT_F32, torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16}
+
+
 def _out_code(out_dtype: torch.dtype) -> int:
-    code = {torch.float32: nat.DT_F32, torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16}.get(out_dtype)
+    code = _DTYPES.get(out_dtype)
     if code is None:
         raise TypeError(f"unsupported dtype {out_dtype}")
     return code
@@ -28,7 +31,7 @@ def _bias(bias: torch.Tensor | None, N: int):
         return None, 0
     if bias.shape != (N,):
         raise ValueError(f"bias has shape {tuple(bias.shape)}, expected ({N},)")
-    b = check_gpu("bias", bias).contiguous()
+    b = nat.on_gpu("bias", bias).contiguous()
     return b, nat.dtype_code(b)
 
 
@@ -54,18 +57,17 @@ class QuantizedWeight:
             raise ValueError(f"in_features must be in [1, {MAX_FEATURES}] and out_features in [1, {MAX_ROWS}], got {K}, {N}")
         if scales.numel() != N or (zero_points is not None and zero_points.numel() != N):
             raise ValueError(f"{N} rows need {N} scales and zero-points: one a row")
-        s = check_gpu("scales", scales).reshape(-1)
+        s = nat.on_gpu("scales", scales).reshape(-1)
         self.scales = (s if s.dtype in (torch.float16, torch.float32) else s.float()).contiguous()
         self.scale_kind = 0 if self.scales.dtype == torch.float16 else 1
         if zero_points is not None and zero_points.dtype != torch.int8:
             raise ValueError(f"zero_points must be int8, got {zero_points.dtype}")
-        self.zero_points = None if zero_points is None else check_gpu("zero_points", zero_points).reshape(-1).contiguous()
+        self.zero_points = None if zero_points is None else nat.on_gpu("zero_points", zero_points).reshape(-1).contiguous()
         self.bits, self.in_features, self.out_features = bits, K, N
-        rows = as_rows(check_gpu("stored", stored))
-        L = nat.lib()
-        self.tiles = nat.workspace(L.ic_linear_weight_bytes(N, K, bits), rows.device)
-        nat.check(L.ic_linear_pack_weight(rows, bits, N, K, rows.stride(0) if N > 1 else width, self.tiles,
-                                          nat.stream()), "ic_linear_pack_weight")
+        rows = as_rows(nat.on_gpu("stored", stored))
+        self.tiles = nat.workspace(nat.lib().ic_linear_weight_bytes(N, K, bits), rows.device)
+        call("ic_linear_pack_weight", rows.data_ptr(), bits, N, K, rows.stride(0) if N > 1 else width,
+             self.tiles.data_ptr(), nat.raw_stream())
 
 
 def quantized_linear(x: QuantizedActivations, weight: QuantizedWeight, bias: torch.Tensor | None = None, *,
@@ -79,10 +81,8 @@ def quantized_linear(x: QuantizedActivations, weight: QuantizedWeight, bias: tor
     code = _out_code(out_dtype)
     b, bcode = _bias(bias, N)
     out = torch.empty((*x.lead, N), dtype=out_dtype, device=data.device)
-    z = w.zero_points
-    nat.check(nat.lib().ic_quantized_linear(
-        data.data_ptr(), data.shape[1], x.scales.data_ptr(), x.sums.data_ptr(), data.shape[0], w.tiles.data_ptr(),
-        w.bits, w.scales.data_ptr(), w.scale_kind, None if z is None else z.data_ptr(),
-        None if b is None else b.data_ptr(), bcode, N, w.in_features, out.data_ptr(), code, N, nat.stream()),
-        "ic_quantized_linear")
+    z, rows, m = w.zero_points, data.shape[0], x.meta.data_ptr()
+    call("ic_quantized_linear", data.data_ptr(), data.shape[1], m, m + 4 * rows, rows, w.tiles.data_ptr(), w.bits,
+         w.scales.data_ptr(), w.scale_kind, None if z is None else z.data_ptr(), None if b is None else b.data_ptr(),
+         bcode, N, w.in_features, out.data_ptr(), code, N, nat.raw_stream())
     return out

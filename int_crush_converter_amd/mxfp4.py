@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
-from .activations import MAX_FEATURES, as_rows, check_gpu
+from .activations import MAX_FEATURES, as_rows, call
 from .linear import MAX_ROWS, _bias, _out_code
 
 BLOCK = 32
@@ -50,13 +50,13 @@ class Mxfp4Tensor:
             raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold {K} columns")
         rows = codes.numel() // have
         _sizes(rows, K)
-        c, s = check_gpu("codes", codes), check_gpu("scales", scales)
+        c, s = nat.on_gpu("codes", codes), nat.on_gpu("scales", scales)
         t = cls._empty(lead, rows, K, c.device)
         if rows:
             c, s = as_rows(c), as_rows(s)
-            nat.check(nat.lib().ic_mxfp4_relayout(
-                c, c.stride(0) if rows > 1 else have, s, s.stride(0) if rows > 1 else s.shape[1], rows, K, t.tiles,
-                t.scales, 1, nat.stream()), "ic_mxfp4_relayout")
+            call("ic_mxfp4_relayout", c.data_ptr(), c.stride(0) if rows > 1 else have, s.data_ptr(),
+                 s.stride(0) if rows > 1 else s.shape[1], rows, K, t.tiles.data_ptr(), t.scales.data_ptr(), 1,
+                 nat.raw_stream())
         return t
 
     def to_packed(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -65,17 +65,16 @@ class Mxfp4Tensor:
         c = torch.empty((rows, (K + 1) // 2), dtype=torch.uint8, device=dev)
         s = torch.empty((rows, -(-K // BLOCK)), dtype=torch.uint8, device=dev)
         if rows:
-            nat.check(nat.lib().ic_mxfp4_relayout(c, c.shape[1], s, s.shape[1], rows, K, self.tiles, self.scales, 0,
-                                                  nat.stream()), "ic_mxfp4_relayout")
+            call("ic_mxfp4_relayout", c.data_ptr(), c.shape[1], s.data_ptr(), s.shape[1], rows, K,
+                 self.tiles.data_ptr(), self.scales.data_ptr(), 0, nat.raw_stream())
         return c.reshape(*self.lead, c.shape[1]), s.reshape(*self.lead, s.shape[1])
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values [*lead, in_features] in ``dtype`` (exact in bfloat16 and float32)."""
         K = self.in_features
         out = torch.empty((*self.lead, K), dtype=dtype, device=self.tiles.device)
-        nat.check(nat.lib().ic_mxfp4_dequantize(self.tiles.data_ptr(), self.scales.data_ptr(), self.rows, K,
-                                                out.data_ptr(), _out_code(dtype), K, nat.stream()),
-                  "ic_mxfp4_dequantize")
+        call("ic_mxfp4_dequantize", self.tiles.data_ptr(), self.scales.data_ptr(), self.rows, K, out.data_ptr(),
+             _out_code(dtype), K, nat.raw_stream())
         return out
 
 
@@ -87,14 +86,13 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4Tensor:
     K = x.shape[-1]
     rows = x.numel() // K if K else 0
     _sizes(rows, K)
-    xg = check_gpu("x", x)
+    xg = nat.on_gpu("x", x)
     code = nat.dtype_code(xg)
     t = Mxfp4Tensor._empty(x.shape[:-1], rows, K, xg.device)
     if rows:
         xr = as_rows(xg)
-        nat.check(nat.lib().ic_mxfp4_quantize(xr.data_ptr(), code, rows, K, xr.stride(0) if rows > 1 else K,
-                                              t.tiles.data_ptr(), t.scales.data_ptr(), nat.stream()),
-                  "ic_mxfp4_quantize")
+        call("ic_mxfp4_quantize", xr.data_ptr(), code, rows, K, xr.stride(0) if rows > 1 else K, t.tiles.data_ptr(),
+             t.scales.data_ptr(), nat.raw_stream())
     return t
 
 
@@ -111,8 +109,7 @@ def mxfp4_linear(x: Mxfp4Tensor, weight: Mxfp4Tensor, bias: torch.Tensor | None 
     code = _out_code(out_dtype)
     b, bcode = _bias(bias, N)
     out = torch.empty((*x.lead, N), dtype=out_dtype, device=x.tiles.device)
-    nat.check(nat.lib().ic_mxfp4_linear(
-        x.tiles.data_ptr(), x.scales.data_ptr(), x.rows, weight.tiles.data_ptr(), weight.scales.data_ptr(),
-        None if b is None else b.data_ptr(), bcode, N, x.in_features, out.data_ptr(), code, N, nat.stream()),
-        "ic_mxfp4_linear")
+    call("ic_mxfp4_linear", x.tiles.data_ptr(), x.scales.data_ptr(), x.rows, weight.tiles.data_ptr(),
+         weight.scales.data_ptr(), None if b is None else b.data_ptr(), bcode, N, x.in_features, out.data_ptr(), code, N,
+         nat.raw_stream())
     return out
