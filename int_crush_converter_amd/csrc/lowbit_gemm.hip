@@ -143,6 +143,17 @@ __device__ __forceinline__ f32x16 mma32_mx(lb_u32x4 w, lb_u32x4 x, f32x16 acc, i
 __device__ __forceinline__ lb_u32x4 low_nibbles(lb_u32x4 p) { return (p << 4) & 0xf0f0f0f0u; }
 __device__ __forceinline__ lb_u32x4 high_nibbles(lb_u32x4 p) { return p & 0xf0f0f0f0u; }
 
+// The 16 bytes that lane `from` holds.  Activations are loaded with four lanes
+// on 64 consecutive bytes of a row (an operand's own order, 16 rows in 16
+// consecutive lanes, makes 64 requests of a load instead of 16) and then
+// exchanged into an operand's order.
+__device__ __forceinline__ lb_u32x4 to_operand(lb_u32x4 v, int from) {
+    lb_u32x4 o;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = (uint32_t)__builtin_amdgcn_ds_bpermute(from * 4, (int)v[k]);
+    return o;
+}
+
 // Few rows: a work-group of WAVES waves takes 16 columns of y and 16 MT rows,
 // its waves a share of K each; the sums are joined in LDS in a fixed order.
 template <int KIND, int MT, int WAVES>
@@ -167,8 +178,8 @@ __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
             xt[i] = reinterpret_cast<const lb_u32x4*>(p.a) + mt * tiles * 64 + lane;
             xs[i] = p.a_scale + mt * words * 64 + lane;
         } else {
-            const int64_t m = (mt0 + i) * 16 + r < p.M ? (mt0 + i) * 16 + r : p.M - 1;
-            row[i] = p.a + m * p.ld_a + g * 16;
+            const int64_t m = (mt0 + i) * 16 + (lane >> 2) < p.M ? (mt0 + i) * 16 + (lane >> 2) : p.M - 1;
+            row[i] = p.a + m * p.ld_a + (lane & 3) * 16;
         }
     }
     const uint32_t* ws = KIND == kMx ? p.w_scale + nt * words * 64 + lane : nullptr;
@@ -192,8 +203,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const lb_u32x4* x = reinterpret_cast<const lb_u32x4*>(row[i] + t * 128);
-                acc[i] = mma_i8(w0, x[0], acc[i]);
-                acc[i] = mma_i8(w1, x[4], acc[i]);
+                const lb_u32x4 x0 = x[0], x1 = x[4];
+                acc[i] = mma_i8(w0, to_operand(x0, r * 4 + g), acc[i]);
+                acc[i] = mma_i8(w1, to_operand(x1, r * 4 + g), acc[i]);
             }
         }
     }
@@ -666,8 +678,8 @@ void launch_tiled(const Operands& p, hipStream_t st) {
 // and leaves CUs idle when there are few; then tiles of 256 x 256 where they
 // fill at least three quarters of their rounds over the 256 CUs, else of
 // 128 x 128.  Measured, us (direct / 128 / 256):
-//   INT4 M 128 4096x4096 (512 work-groups)  19 / 23 / 49;  M 200 (1024)  30 / 23 / 49
-//   INT4 M 2048 4096x4096 (256-tiles fill 1/2)  245 / 43 / 54;  M 3000 (3/4)  - / 60 / 59
+//   INT8 M 128 4096x4096 (512 work-groups)  15 / 25 / 52;  M 333 (1536)  46 / 25 / 52
+//   INT4 M 2048 4096x4096 (256-tiles fill 1/2)  - / 43 / 54;  M 3000 (3/4)  - / 60 / 59
 //   INT4 M 4096 12288x4096 (all)  - / 215 / 189
 //   MXFP4 M 200 4096x4096 (1024)  14 / 15 / 29;  M 333 (1536)  20 / 16 / 30
 //   MXFP4 M 2048 4096x4096 (1/2)  81 / 27 / 34;  M 4096 12288x4096 (all)  - / 131 / 118
@@ -677,7 +689,7 @@ int launch_linear(const Operands& p, hipStream_t st) {
     const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256);
     if (p.M <= 16) launch_direct<KIND, 1, 8>(p, st);
     else if (p.M <= 32) launch_direct<KIND, 2, 8>(p, st);
-    else if (p.M <= 64 || groups < (KIND == kMx ? 1100 : 700)) launch_direct<KIND, 4, 8>(p, st);
+    else if (p.M <= 64 || groups < 1000) launch_direct<KIND, 4, 8>(p, st);
     else if (tiles * 4 >= cdiv(tiles, 256) * 256 * 3) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
     else launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4>(p, st);
     IC_CHECK_LAUNCH();
