@@ -156,6 +156,9 @@ __device__ __forceinline__ lb_u32x4 to_operand(lb_u32x4 v, int from) {
 
 // Few rows: a work-group of WAVES waves takes 16 columns of y and 16 MT rows,
 // its waves a share of K each; the sums are joined in LDS in a fixed order.
+// One row is bound by the weights' bytes and the launch: INT4 1 x 12288 x 4096
+// 6.4 us (25 MB, 4.0 TB/s); more rows by their activations, which every
+// work-group reads again: INT8 333 x 1000 x 2901 10.7 us.
 template <int KIND, int MT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
     typedef typename Acc<KIND>::T acc_t;
@@ -243,6 +246,15 @@ __device__ __forceinline__ void meet() {
 // matrix instructions, so a wave waits neither for LDS nor long at the one
 // barrier that a stage has: when it gets there, what is left of the stage is
 // in registers, and its buffer is filled again.
+//
+// Measured: INT4 8192 x 4096 x 12288 312 us, 2.6 POP/s; MXFP4 8192 x 12288 x
+// 4096 222 us, 3.7 PFLOP/s.  What bounds the first is power: the chip clocks
+// at 1.75 GHz under it, its matrix units are busy for 65 % of the cycles, and
+// the same instructions with the same reads from LDS and nothing else reach
+// 2.7 POP/s on random operands (5.4 PFLOP/s for E2M1; 3.5 and 6.5 from
+// registers alone).  The second loses a fifth to the ends of its 32-stage
+// tiles.  4 waves of 128 x 128 read less LDS but took 383 and 301 us, a wave
+// alone on its SIMD standing still at copies, barriers and outputs.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
     typedef typename Acc32<KIND>::T acc_t;
@@ -749,6 +761,7 @@ extern "C" int ic_quantized_linear(const int8_t* a, int64_t ld_a, const float* s
     IC_REQUIRE(ld_a >= cdiv(K, kActPad) * kActPad && ld_a % 16 == 0 && aligned16(a) && aligned16(tiles),
                "ic_quantized_linear: activations need rows of ic_activation_pitch codes, 16-byte aligned");
     IC_REQUIRE(ld_out >= N, "ic_quantized_linear: ld_out below N");
+    if (ld_a > (1 << 20)) return fail(IC_ERR_RANGE, "ic_quantized_linear: at most 2^20 for ld_a");   // (a lane's 32-bit offset in 256 rows)
     p.wide = aligned16(out) && ld_out % (out_dtype == IC_DTYPE_F32 ? 4 : 8) == 0 && N % 8 == 0;
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 2.0 * M * N * K, (double)M * K + (double)N * K * bits / 8);
