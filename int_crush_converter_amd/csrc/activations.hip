@@ -152,10 +152,13 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
         for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[c][i]) & 0x7fffffffu);
     top = row_reduce<WAVES>(top, red_u, [](unsigned a, unsigned b) { return max(a, b); });
     const bool bad = top >= 0x7f800000u;
-    // z is `unit` times the values held; |z| / s <= 127 (1 + 2^-22), whose halves round to 127 at most
+    // z is `unit` times the values held; |z| / s <= 127 (1 + 2^-22), whose halves round to 127 at most.  The factor
+    // 127 / peak is held as two fp32 values: with the first alone, whose rounding may lie below, a half (z = peak / 2
+    // gives 63.5) would now and then round towards zero.
     const float unit = rot >= 256 ? 0.25f : rot >= 64 ? 0.5f : 1.0f;
     const float peak = bad ? 1.0f : fmaxf(__uint_as_float(top) * unit, kTinyMax);
-    const float inv = bad ? 0.0f : 127.0f / peak * unit;
+    const float ratio = 127.0f / peak;
+    const float inv = bad ? 0.0f : ratio * unit, rest = bad ? 0.0f : __builtin_fmaf(-ratio, peak, 127.0f) / peak * unit;
     int sum = 0;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -167,7 +170,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float z = v[c][4 * w + k];
-                q[k] = bad ? 0 : (int)__builtin_fmaf(z, inv, __builtin_copysignf(0.5f, z));    // truncates
+                q[k] = bad ? 0 : (int)__builtin_fmaf(z, inv, __builtin_fmaf(z, rest, __builtin_copysignf(0.5f, z)));    // truncates
             }
             const unsigned lo = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(q[3], q[2], 0x04000c0c);
             word[w] = lo | hi;
