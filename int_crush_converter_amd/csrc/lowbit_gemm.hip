@@ -695,15 +695,20 @@ void launch_tiled(const Operands& p, hipStream_t st) {
 //   INT4 M 4096 12288x4096 (all)  - / 215 / 189
 //   MXFP4 M 200 4096x4096 (1024)  14 / 15 / 29;  M 333 (1536)  20 / 16 / 30
 //   MXFP4 M 2048 4096x4096 (1/2)  81 / 27 / 34;  M 4096 12288x4096 (all)  - / 131 / 118
+int linear_form(int64_t M, int64_t N) {      // 0, 128 or 256
+    const int64_t groups = cdiv(N, 16) * cdiv(M, 64), tiles = cdiv(M, 256) * cdiv(N, 256);
+    if (M <= 64 || groups < 1000) return 0;
+    return tiles * 4 >= cdiv(tiles, 256) * 256 * 3 ? 256 : 128;
+}
+
 template <int KIND>
 int launch_linear(const Operands& p, hipStream_t st) {
-    const int64_t groups = cdiv(p.N, 16) * cdiv(p.M, 64);
-    const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256);
-    if (p.M <= 16) launch_direct<KIND, 1, 8>(p, st);
+    const int form = linear_form(p.M, p.N);
+    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
+    else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4>(p, st);
+    else if (p.M <= 16) launch_direct<KIND, 1, 8>(p, st);
     else if (p.M <= 32) launch_direct<KIND, 2, 8>(p, st);
-    else if (p.M <= 64 || groups < 1000) launch_direct<KIND, 4, 8>(p, st);
-    else if (tiles * 4 >= cdiv(tiles, 256) * 256 * 3) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
-    else launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4>(p, st);
+    else launch_direct<KIND, 4, 8>(p, st);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
@@ -722,6 +727,8 @@ int check_product(const char* who, const Operands& p) {
 }  // namespace icq
 
 using namespace icq;
+
+extern "C" int ic_linear_form(int64_t M, int64_t N) { return M < 0 || N < 1 ? IC_ERR_ARG : linear_form(M, N); }
 
 extern "C" int64_t ic_linear_weight_bytes(int64_t N, int64_t K, int bits) {
     if (N < 0 || K < 0 || (bits != 4 && bits != 8)) return 0;
