@@ -223,8 +223,8 @@ def lib():
 
 
 def entry(name: str):
-    """The bare ctypes function, for calls that take device addresses (ints) of tensors their caller has checked:
-    some microseconds less than the checked one, which counts where a whole call takes ten."""
+    """The bare ctypes function, for calls that take device addresses (ints) of tensors their caller has checked
+    (``stream_for``): some microseconds less than the checked one, which counts where a whole call takes ten."""
     return getattr(lib().cdll, name)
 
 
@@ -258,8 +258,14 @@ def stream() -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def raw_stream() -> int:
-    return stream() if _raw_stream is None else _raw_stream(torch.cuda.current_device())
+def stream_for(*tensors) -> int:
+    """The current stream's handle, for a call with these tensors' addresses.  All have to lie in the memory of the
+    current GPU: its kernels would run there whatever the tensors' own device is.  None is passed over."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"an operand is on {t.device}, the current device is cuda:{dev}")
+    return stream() if _raw_stream is None else _raw_stream(dev)
 
 
 def device() -> torch.device:

@@ -32,7 +32,7 @@ _entries: dict[str, object] = {}
 
 
 def call(name: str, *args) -> None:
-    """A library call with device addresses, checked tensors behind them."""
+    """A library call with the addresses of tensors that ``nat.stream_for`` has checked."""
     fn = _entries.get(name)
     if fn is None:
         fn = _entries[name] = nat.entry(name)
@@ -82,7 +82,8 @@ class QuantizedActivations:
             data[:, :K] = codes
         else:
             data = codes
-        call("ic_row_sums_i8", data.data_ptr(), rows, K, data.shape[1], meta.data_ptr() + 4 * rows, nat.raw_stream())
+        call("ic_row_sums_i8", data.data_ptr(), rows, K, data.shape[1], meta.data_ptr() + 4 * rows,
+             nat.stream_for(data, meta))
         return cls(data, meta, K, lead)
 
     @property
@@ -94,9 +95,10 @@ class QuantizedActivations:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values ``q * s`` [*lead, in_features], rounded once to ``dtype``."""
         K, data = self.in_features, self.data
+        stream = nat.stream_for(data, self.meta)
         out = torch.empty((*self.lead, K), dtype=dtype, device=data.device)
         call("ic_dequantize_rows", data.data_ptr(), data.shape[0], K, data.shape[1], self.meta.data_ptr(),
-             out.data_ptr(), nat.dtype_code(out), K, nat.raw_stream())
+             out.data_ptr(), nat.dtype_code(out), K, stream)
         return out
 
 
@@ -138,7 +140,7 @@ def _quantize(x, weight, residual, eps, rot_size):
     call("ic_quantize_rows", xr.data_ptr(), code, rows, K, xr.stride(0) if rows > 1 else K,
          None if rr is None else rr.data_ptr(), 0 if rr is None else rr.stride(0) if rows > 1 else K,
          None if w is None else w.data_ptr(), wcode, eps, rot, data.data_ptr(), pitch, m, m + 4 * rows,
-         None if out is None else out.data_ptr(), K, nat.raw_stream())
+         None if out is None else out.data_ptr(), K, nat.stream_for(xr, rr, w))
     if out is not None and x.device.type != "cuda":
         out = out.to(x.device)
     return QuantizedActivations(data, meta, Kp, lead), out

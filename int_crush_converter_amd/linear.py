@@ -67,7 +67,7 @@ class QuantizedWeight:
         rows = as_rows(nat.on_gpu("stored", stored))
         self.tiles = nat.workspace(nat.lib().ic_linear_weight_bytes(N, K, bits), rows.device)
         call("ic_linear_pack_weight", rows.data_ptr(), bits, N, K, rows.stride(0) if N > 1 else width,
-             self.tiles.data_ptr(), nat.raw_stream())
+             self.tiles.data_ptr(), nat.stream_for(rows))
 
 
 def quantized_linear(x: QuantizedActivations, weight: QuantizedWeight, bias: torch.Tensor | None = None, *,
@@ -75,14 +75,13 @@ def quantized_linear(x: QuantizedActivations, weight: QuantizedWeight, bias: tor
     """y [*lead, out_features] in ``out_dtype``.  Rows of x whose scale is NaN give rows of NaN."""
     if x.in_features != weight.in_features:
         raise ValueError(f"activations have {x.in_features} features, the weight {weight.in_features}")
-    data, N, w = x.data, weight.out_features, weight
-    if data.device != w.tiles.device:
-        raise ValueError(f"activations are on {data.device}, the weight on {w.tiles.device}")
+    data, N, w, z = x.data, weight.out_features, weight, weight.zero_points
     code = _out_code(out_dtype)
     b, bcode = _bias(bias, N)
+    stream = nat.stream_for(data, x.meta, w.tiles, w.scales, z)
     out = torch.empty((*x.lead, N), dtype=out_dtype, device=data.device)
-    z, rows, m = w.zero_points, data.shape[0], x.meta.data_ptr()
+    rows, m = data.shape[0], x.meta.data_ptr()
     call("ic_quantized_linear", data.data_ptr(), data.shape[1], m, m + 4 * rows, rows, w.tiles.data_ptr(), w.bits,
          w.scales.data_ptr(), w.scale_kind, None if z is None else z.data_ptr(), None if b is None else b.data_ptr(),
-         bcode, N, w.in_features, out.data_ptr(), code, N, nat.raw_stream())
+         bcode, N, w.in_features, out.data_ptr(), code, N, stream)
     return out

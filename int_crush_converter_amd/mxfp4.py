@@ -56,25 +56,27 @@ class Mxfp4Tensor:
             c, s = as_rows(c), as_rows(s)
             call("ic_mxfp4_relayout", c.data_ptr(), c.stride(0) if rows > 1 else have, s.data_ptr(),
                  s.stride(0) if rows > 1 else s.shape[1], rows, K, t.tiles.data_ptr(), t.scales.data_ptr(), 1,
-                 nat.raw_stream())
+                 nat.stream_for(c, s))
         return t
 
     def to_packed(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(codes [*lead, ceil(K/2)], scales [*lead, ceil(K/32)]), the inverse of ``from_packed``."""
         K, rows, dev = self.in_features, self.rows, self.tiles.device
+        stream = nat.stream_for(self.tiles, self.scales)
         c = torch.empty((rows, (K + 1) // 2), dtype=torch.uint8, device=dev)
         s = torch.empty((rows, -(-K // BLOCK)), dtype=torch.uint8, device=dev)
         if rows:
             call("ic_mxfp4_relayout", c.data_ptr(), c.shape[1], s.data_ptr(), s.shape[1], rows, K,
-                 self.tiles.data_ptr(), self.scales.data_ptr(), 0, nat.raw_stream())
+                 self.tiles.data_ptr(), self.scales.data_ptr(), 0, stream)
         return c.reshape(*self.lead, c.shape[1]), s.reshape(*self.lead, s.shape[1])
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values [*lead, in_features] in ``dtype`` (exact in bfloat16 and float32)."""
-        K = self.in_features
+        K, code = self.in_features, _out_code(dtype)
+        stream = nat.stream_for(self.tiles, self.scales)
         out = torch.empty((*self.lead, K), dtype=dtype, device=self.tiles.device)
         call("ic_mxfp4_dequantize", self.tiles.data_ptr(), self.scales.data_ptr(), self.rows, K, out.data_ptr(),
-             _out_code(dtype), K, nat.raw_stream())
+             code, K, stream)
         return out
 
 
@@ -92,7 +94,7 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4Tensor:
     if rows:
         xr = as_rows(xg)
         call("ic_mxfp4_quantize", xr.data_ptr(), code, rows, K, xr.stride(0) if rows > 1 else K, t.tiles.data_ptr(),
-             t.scales.data_ptr(), nat.raw_stream())
+             t.scales.data_ptr(), nat.stream_for(xr))
     return t
 
 
@@ -103,13 +105,12 @@ def mxfp4_linear(x: Mxfp4Tensor, weight: Mxfp4Tensor, bias: torch.Tensor | None 
         raise ValueError(f"the weight must be 2-D with at least one row, got {(*weight.lead, weight.in_features)}")
     if x.in_features != weight.in_features:
         raise ValueError(f"x has {x.in_features} features, the weight {weight.in_features}")
-    if x.tiles.device != weight.tiles.device:
-        raise ValueError(f"x is on {x.tiles.device}, the weight on {weight.tiles.device}")
     N = weight.rows
     code = _out_code(out_dtype)
     b, bcode = _bias(bias, N)
+    stream = nat.stream_for(x.tiles, x.scales, weight.tiles, weight.scales)
     out = torch.empty((*x.lead, N), dtype=out_dtype, device=x.tiles.device)
     call("ic_mxfp4_linear", x.tiles.data_ptr(), x.scales.data_ptr(), x.rows, weight.tiles.data_ptr(),
          weight.scales.data_ptr(), None if b is None else b.data_ptr(), bcode, N, x.in_features, out.data_ptr(), code, N,
-         nat.raw_stream())
+         stream)
     return out
