@@ -37,7 +37,8 @@ def convert(state: dict[str, torch.Tensor], bits: int, folder: str) -> dict[str,
     icq.quantize_model(icq.QuantizeConfig(input_path=src, output_dir=out, rot_size=ROT, int_bits=bits,
                                           asymmetric=True))
     stored = load_file(os.path.join(out, "model.safetensors"))
-    return {n: icq.QuantizedWeight(stored[n], stored[f"{n}_scale"], stored.get(f"{n}_zp")) for n in NAMES}
+    return {n: icq.QuantizedWeight(stored[n], stored[f"{n}_scale"], stored.get(f"{n}_zp"),
+                                   permutation=stored.get(f"{n}_perm")) for n in NAMES}
 
 
 def run_integer(x, residual, gain, w):

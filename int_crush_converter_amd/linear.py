@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
+from . import packing
 from .activations import MAX_FEATURES, QuantizedActivations, as_rows, call
 
 MAX_ROWS = 1048560
@@ -35,17 +36,33 @@ def _bias(bias: torch.Tensor | None, N: int):
     return b, nat.dtype_code(b)
 
 
+def _unpermuted(rows: torch.Tensor, permutation: torch.Tensor, bits: int, K: int) -> torch.Tensor:
+    """Stored rows with their columns where they were before the converter permuted them: column j of the first
+    len(permutation) goes to permutation[j]."""
+    if permutation.dim() != 1 or permutation.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"expected a permutation of column numbers, got {permutation.dtype} {tuple(permutation.shape)}")
+    p, n = nat.on_gpu("permutation", permutation).long(), permutation.numel()
+    if n > K or not torch.equal(p.sort().values, torch.arange(n, device=p.device)):
+        raise ValueError(f"not a permutation of the first {n} of {K} columns")
+    codes = packing.unpack_int4(rows, K) if bits == 4 else rows
+    out = codes.clone()
+    out[:, p] = codes[:, :n]
+    return packing.pack_int4(out) if bits == 4 else out
+
+
 class QuantizedWeight:
     """A stored weight laid out once for ``quantized_linear``.
 
     stored: int8 [N, K] (INT8) or uint8 [N, ceil(K/2)] (INT4, low nibble first); scales: fp16 or fp32 [N] or [N, 1];
-    zero_points: int8 of the same shape, or None - ``<name>``, ``<name>_scale`` and ``<name>_zp`` of the converter's
-    output.  in_features: K, needed where an INT4 row ends in half a byte."""
+    zero_points: int8 of the same shape, or None; permutation: int32 or int64, up to K column numbers, or None -
+    ``<name>``, ``<name>_scale``, ``<name>_zp`` and ``<name>_perm`` of the converter's output.  A permuted layer's
+    columns are put back in order here, so that its activations are those of any other layer; without its
+    permutation its products are wrong.  in_features: K, needed where an INT4 row ends in half a byte."""
 
     __slots__ = ("tiles", "scales", "scale_kind", "zero_points", "bits", "in_features", "out_features")
 
     def __init__(self, stored: torch.Tensor, scales: torch.Tensor, zero_points: torch.Tensor | None = None, *,
-                 in_features: int | None = None):
+                 permutation: torch.Tensor | None = None, in_features: int | None = None):
         if stored.dim() != 2 or stored.dtype not in (torch.int8, torch.uint8):
             raise ValueError(f"expected int8 [N, K] or packed uint8 [N, ceil(K/2)], got {stored.dtype} {tuple(stored.shape)}")
         N, width = stored.shape
@@ -65,6 +82,8 @@ class QuantizedWeight:
         self.zero_points = None if zero_points is None else nat.on_gpu("zero_points", zero_points).reshape(-1).contiguous()
         self.bits, self.in_features, self.out_features = bits, K, N
         rows = as_rows(nat.on_gpu("stored", stored))
+        if permutation is not None:
+            rows = _unpermuted(rows, permutation, bits, K)
         self.tiles = nat.workspace(nat.lib().ic_linear_weight_bytes(N, K, bits), rows.device)
         call("ic_linear_pack_weight", rows.data_ptr(), bits, N, K, rows.stride(0) if N > 1 else width,
              self.tiles.data_ptr(), nat.stream_for(rows))
