@@ -64,8 +64,7 @@ class QuantizedActivations:
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "QuantizedActivations":
-        """Codes [..., K] (int8) and scales [...] from elsewhere.  The codes are copied unless their rows already
-        have the stored layout."""
+        """Codes [..., K] (int8) and scales [...] from elsewhere.  Both are copied: the rows' sums are kept beside them."""
         if codes.dim() < 1 or codes.dtype != torch.int8:
             raise ValueError(f"expected int8 codes [..., K], got {codes.dtype} {tuple(codes.shape)}")
         lead, K = codes.shape[:-1], codes.shape[-1]
@@ -77,11 +76,9 @@ class QuantizedActivations:
             raise ValueError(f"{scales.numel()} scales for {rows} rows of codes")
         meta = torch.empty((2, rows), dtype=torch.float32, device=codes.device)
         meta[0] = nat.on_gpu("scales", scales).reshape(-1)
-        if K % _PAD or codes.stride(0) != K or codes.data_ptr() % 16:
-            data = torch.zeros(rows, -(-K // _PAD) * _PAD, dtype=torch.int8, device=codes.device)
-            data[:, :K] = codes
-        else:
-            data = codes
+        pitch = -(-K // _PAD) * _PAD
+        data = (torch.zeros if pitch > K else torch.empty)((rows, pitch), dtype=torch.int8, device=codes.device)
+        data[:, :K] = codes
         call("ic_row_sums_i8", data.data_ptr(), rows, K, data.shape[1], meta.data_ptr() + 4 * rows,
              nat.stream_for(data, meta))
         return cls(data, meta, K, lead)
