@@ -65,6 +65,8 @@ __device__ __forceinline__ void rotate16(float (&v)[16], int rot, float sign) {
 }
 
 // op over the 64 lanes: within rows of 16 by DPP, between them by two exchanges.
+// The rotations give the four quads of a row their sums in different orders, so
+// one lane's result is taken for all: a row has one norm and one scale.
 template <int CTRL, typename T>
 __device__ __forceinline__ T dpp_any(T v) {
     return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -84,8 +86,9 @@ __device__ __forceinline__ T row_reduce(T v, T* lds, F op) {
         v = lds[0];
 #pragma unroll
         for (int i = 1; i < WAVES; ++i) v = op(v, lds[i]);
+        return v;
     }
-    return v;
+    return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 
 // WAVES waves hold one row, NC chunks of 16 columns a lane; for WAVES = 1 a

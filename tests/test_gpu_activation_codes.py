@@ -70,3 +70,23 @@ def test_halves_of_rotated_rows(gpu_dev, rot):
     assert torch.equal(x.float().double(), x)
     q = icq.quantize_activations(x.float().to(gpu_dev), rot_size=rot).codes.cpu().long()
     assert torch.equal(q, integer_codes(a))
+
+
+@pytest.mark.parametrize("seed,k", [(433, 120), (3110, 123)])
+def test_a_row_has_one_norm(gpu_dev, seed, k):
+    """Equal values anywhere in a row have equal codes: rows whose sum of squares rounds differently in other orders,
+    with a value next to a half in the first column of four groups of lanes."""
+    import numpy as np
+    import int_crush_converter_amd as icq
+    K = 1024
+    r = np.random.RandomState(seed)
+    x = torch.from_numpy((r.randint(-512, 513, K) / 256).astype(np.float32))
+    x[500] = 6.0
+    near = np.float32((k + 0.5) * 6 / 127)
+    for step in range(-2, 3):
+        c = near
+        for _ in range(abs(step)):
+            c = np.nextafter(c, np.float32(np.sign(step) * 100))
+        x[[0, 64, 128, 192]] = float(c)
+        q, _ = icq.rms_norm_quantize(x[None].to(gpu_dev), torch.ones(K, device=gpu_dev))
+        assert q.codes[0, [0, 64, 128, 192]].unique().numel() == 1
