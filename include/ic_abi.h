@@ -484,8 +484,8 @@ int64_t ic_activation_pitch(int64_t cols);
  * itself) of `dtype`; weight [cols] of weight_dtype (x's, or fp32), NULL =
  * no norm.  codes [rows, ld_q] with ld_q = ic_activation_pitch(cols padded
  * to rot), 16-byte aligned, zeros behind the last column; scales fp32 [rows];
- * sums int32 [rows] = the codes' row sums.  A row with Inf or NaN gets the
- * scale NaN and codes 0.  At most 65536 padded columns. */
+ * sums int32 [rows] = the codes' row sums.  A row with Inf or NaN, or whose
+ * rotated values pass a quarter of fp32's range, gets the scale NaN and codes 0.  At most 65536 padded columns. */
 int ic_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld_x, const void* residual,
                      int64_t ld_r, const void* weight, int weight_dtype, float eps, int rot, int8_t* codes,
                      int64_t ld_q, float* scales, int32_t* sums, void* residual_out, int64_t ld_ro, void* stream);

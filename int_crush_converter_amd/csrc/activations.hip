@@ -103,8 +103,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
     const void* __restrict__ weight, int weight_f32, float eps, int rot, int8_t* __restrict__ codes,
     int64_t ld_q, float* __restrict__ scales, int32_t* __restrict__ sums, void* residual_out,
     int64_t ld_ro) {
-    __shared__ float red_f[WAVES];
-    __shared__ unsigned red_u[WAVES];
+    __shared__ float red_f[WAVES], red_f2[WAVES];
+    __shared__ unsigned red_u[WAVES], red_u2[WAVES];
     __shared__ int red_i[WAVES];
     const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
     const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
@@ -125,23 +125,54 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
         }
     }
     if (weight) {
-        float g[NC][16];                     // on its way while the squares are summed
+        // the weight is on its way while the squares are summed, unless it and the row fill the registers (128 a lane
+        // with 1024 threads, where 89 were spilled: 2048 x 65536 bf16 153 us, 166 with the early load and 16 spilled;
+        // 1024 x 65536 fp32 107 against 97, with residual and rotation 226 against 227)
+        constexpr bool EARLY = WAVES * NC < 64;
+        float g[EARLY ? NC : 1][16];
+        auto load_weight = [&](int c, float (&to)[16]) {
+            if (weight_f32) load16<IC_DTYPE_F32>(weight, 0, c * SPAN + lane * 16, cols, to);
+            else load16<DT>(weight, 0, c * SPAN + lane * 16, cols, to);
+        };
+        if (EARLY) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) load_weight(c, g[c]);
+        }
+        auto squares = [&]() {
+            float ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ss = __builtin_fmaf(v[c][i], v[c][i], ss);
+            return ss;
+        };
+        const auto add = [](float a, float b) { return a + b; };
+        const auto larger = [](unsigned a, unsigned b) { return max(a, b); };
+        float ms = row_reduce<WAVES>(squares(), red_f, add) / (float)cols + eps;
+        if (!(ms >= 0x1p-100f && ms < INFINITY)) {
+            // Squares past fp32's range, or all below it (the whole row takes this branch): again with the row, and
+            // eps, brought to a magnitude of 1 by a power of two.  Rows with Inf or NaN end as NaN here as well.
+            unsigned top = __float_as_uint(sqrtf(eps));
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[c][i]) & 0x7fffffffu);
+            top = row_reduce<WAVES>(top, red_u2, larger);
+            const int e = min(max((int)(top >> 23), 1), 253);          // (254: the power's own would be subnormal)
+            const float f = __uint_as_float((unsigned)(254 - e) << 23);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[c][i] *= f;
+            ms = row_reduce<WAVES>(squares(), red_f2, add) / (float)cols + eps * f * f;
+        }
+        const float rs = 1.0f / sqrtf(ms);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            if (weight_f32) load16<IC_DTYPE_F32>(weight, 0, c * SPAN + lane * 16, cols, g[c]);
-            else load16<DT>(weight, 0, c * SPAN + lane * 16, cols, g[c]);
+            if (!EARLY) load_weight(c, g[0]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * rs * g[EARLY ? c : 0][i];
         }
-        float ss = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ss = __builtin_fmaf(v[c][i], v[c][i], ss);
-        ss = row_reduce<WAVES>(ss, red_f, [](float a, float b) { return a + b; });
-        const float rs = 1.0f / sqrtf(ss / (float)cols + eps);
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[c][i] = v[c][i] * rs * g[c][i];
     }
     if (rot > 1) {
 #pragma unroll
