@@ -13,6 +13,14 @@
 namespace icq {
 namespace {
 
+// Work-groups in runs of 2^20 along the grid's second axis: along one axis a
+// launch has fewer than 2^32 threads, which 2^22 rows of 16 waves fill.
+inline dim3 group_grid(int64_t groups) {
+    const int64_t run = 1 << 20;
+    return dim3((unsigned)(groups < run ? groups : run), (unsigned)cdiv(groups, run));
+}
+__device__ __forceinline__ int64_t group_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 constexpr float kTinyMax = 1e-30f;   // the smallest row maximum that a scale stands for
 
 __device__ __forceinline__ void bfly4(float& a, float& b, float& c, float& d) {
@@ -107,7 +115,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
     __shared__ unsigned red_u[WAVES], red_u2[WAVES];
     __shared__ int red_i[WAVES];
     const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
-    const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const int64_t row = WAVES == 1 ? group_index() * 4 + (threadIdx.x >> 6) : group_index();
     if (row >= rows) return;
     constexpr int SPAN = 64 * WAVES * 16;
 
@@ -241,7 +249,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* __re
 // Row sums of 8-bit codes: one wave a row.
 __global__ __launch_bounds__(256) void row_sums_kernel(const int8_t* __restrict__ codes, int64_t rows, int64_t cols,
                                                        int64_t ld_q, int32_t* __restrict__ sums) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t row = group_index() * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
     int sum = 0;
     for (int64_t c = threadIdx.x & 63; c < cols; c += 64) sum += codes[row * ld_q + c];
@@ -257,7 +265,7 @@ struct RowArgs {
 
 template <int DT, int WAVES, int NC>
 void launch_rows(const RowArgs& a) {
-    const dim3 grid((unsigned)(WAVES == 1 ? cdiv(a.rows, 4) : a.rows)), block(WAVES == 1 ? 256 : 64 * WAVES);
+    const dim3 grid = group_grid(WAVES == 1 ? cdiv(a.rows, 4) : a.rows), block(WAVES == 1 ? 256 : 64 * WAVES);
     hipLaunchKernelGGL((quantize_rows_kernel<DT, WAVES, NC>), grid, block, 0, a.st, a.x, a.rows, a.cols, a.ld_x,
                        a.residual, a.ld_r, a.weight, a.weight_f32, a.eps, a.rot, a.codes, a.ld_q, a.scales, a.sums,
                        a.residual_out, a.ld_ro);
@@ -344,7 +352,7 @@ extern "C" int ic_row_sums_i8(const int8_t* codes, int64_t rows, int64_t cols, i
     if (rows == 0) return IC_OK;
     IC_REQUIRE(codes && sums, "ic_row_sums_i8: null pointer");
     if (cols > 65536 || rows > 0x7fffffff) return fail(IC_ERR_RANGE, "ic_row_sums_i8: at most 65536 columns and 2^31 - 1 rows");
-    hipLaunchKernelGGL(row_sums_kernel, dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, as_stream(stream), codes, rows,
+    hipLaunchKernelGGL(row_sums_kernel, group_grid(cdiv(rows, 4)), dim3(256), 0, as_stream(stream), codes, rows,
                        cols, ld_q, sums);
     IC_CHECK_LAUNCH();
     return IC_OK;
