@@ -271,20 +271,17 @@ void launch_rows(const RowArgs& a) {
                        a.residual_out, a.ld_ro);
 }
 
-template <int DT, int WAVES>
-void launch_chunks(const RowArgs& a) {
-    const int64_t nc = cdiv(a.ld_q, (int64_t)64 * WAVES * 16);
-    if (nc <= 1) launch_rows<DT, WAVES, 1>(a);
-    else if (nc <= 2) launch_rows<DT, WAVES, 2>(a);
-    else if (nc <= 3) launch_rows<DT, WAVES, 3>(a);
-    else launch_rows<DT, WAVES, 4>(a);
-}
-
+// One wave a row up to 1024 columns, four up to 16384, else sixteen.
 template <int DT>
 void launch_waves(const RowArgs& a) {
-    if (a.ld_q <= 1024) launch_chunks<DT, 1>(a);
-    else if (a.ld_q <= 16384) launch_chunks<DT, 4>(a);
-    else launch_chunks<DT, 16>(a);
+    if (a.ld_q <= 1024) return launch_rows<DT, 1, 1>(a);
+    if (a.ld_q <= 4096) return launch_rows<DT, 4, 1>(a);
+    if (a.ld_q <= 8192) return launch_rows<DT, 4, 2>(a);
+    if (a.ld_q <= 12288) return launch_rows<DT, 4, 3>(a);
+    if (a.ld_q <= 16384) return launch_rows<DT, 4, 4>(a);
+    if (a.ld_q <= 32768) return launch_rows<DT, 16, 2>(a);
+    if (a.ld_q <= 49152) return launch_rows<DT, 16, 3>(a);
+    launch_rows<DT, 16, 4>(a);
 }
 
 }  // namespace

@@ -76,22 +76,6 @@ struct Columns {
     }
 };
 
-// Eight consecutive outputs at element `at` of out, 16-byte aligned.
-__device__ __forceinline__ void store8(const Operands& p, lb_f32x4 a, lb_f32x4 b, int64_t at) {
-    if (p.out_dtype == IC_DTYPE_F32) {
-        *reinterpret_cast<lb_f32x4*>(static_cast<float*>(p.out) + at) = a;
-        *reinterpret_cast<lb_f32x4*>(static_cast<float*>(p.out) + at + 4) = b;
-    } else {
-        lb_u32x4 w;
-        if (p.out_dtype == IC_DTYPE_BF16)
-            w = lb_u32x4{pack_half_words<IC_DTYPE_BF16>(a[0], a[1]), pack_half_words<IC_DTYPE_BF16>(a[2], a[3]),
-                         pack_half_words<IC_DTYPE_BF16>(b[0], b[1]), pack_half_words<IC_DTYPE_BF16>(b[2], b[3])};
-        else
-            w = lb_u32x4{pack_half_words<IC_DTYPE_F16>(a[0], a[1]), pack_half_words<IC_DTYPE_F16>(a[2], a[3]),
-                         pack_half_words<IC_DTYPE_F16>(b[0], b[1]), pack_half_words<IC_DTYPE_F16>(b[2], b[3])};
-        *reinterpret_cast<lb_u32x4*>(static_cast<uint16_t*>(p.out) + at) = w;
-    }
-}
 // Four consecutive outputs of row m from column n.
 __device__ __forceinline__ void store4(const Operands& p, lb_f32x4 v, int64_t m, int64_t n) {
     if (m >= p.M || n >= p.N) return;
@@ -116,12 +100,10 @@ __device__ __forceinline__ void store4(const Operands& p, lb_f32x4 v, int64_t m,
 __device__ __forceinline__ i32x4 mma_i8(lb_u32x4 w, lb_u32x4 x, i32x4 acc) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), acc, 0, 0, 0);
 }
-// (byte B of each scale word)
-template <int B>
 __device__ __forceinline__ lb_f32x4 mma_mx(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc, int sw, int sx) {
     const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     const i32x8 b = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, B, sw, B, sx);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, sw, 0, sx);
 }
 // The same products of 32 rows and 32 columns, with twice the operations an
 // instruction (a wave alone on its SIMD reaches 4.7 POP/s and 8.9 PFLOP/s with
@@ -133,6 +115,7 @@ template <> struct Acc32<kMx> { typedef f32x16 T; };
 __device__ __forceinline__ i32x16 mma32_i8(lb_u32x4 w, lb_u32x4 x, i32x16 acc) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), acc, 0, 0, 0);
 }
+// (byte B of each scale word)
 template <int B>
 __device__ __forceinline__ f32x16 mma32_mx(lb_u32x4 w, lb_u32x4 x, f32x16 acc, int sw, int sx) {
     const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
@@ -154,14 +137,15 @@ __device__ __forceinline__ lb_u32x4 to_operand(lb_u32x4 v, int from) {
     return o;
 }
 
-// Few rows: a work-group of WAVES waves takes 16 columns of y and 16 MT rows,
+// Few rows: a work-group of 8 waves takes 16 columns of y and 16 MT rows,
 // its waves a share of K each; the sums are joined in LDS in a fixed order.
 // One row is bound by the weights' bytes and the launch: INT4 1 x 12288 x 4096
 // 6.4 us (25 MB, 4.0 TB/s); more rows by their activations, which every
 // work-group reads again: INT8 333 x 1000 x 2901 10.7 us.
-template <int KIND, int MT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
+template <int KIND, int MT>
+__global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
     typedef typename Acc<KIND>::T acc_t;
+    constexpr int WAVES = 8;
     __shared__ acc_t part[WAVES][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
     const int64_t nt = blockIdx.x, mt0 = (int64_t)blockIdx.y * MT;
@@ -192,7 +176,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_direct_kernel(Operands p) {
             const int sw = (int)(ws[(t >> 2) * 64] >> (8 * (t & 3)));
 #pragma unroll
             for (int i = 0; i < MT; ++i)
-                acc[i] = mma_mx<0>(w, xt[i][t * 64], acc[i], sw & 255, (int)(xs[i][(t >> 2) * 64] >> (8 * (t & 3))) & 255);
+                acc[i] = mma_mx(w, xt[i][t * 64], acc[i], sw & 255, (int)(xs[i][(t >> 2) * 64] >> (8 * (t & 3))) & 255);
         } else {
             lb_u32x4 w0, w1;
             if (KIND == kInt8) {
@@ -667,10 +651,10 @@ __global__ __launch_bounds__(256) void pack_weight_kernel(const uint8_t* __restr
     dst[((int64_t)blockIdx.y * tiles + t) * 64 + lane] = w;
 }
 
-template <int KIND, int MT, int WAVES>
+template <int KIND, int MT>
 void launch_direct(const Operands& p, hipStream_t st) {
     const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16 * MT));
-    hipLaunchKernelGGL((linear_direct_kernel<KIND, MT, WAVES>), grid, dim3(64 * WAVES), 0, st, p);
+    hipLaunchKernelGGL((linear_direct_kernel<KIND, MT>), grid, dim3(512), 0, st, p);
 }
 
 // As many work-groups as run at once (one a CU with tiles of 256 x 256, whose
@@ -706,9 +690,9 @@ int launch_linear(const Operands& p, hipStream_t st) {
     const int form = linear_form(p.M, p.N);
     if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
     else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4>(p, st);
-    else if (p.M <= 16) launch_direct<KIND, 1, 8>(p, st);
-    else if (p.M <= 32) launch_direct<KIND, 2, 8>(p, st);
-    else launch_direct<KIND, 4, 8>(p, st);
+    else if (p.M <= 16) launch_direct<KIND, 1>(p, st);
+    else if (p.M <= 32) launch_direct<KIND, 2>(p, st);
+    else launch_direct<KIND, 4>(p, st);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
