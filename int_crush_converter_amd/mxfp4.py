@@ -44,6 +44,7 @@ class Mxfp4Tensor:
         if codes.dim() < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise ValueError(f"expected uint8 codes and scales, got {codes.dtype} and {scales.dtype}")
         K = in_features if in_features is not None else 2 * codes.shape[-1]
+        _sizes(0, K)
         lead = codes.shape[:-1]
         have, whole = codes.shape[-1], -(-K // BLOCK) * (BLOCK // 2)
         if have not in ((K + 1) // 2, whole) or tuple(scales.shape) != (*lead, -(-K // BLOCK)):
