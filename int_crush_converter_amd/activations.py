@@ -10,6 +10,8 @@ codes), after the regular-Hadamard rotation that the weights had
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _native as nat
@@ -48,9 +50,22 @@ class QuantizedActivations:
     __slots__ = ("data", "meta", "in_features", "lead")
 
     def __init__(self, data: torch.Tensor, meta: torch.Tensor, in_features: int, lead):
-        self.data = data                     # int8 [rows, pitch]
-        self.meta = meta                     # fp32 [2, rows]: the scales; the sums' bits
-        self.in_features, self.lead = in_features, tuple(lead)
+        """data: int8 [rows, pitch], rows of ``lead`` in order, the pitch in_features padded to 128; meta: fp32 [2, rows],
+        the scales and the sums' bits.  ``from_codes`` makes them of codes and scales."""
+        rows, pitch = math.prod(lead), -(-in_features // _PAD) * _PAD
+        if not 1 <= in_features <= MAX_FEATURES:
+            raise ValueError(f"in_features must be in [1, {MAX_FEATURES}], got {in_features}")
+        for name, t, dtype, shape in (("data", data, torch.int8, (rows, pitch)), ("meta", meta, torch.float32, (2, rows))):
+            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} must be contiguous {dtype} {shape} at 16-byte alignment, got {t.dtype} "
+                                 f"{tuple(t.shape)} with strides {t.stride()}")
+        self.data, self.meta, self.in_features, self.lead = data, meta, in_features, tuple(lead)
+
+    @classmethod
+    def _of(cls, data, meta, in_features, lead) -> "QuantizedActivations":
+        q = cls.__new__(cls)                 # of tensors made here, as __init__ wants them
+        q.data, q.meta, q.in_features, q.lead = data, meta, in_features, tuple(lead)
+        return q
 
     @property
     def scales(self) -> torch.Tensor:
@@ -81,7 +96,7 @@ class QuantizedActivations:
         data[:, :K] = codes
         call("ic_row_sums_i8", data.data_ptr(), rows, K, data.shape[1], meta.data_ptr() + 4 * rows,
              nat.stream_for(data, meta))
-        return cls(data, meta, K, lead)
+        return cls._of(data, meta, K, lead)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -140,7 +155,7 @@ def _quantize(x, weight, residual, eps, rot_size):
          None if out is None else out.data_ptr(), K, nat.stream_for(xr, rr, w))
     if out is not None and x.device.type != "cuda":
         out = out.to(x.device)
-    return QuantizedActivations(data, meta, Kp, lead), out
+    return QuantizedActivations._of(data, meta, Kp, lead), out
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,

@@ -8,6 +8,8 @@ has the scale NaN (byte 255)."""
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _native as nat
@@ -22,20 +24,35 @@ def _sizes(rows: int, K: int) -> None:
         raise ValueError(f"in_features must be in [1, {MAX_FEATURES}] and rows at most {MAX_ROWS}, got {K}, {rows}")
 
 
+def _nbytes(rows: int, K: int) -> tuple[int, int]:
+    """ic_mxfp4_code_bytes and ic_mxfp4_scale_bytes."""
+    return -(-rows // 16) * -(-K // 128) * 1024, -(-rows // 16) * -(-K // 512) * 256
+
+
 class Mxfp4Tensor:
     """A tensor [*lead, in_features] in microscaled 4-bit form, on the GPU, in the tiles that the products read."""
 
     __slots__ = ("tiles", "scales", "in_features", "lead", "rows")
 
     def __init__(self, tiles: torch.Tensor, scales: torch.Tensor, in_features: int, lead, rows: int):
+        """tiles and scales: the bytes of csrc/lowbit.hpp's layout, one after another; rows: those of ``lead``.
+        ``from_packed`` makes them of row-major codes and scales."""
+        _sizes(rows, in_features)
+        if rows != math.prod(lead):
+            raise ValueError(f"{rows} rows for the shape {tuple(lead)}")
+        for name, t, n in zip(("tiles", "scales"), (tiles, scales), _nbytes(rows, in_features)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != (n,) or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} must be contiguous uint8 ({n},) at 16-byte alignment, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
         self.tiles, self.scales = tiles, scales
         self.in_features, self.lead, self.rows = in_features, tuple(lead), rows
 
     @classmethod
     def _empty(cls, lead, rows: int, K: int, dev: torch.device) -> "Mxfp4Tensor":
-        # ic_mxfp4_code_bytes and ic_mxfp4_scale_bytes
-        return cls(torch.empty(-(-rows // 16) * -(-K // 128) * 1024, dtype=torch.uint8, device=dev),
-                   torch.empty(-(-rows // 16) * -(-K // 512) * 256, dtype=torch.uint8, device=dev), K, lead, rows)
+        t = cls.__new__(cls)                 # of tensors made here, as __init__ wants them
+        t.tiles, t.scales = (torch.empty(n, dtype=torch.uint8, device=dev) for n in _nbytes(rows, K))
+        t.in_features, t.lead, t.rows = K, tuple(lead), rows
+        return t
 
     @classmethod
     def from_packed(cls, codes: torch.Tensor, scales: torch.Tensor, *, in_features: int | None = None) -> "Mxfp4Tensor":

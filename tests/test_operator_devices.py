@@ -38,7 +38,7 @@ def calls(monkeypatch):
 
 
 def integer(i, meta=None):
-    return activations.QuantizedActivations(On(i, 3, 128), On(i if meta is None else meta, 2, 3), 100, (3,))
+    return activations.QuantizedActivations._of(On(i, 3, 128), On(i if meta is None else meta, 2, 3), 100, (3,))
 
 
 def weight(i, scales=None, zeros=None):
@@ -49,7 +49,9 @@ def weight(i, scales=None, zeros=None):
 
 
 def mx(i, scales=None, rows=3):
-    return mxfp4.Mxfp4Tensor(On(i, 1024), On(i if scales is None else scales, 256), 100, (rows,), rows)
+    t = mxfp4.Mxfp4Tensor.__new__(mxfp4.Mxfp4Tensor)
+    t.tiles, t.scales, t.in_features, t.lead, t.rows = On(i, 1024), On(i if scales is None else scales, 256), 100, (rows,), rows
+    return t
 
 
 @pytest.mark.parametrize("where", [1, -1])
