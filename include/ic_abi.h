@@ -513,9 +513,10 @@ int ic_quantized_linear(const int8_t* a, int64_t ld_a, const float* sa, const in
                         const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,
                         int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out, void* stream);
 
-/* Which form ic_quantized_linear and ic_mxfp4_linear take for these sizes: 0
- * (rows directly from memory), 128 or 256 (tiles of so many rows and columns). */
-int ic_linear_form(int64_t M, int64_t N);
+/* Which form a product takes for these sizes: 0 (rows directly from memory),
+ * 128 or 256 (tiles of so many rows and columns).  kind: 0 and 1 =
+ * ic_quantized_linear with INT8 and INT4 weights, 2 = ic_mxfp4_linear. */
+int ic_linear_form(int kind, int64_t M, int64_t N);
 
 /* Microscaled 4-bit floating point (OCP MX): E2M1 elements, one E8M0 scale
  * for 32 consecutive columns, 2^(floor(log2(max|x|)) - 2); elements to the

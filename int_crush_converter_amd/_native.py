@@ -99,7 +99,7 @@ _SIGS = {
                                 _i64, _vp]),
     "ic_dequantize_rows": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i32, _i64, _vp]),
     "ic_row_sums_i8": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp]),
-    "ic_linear_form": (_i32, [_i64, _i64]),
+    "ic_linear_form": (_i32, [_i32, _i64, _i64]),
     "ic_linear_weight_bytes": (_i64, [_i64, _i64, _i32]),
     "ic_linear_pack_weight": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp]),
     "ic_quantized_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp,

@@ -659,7 +659,8 @@ void launch_direct(const Operands& p, hipStream_t st) {
 
 // As many work-groups as run at once (one a CU with tiles of 256 x 256, whose
 // buffers take most of its LDS, two with 128 x 128), each of which walks its
-// XCD's tiles.
+// XCD's tiles.  (INT4's 128 x 128 takes 260 registers, four too many for two a
+// CU: its second half starts as the first ends.)
 template <int KIND, int WM, int WN, int FM, int FN, int BUF>
 void launch_tiled(const Operands& p, hipStream_t st) {
     const int gm = (int)cdiv(p.M, 32 * WM * FM), gn = (int)cdiv(p.N, 32 * WN * FN);
@@ -669,25 +670,40 @@ void launch_tiled(const Operands& p, hipStream_t st) {
     hipLaunchKernelGGL((linear_tiled_kernel<KIND, WM, WN, FM, FN, BUF>), dim3(grid), dim3(64 * WM * WN), 0, st, p, gm, gn);
 }
 
-// Which form: the direct one while it has few work-groups (of 64 rows x 16
-// columns each), since a tile of 128 x 128 takes its K steps one after another
-// and leaves CUs idle when there are few; then tiles of 256 x 256 where they
-// fill at least three quarters of their rounds over the 256 CUs, else of
-// 128 x 128.  Measured, us (direct / 128 / 256):
-//   INT8 M 128 4096x4096 (512 work-groups)  15 / 25 / 52;  M 333 (1536)  46 / 25 / 52
-//   INT4 M 2048 4096x4096 (256-tiles fill 1/2)  - / 43 / 54;  M 3000 (3/4)  - / 60 / 59
-//   INT4 M 4096 12288x4096 (all)  - / 215 / 189
-//   MXFP4 M 200 4096x4096 (1024)  14 / 15 / 29;  M 333 (1536)  20 / 16 / 30
-//   MXFP4 M 2048 4096x4096 (1/2)  81 / 27 / 34;  M 4096 12288x4096 (all)  - / 131 / 118
-int linear_form(int64_t M, int64_t N) {      // 0, 128 or 256
-    const int64_t groups = cdiv(N, 16) * cdiv(M, 64), tiles = cdiv(M, 256) * cdiv(N, 256);
-    if (M <= 64 || groups < 1000) return 0;
-    return tiles * 4 >= cdiv(tiles, 256) * 256 * 3 ? 256 : 128;
+// Which form.  The direct one while it has few work-groups (of 64 rows x 16
+// columns each): a tile of 128 x 128 takes its K steps one after another and
+// leaves CUs idle when there are few.  Its line is where the two meet at K =
+// 4096 (a longer K has it lower, a shorter one higher).  Measured (calls one
+// after another, operands in cache; us), direct against 128 x 128, K = 1024 /
+// 4096 / 12288, 128 x 128 being 10/23/57, 10/22/53 and 7.8/15/33 in each line:
+//   groups (y)             INT8         INT4         MXFP4
+//    693 ( 701 x 1000)    7.7/20/55    8.0/15/34    6.8/9.3/24
+//   1008 ( 192 x 5376)    9.5/25/68    8.5/18/43    6.9/12/26
+//   1152 ( 256 x 4608)     11/28/81    8.7/20/54    6.7/14/41
+//   1280 ( 320 x 4096)     12/30/83    8.8/20/59    6.9/15/44
+//   1344 ( 192 x 7168)     11/32/98    9.9/23/60    7.3/17/44
+// Then tiles of 256 x 256, one a CU, where they fill more than half of a first
+// round over the 256 CUs (up to there 128 x 128 tiles need one round too), or of
+// two and more rounds three quarters, with INT4 two thirds; else of 128 x 128.
+// 128 x 128 against 256 x 256, y of 4096 columns, K = 1024 / 4096 / 12288:
+//   rows (256-tiles)            INT8                        INT4                         MXFP4
+//   2048 (1/2 round)     17/44/115 - 23/55/139      22/49/119 - 25/56/137      12/25/59  - 16/34/82
+//   2304 (0.56)          24/62/160 - 25/59/143      30/69/168 - 26/57/135      16/34/86  - 16/34/84
+//   4096 (1 round)       31/82/225 - 28/69/178      40/94/237 - 29/66/164      25/46/111 - 22/41/99
+//   5120 (0.63 of two)  36/101/279 - 44/117/305    49/114/288 - 47/112/285     32/57/143 - 28/66/171
+//   5632 (0.69 of two)  42/115/328 - 45/118/309    57/135/343 - 48/115/285     34/63/155 - 28/67/171
+//   6144 (0.75 of two)  43/120/336 - 46/121/319    58/138/345 - 50/118/288     35/65/163 - 29/68/174
+//   8192 (2 rounds)     55/157/446 - 53/133/348    77/188/479 - 54/126/320     37/85/216 - 48/77/191
+int linear_form(int kind, int64_t M, int64_t N) {      // 0, 128 or 256
+    const int64_t groups = cdiv(N, 16) * cdiv(M, 64), tiles = cdiv(M, 256) * cdiv(N, 256), rounds = cdiv(tiles, 256);
+    if (M <= 64 || groups < (kind == kInt8 ? 1000 : kind == kInt4 ? 1300 : 1150)) return 0;
+    if (rounds == 1) return tiles > 128 ? 256 : 128;
+    return tiles * 12 >= rounds * 256 * (kind == kInt4 ? 8 : 9) ? 256 : 128;
 }
 
 template <int KIND>
 int launch_linear(const Operands& p, hipStream_t st) {
-    const int form = linear_form(p.M, p.N);
+    const int form = linear_form(KIND, p.M, p.N);
     if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
     else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4>(p, st);
     else if (p.M <= 16) launch_direct<KIND, 1>(p, st);
@@ -712,7 +728,10 @@ int check_product(const char* who, const Operands& p) {
 
 using namespace icq;
 
-extern "C" int ic_linear_form(int64_t M, int64_t N) { return M < 0 || N < 1 ? IC_ERR_ARG : linear_form(M, N); }
+extern "C" int ic_linear_form(int kind, int64_t M, int64_t N) {
+    IC_REQUIRE(kind >= kInt8 && kind <= kMx && M >= 0 && N >= 1, "ic_linear_form: kind must be 0, 1 or 2, M >= 0, N >= 1");
+    return linear_form(kind, M, N);
+}
 
 extern "C" int64_t ic_linear_weight_bytes(int64_t N, int64_t K, int bits) {
     if (N < 0 || K < 0 || (bits != 4 && bits != 8)) return 0;

@@ -20,15 +20,15 @@ import torch
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 KINDS = [(8, True), (8, False), (4, True), (4, False), ("mx", False)]
 # form, M, N: one tile row short, rows of y at no alignment, few rows and many columns; more than one tile a work-group
-SIZES = [(128, 1025, 1000), (128, 1025, 1003), (128, 65, 16000), (128, 2900, 3704), (128, 2900, 3701),
+SIZES = [(128, 1345, 1000), (128, 1345, 1003), (128, 65, 16000), (128, 4400, 3704), (128, 4400, 3701),
          (256, 3300, 3904), (256, 3300, 3901), (256, 5100, 5104), (256, 5100, 5101)]
 DEPTHS = [1, 65, 129, 250, 257, 385, 513, 2901]
 
 
-def form(M, N):
+def form(kind, M, N):
     from int_crush_converter_amd import _native as nat
     nat.load(require_gpu=False)
-    return nat._lib.ic_linear_form(M, N)
+    return nat._lib.ic_linear_form({8: 0, 4: 1, "mx": 2}[kind], M, N)
 
 
 def test_sizes_reach_the_forms():
@@ -36,9 +36,15 @@ def test_sizes_reach_the_forms():
     if not os.path.exists(nat.LIB_PATH):
         from int_crush_converter_amd import build
         build.build()
-    assert all(form(M, N) == f for f, M, N in SIZES)
-    assert form(1, 1 << 20) == 0 and form(64, 1 << 20) == 0 and form(0, 5) == 0
-    assert form(-1, 5) == -1 and form(5, 0) == -1
+    assert all(form(kind, M, N) == f for f, M, N in SIZES for kind in (4, 8, "mx"))
+    assert form(4, 1, 1 << 20) == 0 and form(8, 64, 1 << 20) == 0 and form("mx", 0, 5) == 0
+    # the lines: work-groups of the direct form; half of a round of 256 tiles, three quarters (INT4: two thirds) of several
+    assert [form(k, m, 4096) for k in (8, 4, "mx") for m in (192, 256, 320, 384)] == [0, 128, 128, 128, 0, 0, 0, 128, 0, 0, 128, 128]
+    assert [form(8, m, 4096) for m in (2048, 2049, 4096, 4097, 5888, 5889)] == [128, 256, 256, 128, 128, 256]
+    assert [form(4, m, 4096) for m in (2048, 2049, 4096, 4097, 5376, 5377)] == [128, 256, 256, 128, 128, 256]
+    form(8, 1, 1)
+    L = nat._lib.ic_linear_form
+    assert L(0, -1, 5) == -1 and L(0, 5, 0) == -1 and L(3, 5, 5) == -1 and L(-1, 5, 5) == -1
 
 
 class Problem:
@@ -93,7 +99,7 @@ class Problem:
 @pytest.mark.parametrize("kind,asym", KINDS)
 @pytest.mark.parametrize("tile,M,N", SIZES)
 def test_against_64_bits(gpu_dev, tile, M, N, kind, asym):
-    assert form(M, N) == tile
+    assert form(kind, M, N) == tile
     for K in DEPTHS:
         p = Problem(kind, asym, M, N, K, gpu_dev, M + N + K, with_bias=K % 2 == 1)
         act = p.activations()
@@ -112,9 +118,9 @@ def test_rows_do_not_depend_on_the_form(gpu_dev, kind, asym):
     M, N, K = 3300, 3901, 1300
     p = Problem(kind, asym, M, N, K, gpu_dev, 11)
     full = p.run(p.activations())
-    seen = {form(M, N)}
+    seen = {form(kind, M, N)}
     for lo, hi in ((0, 1500), (700, 2000), (100, 165), (3299, 3300), (256, 320), (1, 18)):
-        seen.add(form(hi - lo, N))
+        seen.add(form(kind, hi - lo, N))
         part = p.run(p.activations(slice(lo, hi)))
         if kind == "mx":
             assert ((part.double() - full[lo:hi].double()).abs() <= 2 * p.room[lo:hi]).all()
@@ -124,12 +130,12 @@ def test_rows_do_not_depend_on_the_form(gpu_dev, kind, asym):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tile,M,N", [(128, 1025, 1000), (256, 3300, 3904)])
+@pytest.mark.parametrize("tile,M,N", [(128, 1345, 1000), (256, 3300, 3904)])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_largest_sums(gpu_dev, bits, tile, M, N):
     """Codes at the ends of their ranges over the longest K: the 32-bit sums and the 24-bit zero-point products hold."""
     import int_crush_converter_amd as icq
-    assert form(M, N) == tile
+    assert form(bits, M, N) == tile
     K = 65536
     lo, hi = (-8, 7) if bits == 4 else (-128, 127)
     for qv, zv in ((lo, hi), (hi, lo)):
@@ -147,13 +153,13 @@ def test_largest_sums(gpu_dev, bits, tile, M, N):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tile,M,N", [(128, 1025, 1003), (128, 2900, 3704), (256, 5100, 5104)])
+@pytest.mark.parametrize("tile,M,N", [(128, 1345, 1003), (128, 4400, 3704), (256, 5100, 5104)])
 @pytest.mark.parametrize("kind", [8, 4, "mx"])
 def test_nan_scales_stay_in_their_rows(gpu_dev, tile, M, N, kind):
     """A NaN scale in a tile's first, inner and last row makes those rows NaN and no other (in E2M1 one block does, and a
     weight's block its column)."""
     import int_crush_converter_amd as icq
-    assert form(M, N) == tile
+    assert form(kind, M, N) == tile
     p = Problem(kind, kind != "mx", M, N, 700, gpu_dev, 3, with_bias=False)
     rows, cols = [0, 77, tile, tile + 33, M - 1], [5, N - 1]
     want = torch.zeros(M, N, dtype=torch.bool, device=gpu_dev)
@@ -174,11 +180,11 @@ def test_nan_scales_stay_in_their_rows(gpu_dev, tile, M, N, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tile,M,N", [(128, 1025, 1000), (256, 3300, 3904)])
+@pytest.mark.parametrize("tile,M,N", [(128, 1345, 1000), (256, 3300, 3904)])
 def test_graph_of_tiles(gpu_dev, tile, M, N):
     """A captured chain with tiled products gives the eager result on every replay, eager work in between."""
     import int_crush_converter_amd as icq
-    assert form(M, N) == tile
+    assert {form(k, M, N) for k in (8, 4, "mx")} == {tile}
     g = torch.Generator(device=gpu_dev).manual_seed(M)
     K = 640
     rand = lambda *s: torch.randn(*s, generator=g, device=gpu_dev)                              # noqa: E731
