@@ -165,8 +165,8 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
     x: [..., K] float32 / bfloat16 / float16; residual: like x or None; weight: [K].  rot_size: 0 (none), 4, 16, 64
     or 256, the size the weights were rotated with; rows are zero-padded to a multiple of it.  Returns the activations
     and ``h`` in x's dtype (None without a residual).  The norm sees the fp32 sum, not its rounding, and holds for any
-    finite row.  A row that holds Inf or NaN, or whose rotated values pass fp32's range, gets the scale NaN and codes
-    0, and leaves the other rows as they are."""
+    finite row.  A row that holds Inf or NaN, or whose rotated values pass a quarter of fp32's range, gets the scale
+    NaN and codes 0, and leaves the other rows as they are."""
     if weight is None:
         raise ValueError("rms_norm_quantize needs the norm's weight; quantize_activations is the form without a norm")
     return _quantize(x, weight, residual, float(eps), rot_size)

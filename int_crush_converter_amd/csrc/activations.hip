@@ -100,11 +100,14 @@ __device__ __forceinline__ T row_reduce(T v, T* lds, F op) {
 }
 
 // WAVES waves hold one row, NC chunks of 16 columns a lane; for WAVES = 1 a
-// work-group of 4 waves holds 4 rows.  HBM bounds it: 8192 x 4096 bf16 with
-// residual and rotation 51 us, 4.6 TB/s; 8192 x 12288 without rotation 57 us,
-// 5.3 TB/s (a large copy: 5.1).  Four waves a row with one chunk a lane, as one
-// wave with four of them took 62 us for the first: three reductions meet at
-// barriers, but four times the waves cover the loads' latency.
+// work-group of 4 waves holds 4 rows.  HBM bounds it.  Traced alone (median of
+// 30): 8192 x 4096 bf16 with residual and rotation 43.8 us, 5.4 TB/s; 8192 x
+// 12288 without rotation 61.5 us (least 56.4), 4.9 TB/s; one call after another
+// 41.8 and 53.7 us (a large copy: 5.1 TB/s).  Four waves a row with one chunk a
+// lane, as one wave with four of them took a fifth longer for the first (62
+// against 51 us, with the loads of that time): three reductions meet at
+// barriers, but four times the waves cover the loads' latency.  16 waves of
+// four chunks spill 16 registers of the row.
 template <int DT, int WAVES, int NC>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_kernel(
     const void* __restrict__ x, int64_t rows, int64_t cols, int64_t ld_x, const void* residual, int64_t ld_r,
@@ -228,7 +231,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
 }
 
 // q * s back as values: one lane per 16 codes.  HBM-bound: 8192 x 12288 to bf16
-// 57 us, 5.3 TB/s.
+// 48.2 us traced alone, 6.3 TB/s (behind the quantisation, whose codes are partly
+// in cache).
 template <int DT>
 __global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* __restrict__ codes, int64_t rows,
                                                               int64_t cols, int64_t ld_q,

@@ -139,9 +139,11 @@ __device__ __forceinline__ lb_u32x4 to_operand(lb_u32x4 v, int from) {
 
 // Few rows: a work-group of 8 waves takes 16 columns of y and 16 MT rows,
 // its waves a share of K each; the sums are joined in LDS in a fixed order.
-// One row is bound by the weights' bytes and the launch: INT4 1 x 12288 x 4096
-// 6.4 us (25 MB, 4.0 TB/s); more rows by their activations, which every
-// work-group reads again: INT8 333 x 1000 x 2901 10.7 us.
+// One row is bound by the weights' bytes (25 MB) and the launch: INT4 1 x 12288 x
+// 4096 6.4 us traced alone, 5.3 us a call in a graph with its weights in cache
+// (4.8 TB/s), 8.3 us from HBM (3.0 TB/s, many weights in turn); MXFP4 8 x 4096 x
+// 12288 6.1, 5.6 and 11.4 us.  More rows are bound by their activations, which
+// every work-group reads and exchanges again: INT8 333 x 1000 x 2901 10.8 us.
 template <int KIND, int MT>
 __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
     typedef typename Acc<KIND>::T acc_t;
@@ -231,14 +233,23 @@ __device__ __forceinline__ void meet() {
 // barrier that a stage has: when it gets there, what is left of the stage is
 // in registers, and its buffer is filled again.
 //
-// Measured: INT4 8192 x 4096 x 12288 312 us, 2.6 POP/s; MXFP4 8192 x 12288 x
-// 4096 222 us, 3.7 PFLOP/s.  What bounds the first is power: the chip clocks
-// at 1.75 GHz under it, its matrix units are busy for 65 % of the cycles, and
-// the same instructions with the same reads from LDS and nothing else reach
-// 2.7 POP/s on random operands (5.4 PFLOP/s for E2M1; 3.5 and 6.5 from
-// registers alone).  The second loses a fifth to the ends of its 32-stage
-// tiles.  4 waves of 128 x 128 read less LDS but took 383 and 301 us, a wave
-// alone on its SIMD standing still at copies, barriers and outputs.
+// Measured, one call after another: INT4 8192 x 4096 x 12288 326 us, 2.5 POP/s
+// (341 to 345 on another card; traced alone 325 to 376); MXFP4 8192 x 12288 x
+// 4096 226 us, 3.7 PFLOP/s (traced 216 to 256).  What bounds the first is power:
+// the chip clocks at 1.7 GHz under it, its matrix units are busy for 63 % of the
+// cycles, and the same instructions with the same reads from LDS and nothing
+// else reach 2.7 POP/s on random operands, 305 us (5.4 PFLOP/s for E2M1, 153 us
+// for the second; 3.5 and 6.5 from registers alone).  The second's matrix units
+// are busy for 47 %: nobody multiplies at the ends of its 32-stage tiles.  4
+// waves of 128 x 128 read less LDS but took 383 and 301 us, a wave alone on its
+// SIMD standing still at copies, barriers and outputs.  For INT4 an earlier
+// kernel with 16 x 16 instructions, a work-group a tile, was faster: 318 to 323
+// us where this one took 341 to 345 in turn on the same card.
+//
+// The 256 x 256 forms of INT4 and INT8 spill 22 and 8 registers, at a tile's
+// start and end, none in the K loop.  Spills are vector-memory operations like
+// those that meet() counts.  It lets the newest N stay outstanding; with spills
+// among these it waits for more copies than it needs, never for fewer.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
     typedef typename Acc32<KIND>::T acc_t;

@@ -47,7 +47,8 @@ __device__ __forceinline__ lb_u32x4 quantize_block(float (&a)[16], float (&b)[16
 
 // One wave per tile of 16 rows x 128 columns; the four waves of a work-group
 // take the four tiles that share a word of scales.  HBM-bound: 8192 x 12288 bf16
-// 52 us, 4.9 TB/s; 5000 x 2900 fp16, rows at no alignment, 10.8 us, 3.4 TB/s.
+// 57.1 us (least 52.4), 4.5 TB/s; 5000 x 2900 fp16, rows at no alignment, 9.7 us,
+// 3.8 TB/s (traced alone, medians of 30).
 template <int DT>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const void* __restrict__ x, int64_t rows, int64_t cols,
                                                              int64_t ld, lb_u32x4* __restrict__ codes,
@@ -66,8 +67,9 @@ __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const void* __restr
 }
 
 // One wave per tile again, but a lane takes 8 columns of one row at a time, so
-// that 16 lanes write 128 consecutive values: 8192 x 12288 to bf16 54 us, 4.7
-// TB/s, where 32 columns a lane took 81 us (64 bytes of 64 rows a store).
+// that 16 lanes write 128 consecutive values: 8192 x 12288 to bf16 37.6 us traced
+// alone, 6.8 TB/s (behind the quantisation, whose codes are in cache); 32 columns
+// a lane (64 bytes of 64 rows a store) took half as long again.
 template <int DT>
 __global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales, int64_t rows,
