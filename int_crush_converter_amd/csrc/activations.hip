@@ -22,6 +22,7 @@ inline dim3 group_grid(int64_t groups) {
 __device__ __forceinline__ int64_t group_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 
 constexpr float kTinyMax = 1e-30f;   // the smallest row maximum that a scale stands for
+constexpr float kTopScale = 0x1.020406p+121f;   // the largest whose 127-fold is finite (fp32's largest value / 127 rounds up)
 
 __device__ __forceinline__ void bfly4(float& a, float& b, float& c, float& d) {
     const float s = (a + b) + (c + d);
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void quantize_rows_k
     }
     sum = row_reduce<WAVES>(sum, red_i, [](int a, int b) { return a + b; });
     if (lane == 0) {
-        scales[row] = bad ? __uint_as_float(0x7fc00000u) : peak / 127.0f;
+        scales[row] = bad ? __uint_as_float(0x7fc00000u) : fminf(peak / 127.0f, kTopScale);
         sums[row] = sum;
     }
 }

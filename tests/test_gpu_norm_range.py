@@ -68,3 +68,17 @@ def test_fp16_rows_are_never_out_of_range(gpu_dev):
     x[1] = 2.0 ** -24
     _, z = exact(x, torch.ones(65536, dtype=F16), None, 1e-6, 1)
     check(icq.rms_norm_quantize(x.to(gpu_dev), torch.ones(65536, device=gpu_dev, dtype=F16))[0], z)
+
+
+@pytest.mark.parametrize("K", [3, 5000, 20000])
+def test_the_largest_value_comes_back_finite(gpu_dev, K):
+    """The scale of a row that holds fp32's largest value (a mask's, say) gives no infinity when it is undone."""
+    import int_crush_converter_amd as icq
+    top = torch.finfo(F32).max
+    x = torch.randn(4, K)
+    x[0, 1], x[1, K - 1], x[2, 0] = top, -top, float(torch.nextafter(torch.tensor(top), torch.tensor(0.0)))
+    q = icq.quantize_activations(x.to(gpu_dev))
+    check(q, x.double())
+    back = q.dequantize(F32).cpu()
+    assert torch.isfinite(back).all()
+    assert (back[0, 1] / top - 1).abs() < 2.0 ** -22 and (back[1, K - 1] / -top - 1).abs() < 2.0 ** -22
