@@ -518,6 +518,75 @@ int ic_quantized_linear(const int8_t* a, int64_t ld_a, const float* sa, const in
  * ic_quantized_linear with INT8 and INT4 weights, 2 = ic_mxfp4_linear. */
 int ic_linear_form(int kind, int64_t M, int64_t N);
 
+/* Rows of activations and the groups (experts, adapters) they belong to.  A
+ * row has per_row (or `top`) choices; pair p = row * per_row + choice.
+ *   ids      int32 [rows, per_row]: the pair's group, -1 = none
+ *   offsets  int32 [groups + 1]: pairs ordered by group, in each group in
+ *            their own order; group g has places offsets[g] .. offsets[g+1]-1
+ *   order    int32 [rows * per_row]: the pair at a place, -1 behind the last
+ *   position int32 [rows, per_row]: the pair's place, -1 = none
+ * At most 1024 groups, 64 choices a row, 1048560 pairs.  Workspace:
+ * ic_group_workspace_bytes(rows, groups). */
+int64_t ic_group_workspace_bytes(int64_t rows, int64_t groups);
+
+/* The order of given ids (int32, or int64 with wide 1) [rows, per_row],
+ * contiguous; ids outside [0, groups) are none.  ids: a copy, -1 for those. */
+int ic_group_rows(const void* given, int wide, int64_t rows, int64_t per_row, int64_t groups, int32_t* ids,
+                  int32_t* offsets, int32_t* order, int32_t* position, void* workspace, void* stream);
+
+/* A router: each token's `top` largest of logits [tokens, experts] (of equals
+ * the lowest; NaN above all; -inf is never chosen and leaves the choice none),
+ * largest first, their weights fp32 exp(x - max) / sum, the sum over the
+ * chosen (renormalize 1) or over all experts (0); none weighs 0.  A token with
+ * NaN or +inf has weights NaN. */
+int ic_route_tokens(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int top,
+                    int renormalize, int32_t* ids, float* weights, int32_t* offsets, int32_t* order,
+                    int32_t* position, void* workspace, void* stream);
+
+/* out[t] = residual[t] + sum_j weights[t, j] y[position[t, j]], in fp32, j in
+ * order, none left out; y [tokens * top, cols], residual (may be NULL, may be
+ * out) and out [tokens, cols] of `dtype`. */
+int ic_combine_rows(const void* y, int dtype, int64_t tokens, int64_t top, int64_t cols, int64_t ld_y,
+                    const int32_t* position, const float* weights, const void* residual, int64_t ld_r, void* out,
+                    int64_t ld_out, void* stream);
+
+/* ic_quantized_linear with a weight for each group: row i of out, the place i
+ * of an order by group, is the product of a row of the activations with the
+ * weight of its group: of row i (top 0; a_rows = rows), or of row order[i] /
+ * top (top > 0; a_rows * ld_a below 2^32).  tiles, sw, zp, bias [groups, N]:
+ * those of all groups, one after another (tiles ic_linear_weight_bytes()
+ * each).  Rows of out behind offsets[groups] are left as they were. */
+int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t a_rows,
+                     const int32_t* offsets, const int32_t* order, int top, int64_t groups, int64_t rows,
+                     const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,
+                     int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out, void* stream);
+
+/* Which form ic_expert_linear takes for these sizes: 16, 32 or 64 (rows
+ * directly from memory, so many at a time), 128 or 256 (tiles). */
+int ic_expert_form(int64_t rows, int64_t groups);
+
+/* Low-rank adapters, bf16 or fp16: a [adapters, rank, K] and b [adapters, N,
+ * rank], contiguous, laid out once for ic_adapted_linear (ic_adapter_down_bytes
+ * and ic_adapter_up_bytes, 16-byte aligned).  At most 1024 of rank 128. */
+int64_t ic_adapter_down_bytes(int64_t adapters, int rank, int64_t K);
+int64_t ic_adapter_up_bytes(int64_t adapters, int64_t N, int rank);
+int ic_adapter_pack(const void* a, const void* b, int64_t adapters, int rank, int64_t N, int64_t K, void* down,
+                    void* up, void* stream);
+
+/* ic_quantized_linear beside which row m adds the adapter ids[m] of its own
+ * (none for ids outside [0, adapters)):
+ *   out[m, n] += scaling[a] sum_r b[a, n, r] sum_k a[a, r, k] sa[m] q[m, k]
+ * down, up: from ic_adapter_pack, of adapter_dtype; scaling fp32 [adapters];
+ * ids, offsets and order: of ic_group_rows with one choice a row and
+ * `adapters` groups.  Workspace: ic_adapted_linear_workspace_bytes(M, rank),
+ * 16-byte aligned. */
+int64_t ic_adapted_linear_workspace_bytes(int64_t M, int rank);
+int ic_adapted_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t M,
+                      const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,
+                      int bias_dtype, int64_t N, int64_t K, const void* down, const void* up, int adapter_dtype,
+                      int64_t adapters, int rank, const float* scaling, const int32_t* ids, const int32_t* offsets,
+                      const int32_t* order, void* workspace, void* out, int out_dtype, int64_t ld_out, void* stream);
+
 /* Microscaled 4-bit floating point (OCP MX): E2M1 elements, one E8M0 scale
  * for 32 consecutive columns, 2^(floor(log2(max|x|)) - 2); elements to the
  * nearest, ties to even, at most 6.  A block with Inf or NaN: scale byte 255,

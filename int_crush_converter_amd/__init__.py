@@ -4,8 +4,9 @@ Public names mirror the reference package ``converter`` (its ``__init__.py``)
 for the hot path: rotation, RTN scales, PiSO scales, packing, DLR Hessians,
 GPTQ / LDLQ layers, the pipeline and the value types.  Beside them stand the
 operators that run what it produced (no counterpart in the reference): norm
-and quantisation of activations, products with the stored weights, and the
-microscaled 4-bit format.  The reference's
+and quantisation of activations, products with the stored weights, one at a
+time, grouped by expert or with the low-rank adapters of many requests, the
+router that orders rows by expert, and the microscaled 4-bit format.  The reference's
 SmoothQuant / SmoothRot / SVD helpers are outside this path and not
 exported.  All arithmetic runs in the gfx950 HIP library
 ``libicq.so`` (see ``include/ic_abi.h``); there is no CPU fallback.
@@ -44,7 +45,10 @@ from .ldlq import ldlq_quantize_layer
 from .calibration_io import load_calibration, build_name_map, get_hessian, get_per_channel_amax
 from .pipeline import quantize_model, should_skip
 from .activations import QuantizedActivations, rms_norm_quantize, quantize_activations
+from .groups import RowGroups, group_rows, route_tokens, combine_experts
+from .adapters import LowRankAdapters
 from .linear import QuantizedWeight, quantized_linear
+from .experts import ExpertWeight, expert_linear
 from .mxfp4 import Mxfp4Tensor, mxfp4_quantize, mxfp4_linear
 from .types import QuantizationResult, QuantizeConfig, ProgressInfo, ProgressSummary, ProgressCallback
 
@@ -64,5 +68,6 @@ __all__ = [
     "compute_piso_scales_int8", "compute_piso_scales_int8_asymmetric",
     "compute_piso_scales_int4", "compute_piso_scales_int4_asymmetric",
     "QuantizedActivations", "rms_norm_quantize", "quantize_activations", "QuantizedWeight", "quantized_linear",
+    "RowGroups", "group_rows", "route_tokens", "combine_experts", "ExpertWeight", "expert_linear", "LowRankAdapters",
     "Mxfp4Tensor", "mxfp4_quantize", "mxfp4_linear",
 ]

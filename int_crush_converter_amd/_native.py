@@ -104,6 +104,19 @@ _SIGS = {
     "ic_linear_pack_weight": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp]),
     "ic_quantized_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp,
                                    _i32, _i64, _vp]),
+    "ic_group_workspace_bytes": (_i64, [_i64, _i64]),
+    "ic_group_rows": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ic_route_tokens": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ic_combine_rows": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp]),
+    "ic_expert_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _vp,
+                                _i32, _i64, _i64, _vp, _i32, _i64, _vp]),
+    "ic_expert_form": (_i32, [_i64, _i64]),
+    "ic_adapter_down_bytes": (_i64, [_i64, _i32, _i64]),
+    "ic_adapter_up_bytes": (_i64, [_i64, _i64, _i32]),
+    "ic_adapter_pack": (_i32, [_vp, _vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp]),
+    "ic_adapted_linear_workspace_bytes": (_i64, [_i64, _i32]),
+    "ic_adapted_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp, _vp,
+                                 _i32, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _vp]),
     "ic_mxfp4_code_bytes": (_i64, [_i64, _i64]),
     "ic_mxfp4_scale_bytes": (_i64, [_i64, _i64]),
     "ic_mxfp4_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),

@@ -1,0 +1,389 @@
+// Rows of activations and the groups they belong to: the router's choice of
+// experts for a token, the order of (row, choice) pairs by group, and the
+// weighted sum that brings the ordered rows back.
+//
+//   chosen:  the k largest of x[t, :], of equals the lowest; -inf is never chosen
+//   weight:  exp(x_e - m) / sum exp(x - m), m = max x, over the chosen or over all
+//   order:   pair t k + j is at offsets[g] + #{earlier pairs of group g}
+//   back:    y[t] = r[t] + sum_j w[t, j] y[position[t, j]]
+//
+// The order is that of a counting sort whose counts are integers, so it does
+// not depend on which work-group comes first.
+#include "common.hpp"
+#include "groups.hpp"
+#include "lowbit.hpp"
+#include "prof.hpp"
+
+namespace icq {
+namespace {
+
+constexpr int kThreads = 1024;          // of a work-group that counts or places
+constexpr int kMaxTop = 64;
+
+__device__ __forceinline__ unsigned wave_max_u32(unsigned v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const unsigned u = (unsigned)__shfl_xor((int)v, o, 64);
+        v = v > u ? v : u;
+    }
+    return v;
+}
+
+// Keys order like the values, a NaN above all of them and the two zeros equal;
+// 0 is what a mask (-inf) took out, or what has been chosen already.
+__device__ __forceinline__ unsigned logit_key(float x) {
+    if (x != x) return 0xffffffffu;
+    return x == -INFINITY ? 0u : float_key(x + 0.0f);
+}
+__device__ __forceinline__ float key_logit(unsigned k) { return k == 0xffffffffu ? __uint_as_float(0x7fc00000u) : key_float(k); }
+
+// The choice of one token by one wave: expert i * 64 + lane in slot i.  Each
+// choice is a maximum over the lanes and a search for its first place.
+template <int DT, int SLOTS>
+__device__ __forceinline__ void choose(const void* logits, int64_t at, int experts, int top, int renormalize,
+                                       int& id, float& weight) {
+    const int lane = threadIdx.x & 63;
+    unsigned key[SLOTS];
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+        const int e = i * 64 + lane;
+        key[i] = e < experts ? logit_key(load_as_f32(logits, DT, at + e)) : 0u;
+    }
+    unsigned own = 0;                    // the lane's largest
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) own = own > key[i] ? own : key[i];
+    unsigned best = wave_max_u32(own);
+    const float peak = key_logit(best);
+    float total = 0.0f;
+    if (!renormalize) {
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) total += key[i] ? expf(key_logit(key[i]) - peak) : 0.0f;
+        total = wave_sum(total);
+    }
+    id = -1;
+    float e = 0.0f;
+    for (int j = 0; j < top && best; ++j) {
+        int slot = 0;
+        unsigned long long at_best = 0;
+#pragma unroll
+        for (int i = SLOTS - 1; i >= 0; --i) {
+            const unsigned long long here = __ballot(key[i] == best);
+            if (here) { at_best = here; slot = i; }
+        }
+        const int first = __builtin_ctzll(at_best);
+        if (lane == j) {
+            id = slot * 64 + first;
+            e = expf(key_logit(best) - peak);
+        }
+        own = 0;
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+            if (i == slot && lane == first) key[i] = 0;
+            own = own > key[i] ? own : key[i];
+        }
+        best = wave_max_u32(own);
+    }
+    if (renormalize) total = wave_sum(e);
+    weight = id < 0 ? 0.0f : e / total;
+}
+
+// What a unit of consecutive pairs adds to each group, for the units behind it.
+struct Units {
+    int64_t pairs;       // of all units
+    int per_unit, units, groups;
+    int32_t* counts;     // [units, groups]
+};
+
+// Places this unit's pairs: groups' ids from `ids` (-1: none, ordered behind
+// all groups), edges and earlier units' shares from the counts.  lds: 3 x 1024
+// ints and a few.
+struct PlaceLds {
+    int total[kMaxGroups], before[kMaxGroups], base[kMaxGroups + 1], waves[2][kThreads / 64];
+};
+__device__ __forceinline__ void place_unit(const Units& u, int unit, const int32_t* ids, PlaceLds& s, int32_t* offsets,
+                                           int32_t* order, int32_t* position) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // threads in rows of `width`: column = group, each row sums every so manieth unit
+    const int width = u.groups <= 64 ? 64 : u.groups <= 128 ? 128 : u.groups <= 256 ? 256 : u.groups <= 512 ? 512 : 1024;
+    const int g = tid & (width - 1), row = tid / width, rows = kThreads / width;
+    s.total[tid] = 0;
+    s.before[tid] = 0;
+    __syncthreads();
+    if (g < u.groups) {
+        int total = 0, before = 0;
+#pragma unroll 8
+        for (int k = row; k < u.units; k += rows) {
+            const int c = u.counts[(int64_t)k * u.groups + g];
+            total += c;
+            before += k < unit ? c : 0;
+        }
+        atomicAdd(&s.total[g], total);       // integers: any order gives the same sum
+        atomicAdd(&s.before[g], before);
+    }
+    __syncthreads();
+    const int total = s.total[tid], before = s.before[tid];      // (zeros behind the last group)
+    const int upto = wave_scan(total), earlier = wave_scan(before);
+    if (lane == 63) {
+        s.waves[0][wave] = upto;
+        s.waves[1][wave] = earlier;
+    }
+    __syncthreads();
+    int start = upto - total, all = 0, mine = 0;
+    for (int w = 0; w < kThreads / 64; ++w) {
+        start += w < wave ? s.waves[0][w] : 0;
+        all += s.waves[0][w];
+        mine += s.waves[1][w];
+    }
+    const int64_t first = (int64_t)unit * u.per_unit;
+    if (tid < u.groups) s.base[tid] = start + before;
+    if (tid == 0) s.base[u.groups] = all + (int)(first - mine);          // pairs of no group
+    if (unit == 0) {
+        if (tid < u.groups) offsets[tid] = start;
+        if (tid == 0) offsets[u.groups] = all;
+    }
+    __syncthreads();
+    if (wave) return;
+    // one wave goes through the unit in order, 64 pairs at a time
+    const int64_t last = first + u.per_unit < u.pairs ? first + u.per_unit : u.pairs;
+    for (int64_t p0 = first; p0 < last; p0 += 64) {
+        const int64_t p = p0 + lane;
+        const bool have = p < last;
+        const int id = have ? ids[p] : -1, key = id < 0 ? u.groups : id;
+        unsigned long long same = __ballot(have);
+        for (int b = 0; (u.groups >> b) != 0; ++b) {
+            const unsigned long long m = __ballot((key >> b) & 1);
+            same &= (key >> b) & 1 ? m : ~m;
+        }
+        const int rank = (int)__builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
+        const int at = s.base[key] + rank;
+        lds_wave_fence();
+        if (have && rank == 0) s.base[key] += __builtin_popcountll(same);
+        lds_wave_fence();
+        if (have) {
+            order[at] = id < 0 ? -1 : (int32_t)p;
+            position[p] = id < 0 ? -1 : at;
+        }
+    }
+}
+
+// Tokens of a unit, a wave each in turn; with one unit the pairs are placed at once.
+template <int DT, int SLOTS>
+__global__ __launch_bounds__(kThreads) void route_kernel(const void* __restrict__ logits, int64_t tokens, int64_t ld, int top,
+                                                         int renormalize, int tokens_per_unit, Units u,
+                                                         int32_t* __restrict__ ids, float* __restrict__ weights,
+                                                         int32_t* offsets, int32_t* order, int32_t* position) {
+    __shared__ PlaceLds s;
+    const int tid = threadIdx.x, lane = tid & 63, unit = blockIdx.x;
+    int* count = s.total;
+    count[tid] = 0;
+    __syncthreads();
+    const int64_t t0 = (int64_t)unit * tokens_per_unit, t1 = t0 + tokens_per_unit < tokens ? t0 + tokens_per_unit : tokens;
+    for (int64_t t = t0 + (tid >> 6); t < t1; t += kThreads / 64) {
+        int id;
+        float w;
+        choose<DT, SLOTS>(logits, t * ld, u.groups, top, renormalize, id, w);
+        if (lane < top) {
+            ids[t * top + lane] = id;
+            weights[t * top + lane] = w;
+            if (id >= 0) atomicAdd(&count[id], 1);
+        }
+    }
+    __syncthreads();
+    for (int g = tid; g < u.groups; g += kThreads) u.counts[(int64_t)unit * u.groups + g] = count[g];
+    if (u.units == 1) {
+        __syncthreads();
+        place_unit(u, 0, ids, s, offsets, order, position);
+    }
+}
+
+// Ids from elsewhere: those outside [0, groups) become -1.
+template <typename ID>
+__global__ __launch_bounds__(kThreads) void count_kernel(const ID* __restrict__ given, Units u, int32_t* __restrict__ ids,
+                                                         int32_t* offsets, int32_t* order, int32_t* position) {
+    __shared__ PlaceLds s;
+    const int tid = threadIdx.x, unit = blockIdx.x;
+    int* count = s.total;
+    count[tid] = 0;
+    __syncthreads();
+    const int64_t first = (int64_t)unit * u.per_unit, last = first + u.per_unit < u.pairs ? first + u.per_unit : u.pairs;
+    for (int64_t p = first + tid; p < last; p += kThreads) {
+        const ID id = given[p];
+        const bool is = id >= 0 && id < u.groups;
+        ids[p] = is ? (int32_t)id : -1;
+        if (is) atomicAdd(&count[(int)id], 1);
+    }
+    __syncthreads();
+    for (int g = tid; g < u.groups; g += kThreads) u.counts[(int64_t)unit * u.groups + g] = count[g];
+    if (u.units == 1) {
+        __syncthreads();
+        place_unit(u, 0, ids, s, offsets, order, position);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void place_kernel(Units u, const int32_t* __restrict__ ids, int32_t* offsets,
+                                                         int32_t* order, int32_t* position) {
+    __shared__ PlaceLds s;
+    place_unit(u, blockIdx.x, ids, s, offsets, order, position);
+}
+
+// Units of whole rows (a row has `per_row` pairs): at least 16 rows, one a wave
+// of the work-group, and at most 256 units.
+int rows_per_unit(int64_t rows) {
+    const int64_t n = cdiv(rows, 256);
+    return (int)(n < 16 ? 16 : n);
+}
+
+// Rows back to their tokens: a lane has 8 columns, and the k rows' loads in
+// flight together (8 at a time).
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t base, int c0, int cols, float (&v)[8]) {
+    if (c0 + 8 <= cols) {
+        if (DT == IC_DTYPE_F32) {
+            const lb_f32x4_any* q = reinterpret_cast<const lb_f32x4_any*>(static_cast<const float*>(p) + base + c0);
+            const lb_f32x4 a = q[0], b = q[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+        } else {
+            const lb_u32x4 t = *reinterpret_cast<const lb_u32x4_any*>(static_cast<const uint16_t*>(p) + base + c0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = half_word<DT>(t[i], 0);
+                v[2 * i + 1] = half_word<DT>(t[i], 1);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? load_as_f32(p, DT, base + c0 + i) : 0.0f;
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void combine_kernel(const void* __restrict__ y, int64_t pairs, int cols, int64_t ld_y,
+                                                      const int32_t* __restrict__ position, const float* __restrict__ weights,
+                                                      int top, const void* residual, int64_t ld_r, void* out, int64_t ld_out,
+                                                      int chunks) {
+    const int64_t t = blockIdx.x / (unsigned)chunks;
+    const int c0 = ((int)(blockIdx.x % (unsigned)chunks) * 256 + threadIdx.x) * 8;
+    if (c0 >= cols) return;
+    float sum[8];
+    if (residual) load8<DT>(residual, t * ld_r, c0, cols, sum);
+    else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+    }
+    for (int j = 0; j < top; ++j) {
+        const int at = position[t * top + j];
+        if (at < 0 || at >= pairs) continue;
+        const float w = weights[t * top + j];
+        float v[8];
+        load8<DT>(y, at * ld_y, c0, cols, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(w, v[i], sum[i]);
+    }
+    store_cols<DT, 8>(out, t * ld_out, c0, cols, sum);
+}
+
+int check_groups(const char* who, int64_t rows, int64_t per_row, int64_t groups) {
+    const std::string w(who);
+    if (rows < 0 || per_row < 1 || groups < 1) return fail(IC_ERR_ARG, w + ": rows must be >= 0, groups and choices >= 1");
+    if (groups > kMaxGroups || per_row > kMaxTop || rows > kMaxRows || rows * per_row > kMaxRows)
+        return fail(IC_ERR_RANGE, w + ": at most 1024 groups, 64 choices a row and 1048560 pairs");
+    return IC_OK;
+}
+
+template <int DT>
+void launch_route(const void* logits, int64_t tokens, int64_t ld, int top, int renormalize, int per, const Units& u, int32_t* ids,
+                  float* weights, int32_t* offsets, int32_t* order, int32_t* position, hipStream_t st) {
+    auto go = [&](auto slots) {
+        hipLaunchKernelGGL((route_kernel<DT, decltype(slots)::value>), dim3(u.units), dim3(kThreads), 0, st, logits, tokens, ld, top,
+                           renormalize, per, u, ids, weights, offsets, order, position);
+    };
+    if (u.groups <= 64) go(std::integral_constant<int, 1>{});
+    else if (u.groups <= 128) go(std::integral_constant<int, 2>{});
+    else if (u.groups <= 256) go(std::integral_constant<int, 4>{});
+    else if (u.groups <= 512) go(std::integral_constant<int, 8>{});
+    else go(std::integral_constant<int, 16>{});
+}
+
+}  // namespace
+}  // namespace icq
+
+using namespace icq;
+
+extern "C" int64_t ic_group_workspace_bytes(int64_t rows, int64_t groups) {
+    if (rows < 0 || groups < 1 || groups > kMaxGroups || rows > kMaxRows) return 0;
+    return cdiv(rows, rows_per_unit(rows)) * groups * 4;
+}
+
+extern "C" int ic_route_tokens(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int top, int renormalize,
+                               int32_t* ids, float* weights, int32_t* offsets, int32_t* order, int32_t* position,
+                               void* workspace, void* stream) {
+    if (const int rc = check_groups("ic_route_tokens", tokens, top, experts)) return rc;
+    IC_REQUIRE(dtype >= 0 && dtype <= 2, "ic_route_tokens: unknown dtype");
+    IC_REQUIRE(top <= experts, "ic_route_tokens: more choices than experts");
+    IC_REQUIRE(offsets && (tokens == 0 || (logits && ids && weights && order && position && workspace)),
+               "ic_route_tokens: null pointer");
+    IC_REQUIRE(tokens <= 1 || ld >= experts, "ic_route_tokens: leading dimension below the number of experts");
+    hipStream_t st = as_stream(stream);
+    const int per = rows_per_unit(tokens);
+    const int units = tokens ? (int)cdiv(tokens, per) : 1;
+    ProfScope prof(st, PT_OTHER, 0.0, (double)tokens * experts * (dtype == IC_DTYPE_F32 ? 4 : 2) + 16.0 * tokens * top);
+    const Units u{tokens * top, per * top, units, (int)experts, static_cast<int32_t*>(workspace)};
+    if (tokens == 0) {
+        hipLaunchKernelGGL(place_kernel, dim3(1), dim3(kThreads), 0, st, Units{0, 1, 0, (int)experts, nullptr}, ids, offsets, order, position);
+        IC_CHECK_LAUNCH();
+        return IC_OK;
+    }
+    if (dtype == IC_DTYPE_F32) launch_route<IC_DTYPE_F32>(logits, tokens, ld, top, renormalize, per, u, ids, weights, offsets, order, position, st);
+    else if (dtype == IC_DTYPE_BF16) launch_route<IC_DTYPE_BF16>(logits, tokens, ld, top, renormalize, per, u, ids, weights, offsets, order, position, st);
+    else launch_route<IC_DTYPE_F16>(logits, tokens, ld, top, renormalize, per, u, ids, weights, offsets, order, position, st);
+    if (units > 1) hipLaunchKernelGGL(place_kernel, dim3(units), dim3(kThreads), 0, st, u, ids, offsets, order, position);
+    IC_CHECK_LAUNCH();
+    return IC_OK;
+}
+
+extern "C" int ic_group_rows(const void* given, int wide, int64_t rows, int64_t per_row, int64_t groups, int32_t* ids, int32_t* offsets,
+                             int32_t* order, int32_t* position, void* workspace, void* stream) {
+    if (const int rc = check_groups("ic_group_rows", rows, per_row, groups)) return rc;
+    IC_REQUIRE(offsets && (rows == 0 || (given && ids && order && position && workspace)), "ic_group_rows: null pointer");
+    hipStream_t st = as_stream(stream);
+    const int per = rows_per_unit(rows);
+    const int units = rows ? (int)cdiv(rows, per) : 1;
+    ProfScope prof(st, PT_OTHER, 0.0, (wide ? 20.0 : 16.0) * rows * per_row);
+    const Units u{rows * per_row, (int)(per * per_row), units, (int)groups, static_cast<int32_t*>(workspace)};
+    if (rows == 0) {
+        hipLaunchKernelGGL(place_kernel, dim3(1), dim3(kThreads), 0, st, Units{0, 1, 0, (int)groups, nullptr}, ids, offsets, order, position);
+        IC_CHECK_LAUNCH();
+        return IC_OK;
+    }
+    if (wide) hipLaunchKernelGGL(count_kernel<int64_t>, dim3(units), dim3(kThreads), 0, st, static_cast<const int64_t*>(given), u, ids, offsets, order, position);
+    else hipLaunchKernelGGL(count_kernel<int32_t>, dim3(units), dim3(kThreads), 0, st, static_cast<const int32_t*>(given), u, ids, offsets, order, position);
+    if (units > 1) hipLaunchKernelGGL(place_kernel, dim3(units), dim3(kThreads), 0, st, u, ids, offsets, order, position);
+    IC_CHECK_LAUNCH();
+    return IC_OK;
+}
+
+extern "C" int ic_combine_rows(const void* y, int dtype, int64_t tokens, int64_t top, int64_t cols, int64_t ld_y, const int32_t* position,
+                               const float* weights, const void* residual, int64_t ld_r, void* out, int64_t ld_out, void* stream) {
+    IC_REQUIRE(tokens >= 0 && top >= 1 && cols >= 1, "ic_combine_rows: tokens must be >= 0, top and cols >= 1");
+    IC_REQUIRE(dtype >= 0 && dtype <= 2, "ic_combine_rows: unknown dtype");
+    if (tokens > kMaxRows || top > kMaxTop || tokens * top > kMaxRows || cols > kMaxRows)
+        return fail(IC_ERR_RANGE, "ic_combine_rows: at most 64 choices a token, 1048560 pairs and as many columns");
+    if (tokens == 0) return IC_OK;
+    IC_REQUIRE(y && position && weights && out, "ic_combine_rows: null pointer");
+    IC_REQUIRE(ld_y >= cols && ld_out >= cols && (!residual || ld_r >= cols), "ic_combine_rows: leading dimension below cols");
+    const int chunks = (int)cdiv(cols, 2048);
+    if (tokens * chunks > 0x7fffff) return fail(IC_ERR_RANGE, "ic_combine_rows: more than 2^23 pieces of 2048 columns");
+    hipStream_t st = as_stream(stream);
+    const int es = dtype == IC_DTYPE_F32 ? 4 : 2;
+    ProfScope prof(st, PT_OTHER, 2.0 * tokens * top * cols, (double)es * tokens * cols * (top + (residual ? 2 : 1)));
+    auto go = [&](auto dt) {
+        hipLaunchKernelGGL(combine_kernel<decltype(dt)::value>, dim3((unsigned)(tokens * chunks)), dim3(256), 0, st, y, tokens * top,
+                           (int)cols, ld_y, position, weights, (int)top, residual, ld_r, out, ld_out, chunks);
+    };
+    if (dtype == IC_DTYPE_F32) go(std::integral_constant<int, IC_DTYPE_F32>{});
+    else if (dtype == IC_DTYPE_BF16) go(std::integral_constant<int, IC_DTYPE_BF16>{});
+    else go(std::integral_constant<int, IC_DTYPE_F16>{});
+    IC_CHECK_LAUNCH();
+    return IC_OK;
+}

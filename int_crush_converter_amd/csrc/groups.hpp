@@ -1,0 +1,83 @@
+// Rows ordered by group (expert, adapter), as the kernels that work on them see them.
+#pragma once
+
+#include "common.hpp"
+
+namespace icq {
+
+constexpr int kMaxGroups = 1024;
+
+// Inclusive sum over the 64 lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v, o, 64);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
+
+// Rows [first, end) of group g; ends past `rows` count as `rows`.
+__device__ __forceinline__ int group_edge(const int32_t* offsets, int g, int rows) {
+    const int o = offsets[g];
+    return o < 0 ? 0 : o < rows ? o : rows;
+}
+
+struct GroupTile {
+    int group, first, end;      // rows [first, end) of the group, of which the tile has the first `height`
+};
+
+// Tile number `index` of the groups' rows cut into tiles of `height` rows
+// (a group's last one may be shorter; empty groups have none).  Every lane of
+// the wave gets the same answer; group -1 behind the last tile.  Two steps of
+// a sum over lanes: runs of groups, then the groups of one run.
+__device__ __forceinline__ GroupTile find_tile(const int32_t* offsets, int groups, int rows, int height, int index) {
+    const int lane = threadIdx.x & 63, run = (groups + 63) >> 6;
+    int tiles = 0;
+    int edge = lane * run < groups ? group_edge(offsets, lane * run, rows) : 0;
+    const int first_edge = edge;
+    for (int i = 0; i < run; ++i) {
+        const int g = lane * run + i;
+        if (g < groups) {
+            const int next = group_edge(offsets, g + 1, rows);
+            if (next > edge) tiles += (next - edge + height - 1) / height;
+            edge = next;
+        }
+    }
+    const int sum = wave_scan(tiles);
+    const unsigned long long past = __ballot(sum > index);
+    if (!past) return GroupTile{-1, 0, 0};
+    const int l = __builtin_ctzll(past);
+    int rest = index - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l));
+    if (run == 1) return GroupTile{l, __builtin_amdgcn_readlane(first_edge, l) + rest * height, __builtin_amdgcn_readlane(edge, l)};
+    const int g = l * run + lane;
+    const bool mine = lane < run && g < groups;
+    const int lo = mine ? group_edge(offsets, g, rows) : 0, hi = mine ? group_edge(offsets, g + 1, rows) : 0;
+    const int own = hi > lo ? (hi - lo + height - 1) / height : 0, upto = wave_scan(own);
+    const int k = __builtin_ctzll(__ballot(upto > rest));
+    rest -= __builtin_amdgcn_readlane(upto, k) - __builtin_amdgcn_readlane(own, k);
+    return GroupTile{l * run + k, __builtin_amdgcn_readlane(lo, k) + rest * height, __builtin_amdgcn_readlane(hi, k)};
+}
+
+// starts[g] = tiles of `height` rows of the groups before g, for g <= groups
+// (LDS; one wave).
+__device__ __forceinline__ void group_starts(const int32_t* offsets, int groups, int rows, int height, int* starts) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int g0 = 0; g0 < groups; g0 += 64) {
+        const int g = g0 + lane;
+        const int lo = g < groups ? group_edge(offsets, g, rows) : 0, hi = g < groups ? group_edge(offsets, g + 1, rows) : 0;
+        const int own = hi > lo ? (hi - lo + height - 1) / height : 0, upto = wave_scan(own);
+        if (g < groups) starts[g] = before + upto - own;
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (lane == 0) starts[groups] = before;
+}
+
+// At most so many tiles of `height` rows, wherever the groups' edges lie.
+inline int64_t most_tiles(int64_t rows, int64_t groups, int64_t height) {
+    return rows / height + (rows < groups ? rows : groups);
+}
+
+}  // namespace icq

@@ -6,14 +6,23 @@
 //   4-bit floating point, accumulated in fp32.
 // The weights are the matrix instructions' first operand, so a lane ends
 // with four consecutive outputs of one row of y.
+//
+// Two further modes of the integer kinds:
+//   grouped   rows of y are ordered by group, each group has a weight of its
+//             own, and row i of y may come from another row of x;
+//   adapted   y[m, n] += sum_r t[m, r] B_a[n, r], a the adapter of row m and
+//             t = scale_a A_a x in fp32 (adapters.hip).
 #include "common.hpp"
 #include "prof.hpp"
 #include "lowbit.hpp"
+#include "adapters.hpp"
+#include "groups.hpp"
 
 namespace icq {
 namespace {
 
 enum Kind { kInt8 = 0, kInt4 = 1, kMx = 2 };
+enum Mode { kPlain, kGrouped, kAdapted };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -36,7 +45,22 @@ struct Operands {
     int out_dtype;
     int64_t ld_out;
     int wide;                // rows of out are 16-byte aligned and whole groups of 8 values
+    // kGrouped: w, sw, zp and bias are those of all groups, one after another
+    const int32_t* offsets;  // [groups + 1]
+    const int32_t* order;    // [M], where top > 0: row i of y is of row order[i] / top of the activations
+    int groups, top;
+    int a_rows;              // rows of the activations
+    int64_t w_group;         // bytes of a group's tiles
+    Adapted ad;              // kAdapted
 };
+
+// The row of activations that row m of y comes from.
+template <int MODE>
+__device__ __forceinline__ int source_row(const Operands& p, int m) {
+    if (MODE != kGrouped || !p.top) return m;
+    const int s = (int)((unsigned)p.order[m] / (unsigned)p.top);
+    return s < p.a_rows ? s : p.a_rows - 1;
+}
 
 template <int KIND> struct Acc { typedef i32x4 T; };
 template <> struct Acc<kMx> { typedef lb_f32x4 T; };
@@ -47,10 +71,10 @@ template <int KIND>
 struct Columns {
     float sw[4], bias[4];
     int zp[4];
-    __device__ __forceinline__ void load(const Operands& p, int64_t n0) {
+    __device__ __forceinline__ void load(const Operands& p, int64_t n0, int64_t first = 0) {    // (first: a group's columns)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int64_t n = n0 + i < p.N ? n0 + i : p.N - 1;
+            const int64_t n = first + (n0 + i < p.N ? n0 + i : p.N - 1);
             if (KIND != kMx) {
                 sw[i] = p.sw_f32 ? static_cast<const float*>(p.sw)[n] : f16_bits_to_f32(static_cast<const uint16_t*>(p.sw)[n]);
                 zp[i] = p.zp ? p.zp[n] : 0;
@@ -77,8 +101,8 @@ struct Columns {
 };
 
 // Four consecutive outputs of row m from column n.
-__device__ __forceinline__ void store4(const Operands& p, lb_f32x4 v, int64_t m, int64_t n) {
-    if (m >= p.M || n >= p.N) return;
+__device__ __forceinline__ void store4(const Operands& p, lb_f32x4 v, int64_t m, int64_t n, int64_t end) {
+    if (m >= end || n >= p.N) return;
     const int64_t at = m * p.ld_out + n;
     if (p.wide && n + 4 <= p.N) {
         if (p.out_dtype == IC_DTYPE_F32)
@@ -144,13 +168,22 @@ __device__ __forceinline__ lb_u32x4 to_operand(lb_u32x4 v, int from) {
 // (4.8 TB/s), 8.3 us from HBM (3.0 TB/s, many weights in turn); MXFP4 8 x 4096 x
 // 12288 6.1, 5.6 and 11.4 us.  More rows are bound by their activations, which
 // every work-group reads and exchanges again: INT8 333 x 1000 x 2901 10.8 us.
-template <int KIND, int MT>
+template <int KIND, int MT, int MODE = kPlain>
 __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
     typedef typename Acc<KIND>::T acc_t;
     constexpr int WAVES = 8;
     __shared__ acc_t part[WAVES][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-    const int64_t nt = blockIdx.x, mt0 = (int64_t)blockIdx.y * MT;
+    const int64_t nt = blockIdx.x;
+    int64_t mt0 = (int64_t)blockIdx.y * MT, m0 = mt0 * 16, m_end = p.M, column0 = 0;
+    if constexpr (MODE == kGrouped) {
+        const GroupTile tile = find_tile(p.offsets, p.groups, (int)p.M, 16 * MT, blockIdx.y);
+        if (tile.group < 0) return;
+        m0 = tile.first;
+        m_end = tile.end;
+        column0 = tile.group * p.N;
+        p.w += tile.group * p.w_group;
+    }
     const int64_t tiles = cdiv(p.K, 128), words = cdiv(p.K, 512);
     const int64_t t0 = tiles * wave / WAVES, t1 = tiles * (wave + 1) / WAVES;
     const lb_u32x4* wt = reinterpret_cast<const lb_u32x4*>(p.w) + nt * tiles * (KIND == kInt8 ? 128 : 64) + lane;
@@ -167,8 +200,8 @@ __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
             xt[i] = reinterpret_cast<const lb_u32x4*>(p.a) + mt * tiles * 64 + lane;
             xs[i] = p.a_scale + mt * words * 64 + lane;
         } else {
-            const int64_t m = (mt0 + i) * 16 + (lane >> 2) < p.M ? (mt0 + i) * 16 + (lane >> 2) : p.M - 1;
-            row[i] = p.a + m * p.ld_a + (lane & 3) * 16;
+            const int64_t m = m0 + i * 16 + (lane >> 2) < m_end ? m0 + i * 16 + (lane >> 2) : m_end - 1;
+            row[i] = p.a + source_row<MODE>(p, (int)m) * p.ld_a + (lane & 3) * 16;
         }
     }
     const uint32_t* ws = KIND == kMx ? p.w_scale + nt * words * 64 + lane : nullptr;
@@ -202,14 +235,15 @@ __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
     for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
     Columns<KIND> cols;
-    cols.load(p, nt * 16 + g * 4);
+    cols.load(p, nt * 16 + g * 4, column0);
     for (int i = wave; i < MT; i += WAVES) {
         acc_t s = part[0][i][lane];
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) s += part[k][i][lane];
-        const int64_t m = (mt0 + i) * 16 + r < p.M ? (mt0 + i) * 16 + r : p.M - 1;
-        store4(p, cols.finish(s, KIND == kMx ? 1.0f : p.sa[m], KIND != kMx && p.zp ? p.sums[m] : 0), (mt0 + i) * 16 + r,
-               nt * 16 + g * 4);
+        const int64_t m = m0 + i * 16 + r < m_end ? m0 + i * 16 + r : m_end - 1, from = source_row<MODE>(p, (int)m);
+        lb_f32x4 y = cols.finish(s, KIND == kMx ? 1.0f : p.sa[from], KIND != kMx && p.zp ? p.sums[from] : 0);
+        if constexpr (MODE == kAdapted) y += adapter_dot4(p.ad, p.N, m, nt * 16 + g * 4);
+        store4(p, y, m0 + i * 16 + r, nt * 16 + g * 4, m_end);
     }
 }
 
@@ -250,7 +284,7 @@ __device__ __forceinline__ void meet() {
 // start and end, none in the K loop.  Spills are vector-memory operations like
 // those that meet() counts.  It lets the newest N stay outstanding; with spills
 // among these it waits for more copies than it needs, never for fewer.
-template <int KIND, int WM, int WN, int FM, int FN, int BUF>
+template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE = kPlain>
 __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
     typedef typename Acc32<KIND>::T acc_t;
     constexpr int WAVES = WM * WN, BM = 32 * WM * FM, BN = 32 * WN * FN;
@@ -264,13 +298,21 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
     constexpr int STORES = FM * 4;                                                // a lane's stores of a whole 16-bit tile
     // one array for all of it: the compiler guards reads of a second one with waits for every copy in flight.
     // BUF stages; two sets of scale words; a column's bias, scale and zero-point; a row's scale and code sum
-    constexpr int SCALES = BUF * STAGE, COLS = SCALES + 2 * S_WORDS, ROWS = COLS + BN * 3 / 4;
-    __shared__ lb_u32x4 lds[ROWS + (KIND == kMx ? 0 : BM / 2)];
+    // (and a group's first row of tiles)
+    constexpr int SCALES = BUF * STAGE, COLS = SCALES + 2 * S_WORDS, ROWS = COLS + BN * 3 / 4, GROUPS = ROWS + (KIND == kMx ? 0 : BM / 2);
+    __shared__ lb_u32x4 lds[GROUPS + (MODE == kGrouped ? kMaxGroups / 4 + 1 : 0)];
     float* const col = reinterpret_cast<float*>(lds + COLS);
     float* const row = reinterpret_cast<float*>(lds + ROWS);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, r = lane & 31;
     const int wm = wave / WN, wn = wave % WN;
     const int lane16 = lane * 16;
+
+    int* const starts = reinterpret_cast<int*>(lds + GROUPS);
+    if constexpr (MODE == kGrouped) {
+        if (wave == 0) group_starts(p.offsets, p.groups, (int)p.M, BM, starts);
+        __syncthreads();
+        grid_m = __builtin_amdgcn_readfirstlane(starts[p.groups]);
+    }
 
     // work-groups are dealt to the 8 XCDs in turn: each XCD gets one run of tiles, walked in bands of 8 tile rows so
     // that what its L2 holds is used again
@@ -287,18 +329,41 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
 
     // ---- copies.  Rows and tiles past the last repeat the last; their outputs are dropped.
     int bm = 0, bn = 0;
+    int group = 0, row0 = 0, row_end = (int)p.M;           // the tile's first row, and the end of the rows it may have
     __amdgpu_buffer_rsrc_t x_buf, w_buf, xs_buf, ws_buf;
     int x_row[KIND == kMx ? X_LOADS : 1], w_row[W_LOADS], x_off[KIND == kMx ? 1 : X_LOADS], s_off[S_LOADS + 1];
-    auto buffer = [](const void* base) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
+    auto buffer = [](const void* base, int bytes = 0x7fffffff) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
     };
     auto aim = [&]() {
-        const int band = tile / (8 * grid_n), rows_in = grid_m - band * 8 < 8 ? grid_m - band * 8 : 8;
-        const int in_band = tile - band * 8 * grid_n;
+        int at = tile, rows_of = grid_m;                   // the tile's place among those of its group
+        if constexpr (MODE == kGrouped) {
+            // the last group that starts at or before the tile's row of tiles (empty groups start where the next one does)
+            const int tile_row = tile / grid_n;
+            int past = p.groups;
+            group = 0;
+            while (past - group > 1) {
+                const int mid = (group + past) >> 1;
+                if (starts[mid] <= tile_row) group = mid;
+                else past = mid;
+            }
+            group = __builtin_amdgcn_readfirstlane(group);
+            const int s0 = __builtin_amdgcn_readfirstlane(starts[group]);
+            rows_of = __builtin_amdgcn_readfirstlane(starts[group + 1]) - s0;
+            at -= s0 * grid_n;
+        }
+        const int band = at / (8 * grid_n), rows_in = rows_of - band * 8 < 8 ? rows_of - band * 8 : 8;
+        const int in_band = at - band * 8 * grid_n;
         bm = band * 8 + in_band % rows_in;
         bn = in_band / rows_in;
+        if constexpr (MODE == kGrouped) {
+            row0 = group_edge(p.offsets, group, (int)p.M) + bm * BM;
+            row_end = group_edge(p.offsets, group + 1, (int)p.M);
+        } else {
+            row0 = bm * BM;
+        }
         const int nt = bn * (BN / 16), nl = n_tiles - 1 - nt;
-        w_buf = buffer(p.w + (int64_t)nt * w_pitch);
+        w_buf = buffer(p.w + (MODE == kGrouped ? group * p.w_group : 0) + (int64_t)nt * w_pitch);
 #pragma unroll
         for (int i = 0; i < W_LOADS; ++i) w_row[i] = (i * WAVES + wave < nl ? i * WAVES + wave : nl) * w_pitch;
         if constexpr (KIND == kMx) {
@@ -317,15 +382,19 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
         } else {
             // INT4: 8 rows of 128 bytes a copy, chunk c of row r in slot c ^ (r >> 1 & 7); INT8: 16 rows of 64 bytes, chunk
             // c in slot c ^ (r >> 2 & 3).  16 lanes that read one chunk of 16 rows then touch all 64 banks once.
-            const int row0 = KIND == kInt4 ? lane >> 3 : lane >> 2;
+            const int lane_row = KIND == kInt4 ? lane >> 3 : lane >> 2;
             const int chunk = KIND == kInt4 ? (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4)) : (lane & 3) ^ (lane >> 4);
             static_assert(WAVES % 2 == 0, "a wave's copies begin at rows of one parity of 8");
-            const int ml = (int)p.M - 1 - bm * BM;
-            x_buf = buffer(p.a + (int64_t)bm * BM * p.ld_a);
+            const int ml = row_end - 1 - row0;
+            // (gathered rows lie anywhere in the activations, which have less than 2^32 bytes then)
+            if (MODE == kGrouped && p.top) x_buf = buffer(p.a, -1);
+            else x_buf = buffer(p.a + (int64_t)row0 * p.ld_a);
 #pragma unroll
             for (int i = 0; i < X_LOADS; ++i) {
-                const int row = (i * WAVES + wave) * (KIND == kInt4 ? 8 : 16) + row0;
-                x_off[i] = (row < ml ? row : ml) * (int)p.ld_a + chunk * 16;
+                int row = (i * WAVES + wave) * (KIND == kInt4 ? 8 : 16) + lane_row;
+                row = row < ml ? row : ml;
+                if (MODE == kGrouped && p.top) row = source_row<MODE>(p, row0 + row);
+                x_off[i] = (int)((unsigned)row * (unsigned)p.ld_a) + chunk * 16;
             }
         }
     };
@@ -358,6 +427,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
     // of 8 consecutive outputs.
     lb_u32x4 xv[2][FM], wv[2][FN];
     int xs[KIND == kMx ? FM : 1][2], ws[KIND == kMx ? FN : 1][2];
+    const int w_column = (r >> 4) * 16 + (r >> 2 & 1) * 8 + (r >> 3 & 1) * 4 + (r & 3);
     const int w_lane = (r >> 4) * 64 + h * 16 + (r >> 2 & 1) * 8 + (r >> 3 & 1) * 4 + (r & 3);
     auto read_x = [&](const lb_u32x4* s, lb_u32x4 (&to)[FM], int c) {
 #pragma unroll
@@ -389,7 +459,11 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
     auto start = [&]() {                                   // a tile's first copies
         aim();
         const int tid = threadIdx.x;
-        const int64_t n = bn * BN + tid < p.N ? bn * BN + tid : p.N - 1, m = bm * BM + tid < p.M ? bm * BM + tid : p.M - 1;
+        int64_t n = bn * BN + tid < p.N ? bn * BN + tid : p.N - 1, m = row0 + tid < row_end ? row0 + tid : row_end - 1;
+        if constexpr (MODE == kGrouped) {
+            n += group * p.N;
+            m = source_row<MODE>(p, (int)m);
+        }
         if (KIND != kMx) {
             c_scale = p.sw_f32 ? static_cast<const float*>(p.sw)[n] : f16_bits_to_f32(static_cast<const uint16_t*>(p.sw)[n]);
             r_scale = p.sa[m];
@@ -523,8 +597,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
         }
 
         // ---- outputs, after the next tile's first copies
-        const int m0 = bm * BM + wm * FM * 32, n0 = bn * BN + wn * FN * 32;
-        const bool whole = p.wide && p.out_dtype != IC_DTYPE_F32 && (bm + 1) * BM <= p.M && (bn + 1) * BN <= p.N;
+        const int m0 = row0 + wm * FM * 32, n0 = bn * BN + wn * FN * 32, m_end = row_end;
+        const bool whole = p.wide && p.out_dtype != IC_DTYPE_F32 && row0 + BM <= m_end && (bn + 1) * BN <= p.N;
         tile += gridDim.x >> 3;
         const bool more = tile < last;                     // (all waves are done with the buffers)
         // y from the accumulated sum: INT4 operands are held as 16 q, and the shift is exact.  |zp| <= 2^7 and
@@ -551,7 +625,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int m = m1 + i * 32 + k * 8, n = n0 + (chunk ^ (k & 1) * 4) * width;
-                    if (m >= p.M || n >= p.N) continue;
+                    if (m >= m_end || n >= p.N) continue;
                     if (p.out_dtype == IC_DTYPE_F32) *reinterpret_cast<lb_u32x4*>(static_cast<float*>(p.out) + m * p.ld_out + n) = v[k];
                     else *reinterpret_cast<lb_u32x4*>(static_cast<uint16_t*>(p.out) + m * p.ld_out + n) = v[k];
                 }
@@ -563,6 +637,8 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
                 const float sa = KIND == kMx ? 0.0f : row[rw + i * 32 + r], sum = KIND == kMx ? 0.0f : row[BM + rw + i * 32 + r];
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
+                    f32x16 added;
+                    if constexpr (MODE == kAdapted) added = adapter_block(p.ad, p.N, m0 + i * 32 + r < m_end ? m0 + i * 32 + r : m_end - 1, n0 + j * 32 + w_column, h);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         lb_f32x4 v[2];
@@ -576,7 +652,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
                                 zero = *reinterpret_cast<const lb_f32x4*>(col + 2 * BN + c);
                             }
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[k][e] = value(acc[i][j][8 * q + 4 * k + e], sw[e], zero[e], bias[e], sa, sum);
+                            for (int e = 0; e < 4; ++e) {
+                                v[k][e] = value(acc[i][j][8 * q + 4 * k + e], sw[e], zero[e], bias[e], sa, sum);
+                                if constexpr (MODE == kAdapted) v[k][e] += added[8 * q + 4 * k + e];
+                            }
                         }
                         if (p.out_dtype == IC_DTYPE_F32) {
                             area[r * 8 + ((q * 4 + h * 2) ^ (r >> 1 & 7))] = __builtin_bit_cast(lb_u32x4, v[0]);
@@ -607,22 +686,37 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
             sum_t* area = reinterpret_cast<sum_t*>(lds) + wave * 32 * PITCH;
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
+                if constexpr (MODE == kAdapted) {
+                    // whole values, in place of the sums
+                    const float sa = row[wm * FM * 32 + i * 32 + r], sum = row[BM + wm * FM * 32 + i * 32 + r];
 #pragma unroll
-                for (int j = 0; j < FN; ++j)
+                    for (int j = 0; j < FN; ++j) {
+                        const f32x16 added = adapter_block(p.ad, p.N, m0 + i * 32 + r < m_end ? m0 + i * 32 + r : m_end - 1, n0 + j * 32 + w_column, h);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        *reinterpret_cast<sum4_t*>(area + r * PITCH + j * 32 + (k >> 1) * 16 + h * 8 + (k & 1) * 4) =
-                            sum4_t{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+                        for (int k = 0; k < 16; ++k) {
+                            const int n = j * 32 + (k >> 3) * 16 + h * 8 + (k & 7), c = wn * FN * 32 + n;
+                            area[r * PITCH + n] = __builtin_bit_cast(sum_t, value(acc[i][j][k], col[BN + c], col[2 * BN + c], col[c], sa, sum) + added[k]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            *reinterpret_cast<sum4_t*>(area + r * PITCH + j * 32 + (k >> 1) * 16 + h * 8 + (k & 1) * 4) =
+                                sum4_t{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+                }
                 lds_wave_fence();
-                const int rows = (int)p.M - (m0 + i * 32) < 32 ? (int)p.M - (m0 + i * 32) : 32;
+                const int rows = m_end - (m0 + i * 32) < 32 ? m_end - (m0 + i * 32) : 32;
 #pragma unroll 4
                 for (int e = lane; e < rows * FN * 32; e += 64) {
                     const int m = e / (FN * 32), n = e % (FN * 32);
                     if (n0 + n >= p.N) continue;
                     const sum_t s = area[m * PITCH + n];
                     const int c = wn * FN * 32 + n, o = wm * FM * 32 + i * 32 + m;
-                    const float v = KIND == kMx ? value(s, 0.0f, 0.0f, col[c], 0.0f, 0.0f)
-                                                : value(s, col[BN + c], col[2 * BN + c], col[c], row[o], row[BM + o]);
+                    const float v = MODE == kAdapted ? __builtin_bit_cast(float, s)
+                                    : KIND == kMx    ? value(s, 0.0f, 0.0f, col[c], 0.0f, 0.0f)
+                                                     : value(s, col[BN + c], col[2 * BN + c], col[c], row[o], row[BM + o]);
                     store_from_f32(p.out, p.out_dtype, (m0 + i * 32 + m) * p.ld_out + n0 + n, v);
                 }
                 lds_wave_fence();
@@ -662,23 +756,24 @@ __global__ __launch_bounds__(256) void pack_weight_kernel(const uint8_t* __restr
     dst[((int64_t)blockIdx.y * tiles + t) * 64 + lane] = w;
 }
 
-template <int KIND, int MT>
+template <int KIND, int MT, int MODE>
 void launch_direct(const Operands& p, hipStream_t st) {
-    const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16 * MT));
-    hipLaunchKernelGGL((linear_direct_kernel<KIND, MT>), grid, dim3(512), 0, st, p);
+    const int64_t rows = MODE == kGrouped ? most_tiles(p.M, p.groups, 16 * MT) : cdiv(p.M, 16 * MT);
+    const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)rows);
+    hipLaunchKernelGGL((linear_direct_kernel<KIND, MT, MODE>), grid, dim3(512), 0, st, p);
 }
 
 // As many work-groups as run at once (one a CU with tiles of 256 x 256, whose
 // buffers take most of its LDS, two with 128 x 128), each of which walks its
 // XCD's tiles.  (INT4's 128 x 128 takes 260 registers, four too many for two a
 // CU: its second half starts as the first ends.)
-template <int KIND, int WM, int WN, int FM, int FN, int BUF>
+template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE>
 void launch_tiled(const Operands& p, hipStream_t st) {
-    const int gm = (int)cdiv(p.M, 32 * WM * FM), gn = (int)cdiv(p.N, 32 * WN * FN);
+    const int gm = (int)(MODE == kGrouped ? most_tiles(p.M, p.groups, 32 * WM * FM) : cdiv(p.M, 32 * WM * FM)), gn = (int)cdiv(p.N, 32 * WN * FN);
     const int64_t tiles = (int64_t)gm * gn;
     constexpr int64_t at_once = WM * WN == 4 ? 512 : 256;
     const unsigned grid = (unsigned)(tiles < at_once ? cdiv(tiles, 8) * 8 : at_once);
-    hipLaunchKernelGGL((linear_tiled_kernel<KIND, WM, WN, FM, FN, BUF>), dim3(grid), dim3(64 * WM * WN), 0, st, p, gm, gn);
+    hipLaunchKernelGGL((linear_tiled_kernel<KIND, WM, WN, FM, FN, BUF, MODE>), dim3(grid), dim3(64 * WM * WN), 0, st, p, gm, gn);
 }
 
 // Which form.  The direct one while it has few work-groups (of 64 rows x 16
@@ -712,14 +807,32 @@ int linear_form(int kind, int64_t M, int64_t N) {      // 0, 128 or 256
     return tiles * 12 >= rounds * 256 * (kind == kInt4 ? 8 : 9) ? 256 : 128;
 }
 
-template <int KIND>
+template <int KIND, int MODE = kPlain>
 int launch_linear(const Operands& p, hipStream_t st) {
     const int form = linear_form(KIND, p.M, p.N);
-    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4>(p, st);
-    else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4>(p, st);
-    else if (p.M <= 16) launch_direct<KIND, 1>(p, st);
-    else if (p.M <= 32) launch_direct<KIND, 2>(p, st);
-    else launch_direct<KIND, 4>(p, st);
+    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4, MODE>(p, st);
+    else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4, MODE>(p, st);
+    else if (p.M <= 16) launch_direct<KIND, 1, MODE>(p, st);
+    else if (p.M <= 32) launch_direct<KIND, 2, MODE>(p, st);
+    else launch_direct<KIND, 4, MODE>(p, st);
+    IC_CHECK_LAUNCH();
+    return IC_OK;
+}
+
+// Which form a grouped product takes, by the rows that a group has on average.
+int expert_form(int64_t rows, int64_t groups) {      // 16, 32 or 64 (rows directly from memory), 128 or 256
+    const int64_t each = cdiv(rows, groups);
+    return each <= 16 ? 16 : each <= 32 ? 32 : each <= 128 ? 64 : each <= 512 ? 128 : 256;
+}
+
+template <int KIND>
+int launch_experts(const Operands& p, hipStream_t st) {
+    const int form = expert_form(p.M, p.groups);
+    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4, kGrouped>(p, st);
+    else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4, kGrouped>(p, st);
+    else if (form == 64) launch_direct<KIND, 4, kGrouped>(p, st);
+    else if (form == 32) launch_direct<KIND, 2, kGrouped>(p, st);
+    else launch_direct<KIND, 1, kGrouped>(p, st);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
@@ -765,28 +878,90 @@ extern "C" int ic_linear_pack_weight(const void* stored, int bits, int64_t N, in
     return IC_OK;
 }
 
+namespace icq {
+namespace {
+
+// The operands of the integer kinds, checked.  Rows of y and of the activations differ where groups gather.
+int integer_product(const char* who, Operands& p, const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t M,
+                    const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias, int bias_dtype,
+                    int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out) {
+    const std::string w(who);
+    p.a = reinterpret_cast<const uint8_t*>(a); p.ld_a = ld_a; p.sa = sa; p.sums = sums;
+    p.w = static_cast<const uint8_t*>(tiles); p.sw = sw; p.sw_f32 = sw_kind; p.zp = zp;
+    p.bias = bias; p.bias_dtype = bias_dtype; p.M = M; p.N = N; p.K = K;
+    p.out = out; p.out_dtype = out_dtype; p.ld_out = ld_out;
+    if (const int rc = check_product(who, p)) return rc;
+    IC_REQUIRE(bits == 4 || bits == 8, w + ": bits must be 4 or 8");
+    IC_REQUIRE(sw_kind == 0 || sw_kind == 1, w + ": sw_kind must be 0 (fp16) or 1 (fp32)");
+    if (M == 0) return IC_OK;
+    IC_REQUIRE(a && sa && tiles && sw && out && (!zp || sums), w + ": null pointer");
+    IC_REQUIRE(ld_a >= cdiv(K, kActPad) * kActPad && ld_a % 16 == 0 && aligned16(a) && aligned16(tiles),
+               w + ": activations need rows of ic_activation_pitch codes, 16-byte aligned");
+    IC_REQUIRE(ld_out >= N, w + ": ld_out below N");
+    if (ld_a > (1 << 20)) return fail(IC_ERR_RANGE, w + ": at most 2^20 for ld_a");   // (a lane's 32-bit offset in 256 rows)
+    p.wide = aligned16(out) && ld_out % (out_dtype == IC_DTYPE_F32 ? 4 : 8) == 0 && N % 8 == 0;
+    return IC_OK;
+}
+
+}  // namespace
+}  // namespace icq
+
 extern "C" int ic_quantized_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t M,
                                    const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp,
                                    const void* bias, int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype,
                                    int64_t ld_out, void* stream) {
     Operands p{};
-    p.a = reinterpret_cast<const uint8_t*>(a); p.ld_a = ld_a; p.sa = sa; p.sums = sums;
-    p.w = static_cast<const uint8_t*>(tiles); p.sw = sw; p.sw_f32 = sw_kind; p.zp = zp;
-    p.bias = bias; p.bias_dtype = bias_dtype; p.M = M; p.N = N; p.K = K;
-    p.out = out; p.out_dtype = out_dtype; p.ld_out = ld_out;
-    if (const int rc = check_product("ic_quantized_linear", p)) return rc;
-    IC_REQUIRE(bits == 4 || bits == 8, "ic_quantized_linear: bits must be 4 or 8");
-    IC_REQUIRE(sw_kind == 0 || sw_kind == 1, "ic_quantized_linear: sw_kind must be 0 (fp16) or 1 (fp32)");
+    if (const int rc = integer_product("ic_quantized_linear", p, a, ld_a, sa, sums, M, tiles, bits, sw, sw_kind, zp, bias, bias_dtype, N,
+                                       K, out, out_dtype, ld_out)) return rc;
     if (M == 0) return IC_OK;
-    IC_REQUIRE(a && sa && tiles && sw && out && (!zp || sums), "ic_quantized_linear: null pointer");
-    IC_REQUIRE(ld_a >= cdiv(K, kActPad) * kActPad && ld_a % 16 == 0 && aligned16(a) && aligned16(tiles),
-               "ic_quantized_linear: activations need rows of ic_activation_pitch codes, 16-byte aligned");
-    IC_REQUIRE(ld_out >= N, "ic_quantized_linear: ld_out below N");
-    if (ld_a > (1 << 20)) return fail(IC_ERR_RANGE, "ic_quantized_linear: at most 2^20 for ld_a");   // (a lane's 32-bit offset in 256 rows)
-    p.wide = aligned16(out) && ld_out % (out_dtype == IC_DTYPE_F32 ? 4 : 8) == 0 && N % 8 == 0;
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 2.0 * M * N * K, (double)M * K + (double)N * K * bits / 8);
     return bits == 8 ? launch_linear<kInt8>(p, st) : launch_linear<kInt4>(p, st);
+}
+
+extern "C" int ic_expert_form(int64_t rows, int64_t groups) {
+    IC_REQUIRE(rows >= 0 && groups >= 1, "ic_expert_form: rows must be >= 0, groups >= 1");
+    return expert_form(rows, groups);
+}
+
+extern "C" int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t a_rows,
+                                const int32_t* offsets, const int32_t* order, int top, int64_t groups, int64_t rows,
+                                const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,
+                                int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out, void* stream) {
+    Operands p{};
+    if (const int rc = integer_product("ic_expert_linear", p, a, ld_a, sa, sums, rows, tiles, bits, sw, sw_kind, zp, bias, bias_dtype, N,
+                                       K, out, out_dtype, ld_out)) return rc;
+    IC_REQUIRE(groups >= 1 && groups <= kMaxGroups, "ic_expert_linear: 1 to 1024 groups");
+    if (rows == 0) return IC_OK;
+    IC_REQUIRE(top >= 0 && offsets && (top == 0 || order), "ic_expert_linear: gathered rows need their order");
+    IC_REQUIRE(top > 0 ? a_rows >= 1 && a_rows <= kMaxRows : a_rows == rows,
+               "ic_expert_linear: rows of activations and of the result differ, and none are gathered");
+    if (top > 0 && a_rows * ld_a > 0xffffffffll) return fail(IC_ERR_RANGE, "ic_expert_linear: gathered activations have less than 2^32 bytes");
+    p.offsets = offsets; p.order = order; p.top = top; p.groups = (int)groups; p.a_rows = (int)a_rows;
+    p.w_group = ic_linear_weight_bytes(N, K, bits);
+    hipStream_t st = as_stream(stream);
+    ProfScope prof(st, PT_OTHER, 2.0 * rows * N * K, (double)a_rows * K + (double)groups * N * K * bits / 8);
+    return bits == 8 ? launch_experts<kInt8>(p, st) : launch_experts<kInt4>(p, st);
+}
+
+extern "C" int ic_adapted_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t M,
+                                 const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,
+                                 int bias_dtype, int64_t N, int64_t K, const void* down, const void* up, int adapter_dtype,
+                                 int64_t adapters, int rank, const float* scaling, const int32_t* ids, const int32_t* offsets,
+                                 const int32_t* order, void* workspace, void* out, int out_dtype, int64_t ld_out, void* stream) {
+    Operands p{};
+    if (const int rc = integer_product("ic_adapted_linear", p, a, ld_a, sa, sums, M, tiles, bits, sw, sw_kind, zp, bias, bias_dtype, N, K,
+                                       out, out_dtype, ld_out)) return rc;
+    IC_REQUIRE(adapter_dtype == IC_DTYPE_BF16 || adapter_dtype == IC_DTYPE_F16, "ic_adapted_linear: adapters are bf16 or fp16");
+    IC_REQUIRE(adapters >= 1 && adapters <= kMaxGroups && rank >= 1 && rank <= kMaxRank, "ic_adapted_linear: 1 to 1024 adapters of rank 1 to 128");
+    if (M == 0) return IC_OK;
+    IC_REQUIRE(down && up && scaling && ids && offsets && order && workspace, "ic_adapted_linear: null pointer");
+    IC_REQUIRE(aligned16(down) && aligned16(up) && aligned16(workspace), "ic_adapted_linear: adapters and workspace need 16-byte alignment");
+    hipStream_t st = as_stream(stream);
+    ProfScope prof(st, PT_OTHER, 2.0 * M * N * K + 2.0 * M * rank * (N + K), (double)M * K + (double)N * K * bits / 8);
+    p.ad = Adapted{ids, static_cast<float*>(workspace), static_cast<const uint16_t*>(up), adapter_dtype == IC_DTYPE_F16, padded_rank(rank), (int)adapters};
+    if (const int rc = launch_shrink(p.ad, a, ld_a, sa, M, K, down, rank, scaling, offsets, order, st)) return rc;
+    return bits == 8 ? launch_linear<kInt8, kAdapted>(p, st) : launch_linear<kInt4, kAdapted>(p, st);
 }
 
 extern "C" int ic_mxfp4_linear(const void* a, const void* a_scales, int64_t M, const void* w, const void* w_scales,

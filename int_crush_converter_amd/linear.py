@@ -4,7 +4,8 @@ scale, and where asymmetric a zero-point, a row:
 
     y[m, n] = sa[m] sw[n] (sum_k a q - zp[n] sum_k a) + b[n]
 
-The sums are exact in 32-bit integers (int8 matrix instructions)."""
+The sums are exact in 32-bit integers (int8 matrix instructions).  Beside the
+shared weight each row may add a low-rank adapter of its own (``adapters.py``)."""
 
 from __future__ import annotations
 
@@ -13,6 +14,8 @@ import torch
 from . import _native as nat
 from . import packing
 from .activations import MAX_FEATURES, QuantizedActivations, as_rows, call
+from .adapters import LowRankAdapters
+from .groups import RowGroups
 
 MAX_ROWS = 1048560
 
@@ -90,17 +93,41 @@ class QuantizedWeight:
 
 
 def quantized_linear(x: QuantizedActivations, weight: QuantizedWeight, bias: torch.Tensor | None = None, *,
+                     adapters: LowRankAdapters | None = None, groups: RowGroups | None = None,
                      out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """y [*lead, out_features] in ``out_dtype``.  Rows of x whose scale is NaN give rows of NaN."""
+    """y [*lead, out_features] in ``out_dtype``.  Rows of x whose scale is NaN give rows of NaN.
+
+    adapters, groups: each row adds the low-rank adapter of its own request; ``groups`` is ``group_rows`` of the rows'
+    adapter numbers (one a row, -1 for none), made once for a batch and used with all its layers."""
     if x.in_features != weight.in_features:
         raise ValueError(f"activations have {x.in_features} features, the weight {weight.in_features}")
     data, N, w, z = x.data, weight.out_features, weight, weight.zero_points
     code = _out_code(out_dtype)
     b, bcode = _bias(bias, N)
     stream = nat.stream_for(data, x.meta, w.tiles, w.scales, z)
-    out = torch.empty((*x.lead, N), dtype=out_dtype, device=data.device)
     rows, m = data.shape[0], x.meta.data_ptr()
-    call("ic_quantized_linear", data.data_ptr(), data.shape[1], m, m + 4 * rows, rows, w.tiles.data_ptr(), w.bits,
+    if adapters is None:
+        if groups is not None:
+            raise ValueError("groups are those of adapters' rows: expert_linear is the product with a weight a group")
+        out = torch.empty((*x.lead, N), dtype=out_dtype, device=data.device)
+        call("ic_quantized_linear", data.data_ptr(), data.shape[1], m, m + 4 * rows, rows, w.tiles.data_ptr(), w.bits,
+             w.scales.data_ptr(), w.scale_kind, None if z is None else z.data_ptr(), None if b is None else b.data_ptr(),
+             bcode, N, w.in_features, out.data_ptr(), code, N, stream)
+        return out
+    ad = adapters
+    if (ad.in_features, ad.out_features) != (w.in_features, N):
+        raise ValueError(f"adapters are {ad.out_features} x {ad.in_features}, the weight {N} x {w.in_features}")
+    if groups is None:
+        raise ValueError("adapters need the rows' groups: group_rows(ids, adapters.count)")
+    if (groups.rows, groups.per_row, groups.groups) != (rows, 1, ad.count):
+        raise ValueError(f"groups are of {groups.rows} rows with {groups.per_row} choices among {groups.groups}, expected "
+                         f"{rows} rows with one among {ad.count} adapters")
+    nat.stream_for(ad.down, ad.up, ad.scaling, groups.data)
+    out = torch.empty((*x.lead, N), dtype=out_dtype, device=data.device)
+    ws = torch.empty((rows, -(-ad.rank // 16) * 16), dtype=torch.float32, device=data.device)
+    ids, offsets, order, _ = groups.pointers()
+    call("ic_adapted_linear", data.data_ptr(), data.shape[1], m, m + 4 * rows, rows, w.tiles.data_ptr(), w.bits,
          w.scales.data_ptr(), w.scale_kind, None if z is None else z.data_ptr(), None if b is None else b.data_ptr(),
-         bcode, N, w.in_features, out.data_ptr(), code, N, stream)
+         bcode, N, w.in_features, ad.down.data_ptr(), ad.up.data_ptr(), ad.code, ad.count, ad.rank,
+         ad.scaling.data_ptr(), ids, offsets, order, ws.data_ptr(), out.data_ptr(), code, N, stream)
     return out
