@@ -561,9 +561,9 @@ int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32
                      const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,
                      int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out, void* stream);
 
-/* Which form ic_expert_linear takes for these sizes: 16, 32 or 64 (rows
- * directly from memory, so many at a time), 128 or 256 (tiles). */
-int ic_expert_form(int64_t rows, int64_t groups);
+/* Which form ic_expert_linear takes for these sizes: 16 (16 rows at a time,
+ * directly from memory), or tiles of 32, 64, 128 or 256 rows. */
+int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N);
 
 /* Low-rank adapters, bf16 or fp16: a [adapters, rank, K] and b [adapters, N,
  * rank], contiguous, laid out once for ic_adapted_linear (ic_adapter_down_bytes

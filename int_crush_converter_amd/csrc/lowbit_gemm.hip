@@ -168,22 +168,13 @@ __device__ __forceinline__ lb_u32x4 to_operand(lb_u32x4 v, int from) {
 // (4.8 TB/s), 8.3 us from HBM (3.0 TB/s, many weights in turn); MXFP4 8 x 4096 x
 // 12288 6.1, 5.6 and 11.4 us.  More rows are bound by their activations, which
 // every work-group reads and exchanges again: INT8 333 x 1000 x 2901 10.8 us.
-template <int KIND, int MT, int MODE = kPlain>
+template <int KIND, int MT>
 __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
     typedef typename Acc<KIND>::T acc_t;
     constexpr int WAVES = 8;
     __shared__ acc_t part[WAVES][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-    const int64_t nt = blockIdx.x;
-    int64_t mt0 = (int64_t)blockIdx.y * MT, m0 = mt0 * 16, m_end = p.M, column0 = 0;
-    if constexpr (MODE == kGrouped) {
-        const GroupTile tile = find_tile(p.offsets, p.groups, (int)p.M, 16 * MT, blockIdx.y);
-        if (tile.group < 0) return;
-        m0 = tile.first;
-        m_end = tile.end;
-        column0 = tile.group * p.N;
-        p.w += tile.group * p.w_group;
-    }
+    const int64_t nt = blockIdx.x, mt0 = (int64_t)blockIdx.y * MT;
     const int64_t tiles = cdiv(p.K, 128), words = cdiv(p.K, 512);
     const int64_t t0 = tiles * wave / WAVES, t1 = tiles * (wave + 1) / WAVES;
     const lb_u32x4* wt = reinterpret_cast<const lb_u32x4*>(p.w) + nt * tiles * (KIND == kInt8 ? 128 : 64) + lane;
@@ -200,8 +191,8 @@ __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
             xt[i] = reinterpret_cast<const lb_u32x4*>(p.a) + mt * tiles * 64 + lane;
             xs[i] = p.a_scale + mt * words * 64 + lane;
         } else {
-            const int64_t m = m0 + i * 16 + (lane >> 2) < m_end ? m0 + i * 16 + (lane >> 2) : m_end - 1;
-            row[i] = p.a + source_row<MODE>(p, (int)m) * p.ld_a + (lane & 3) * 16;
+            const int64_t m = (mt0 + i) * 16 + (lane >> 2) < p.M ? (mt0 + i) * 16 + (lane >> 2) : p.M - 1;
+            row[i] = p.a + m * p.ld_a + (lane & 3) * 16;
         }
     }
     const uint32_t* ws = KIND == kMx ? p.w_scale + nt * words * 64 + lane : nullptr;
@@ -235,15 +226,110 @@ __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
     for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
     Columns<KIND> cols;
-    cols.load(p, nt * 16 + g * 4, column0);
+    cols.load(p, nt * 16 + g * 4);
     for (int i = wave; i < MT; i += WAVES) {
         acc_t s = part[0][i][lane];
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) s += part[k][i][lane];
-        const int64_t m = m0 + i * 16 + r < m_end ? m0 + i * 16 + r : m_end - 1, from = source_row<MODE>(p, (int)m);
-        lb_f32x4 y = cols.finish(s, KIND == kMx ? 1.0f : p.sa[from], KIND != kMx && p.zp ? p.sums[from] : 0);
-        if constexpr (MODE == kAdapted) y += adapter_dot4(p.ad, p.N, m, nt * 16 + g * 4);
-        store4(p, y, m0 + i * 16 + r, nt * 16 + g * 4, m_end);
+        const int64_t m = (mt0 + i) * 16 + r < p.M ? (mt0 + i) * 16 + r : p.M - 1;
+        store4(p, cols.finish(s, KIND == kMx ? 1.0f : p.sa[m], KIND != kMx && p.zp ? p.sums[m] : 0), (mt0 + i) * 16 + r,
+               nt * 16 + g * 4, p.M);
+    }
+}
+
+// The same for grouped and adapted products: a work-group of 8 waves takes 16 NT
+// columns and 16 MT rows, its waves a share of K each, so that activations that
+// have been loaded and exchanged serve NT tiles of weights.  The next step's
+// loads are on their way during a step's products.  Sums are integers: waves
+// add theirs in LDS in any order.
+template <int KIND, int MT, int NT, int MODE>
+__global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
+    constexpr int WAVES = 8, W = KIND == kInt8 ? 2 : 1;
+    static_assert(KIND != kMx && MODE != kPlain, "integer kinds");
+    __shared__ int sum[MT * NT][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    const int n_tiles = (int)cdiv(p.N, 16), nt0 = (int)blockIdx.x * NT;
+    int m0 = (int)blockIdx.y * 16 * MT, m_end = (int)p.M;
+    int64_t column0 = 0;
+    const uint8_t* weight = p.w;
+    if constexpr (MODE == kGrouped) {
+        const GroupTile tile = find_tile(p.offsets, p.groups, (int)p.M, 16 * MT, blockIdx.y);
+        if (tile.group < 0) return;
+        m0 = tile.first;
+        m_end = tile.end;
+        column0 = tile.group * p.N;
+        weight += tile.group * p.w_group;
+    }
+    const int tiles = (int)cdiv(p.K, 128), t0 = tiles * wave / WAVES, t1 = tiles * (wave + 1) / WAVES;
+    const lb_u32x4* wt[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)       // (tiles past the last repeat the last; their outputs are dropped)
+        wt[j] = reinterpret_cast<const lb_u32x4*>(weight) + (int64_t)(nt0 + j < n_tiles ? nt0 + j : n_tiles - 1) * tiles * (64 * W) + lane;
+    const lb_u32x4* row[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int m = m0 + i * 16 + (lane >> 2) < m_end ? m0 + i * 16 + (lane >> 2) : m_end - 1;
+        row[i] = reinterpret_cast<const lb_u32x4*>(p.a + source_row<MODE>(p, m) * p.ld_a) + (lane & 3);
+    }
+    i32x4 acc[MT][NT];
+    lb_u32x4 w[NT][W], x[MT][2];
+    auto load = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[j][k] = wt[j][(t * W + k) * 64];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            x[i][0] = row[i][t * 8];
+            x[i][1] = row[i][t * 8 + 4];
+        }
+    };
+    if (t0 < t1) load(t0);
+    for (int k = threadIdx.x; k < MT * NT * 256; k += 64 * WAVES) (&sum[0][0][0])[k] = 0;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        lb_u32x4 now[NT][W], to[MT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int k = 0; k < W; ++k) now[j][k] = w[j][k];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            to[i][0] = x[i][0];
+            to[i][1] = x[i][1];
+        }
+        if (t + 1 < t1) load(t + 1);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const lb_u32x4 x0 = to_operand(to[i][0], r * 4 + g), x1 = to_operand(to[i][1], r * 4 + g);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                acc[i][j] = mma_i8(KIND == kInt8 ? now[j][0] : low_nibbles(now[j][0]), x0, acc[i][j]);
+                acc[i][j] = mma_i8(KIND == kInt8 ? now[j][W - 1] : high_nibbles(now[j][0]), x1, acc[i][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) atomicAdd(&sum[i * NT + j][k][lane], acc[i][j][k]);
+    __syncthreads();
+    for (int u = wave; u < MT * NT; u += WAVES) {
+        const int i = u / NT, j = u % NT, m = m0 + i * 16 + r, n = (nt0 + j) * 16 + g * 4;
+        if (m >= m_end || n >= p.N) continue;
+        Columns<KIND> cols;
+        cols.load(p, n, column0);
+        const int from = source_row<MODE>(p, m);
+        const i32x4 s = {sum[u][0][lane], sum[u][1][lane], sum[u][2][lane], sum[u][3][lane]};
+        lb_f32x4 y = cols.finish(s, p.sa[from], p.zp ? p.sums[from] : 0);
+        if constexpr (MODE == kAdapted) y += adapter_dot4(p.ad, p.N, m, n);
+        store4(p, y, m, n, m_end);
     }
 }
 
@@ -756,11 +842,16 @@ __global__ __launch_bounds__(256) void pack_weight_kernel(const uint8_t* __restr
     dst[((int64_t)blockIdx.y * tiles + t) * 64 + lane] = w;
 }
 
-template <int KIND, int MT, int MODE>
+template <int KIND, int MT>
 void launch_direct(const Operands& p, hipStream_t st) {
+    const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)cdiv(p.M, 16 * MT));
+    hipLaunchKernelGGL((linear_direct_kernel<KIND, MT>), grid, dim3(512), 0, st, p);
+}
+
+template <int KIND, int MT, int NT, int MODE>
+void launch_wide(const Operands& p, hipStream_t st) {
     const int64_t rows = MODE == kGrouped ? most_tiles(p.M, p.groups, 16 * MT) : cdiv(p.M, 16 * MT);
-    const dim3 grid((unsigned)cdiv(p.N, 16), (unsigned)rows);
-    hipLaunchKernelGGL((linear_direct_kernel<KIND, MT, MODE>), grid, dim3(512), 0, st, p);
+    hipLaunchKernelGGL((linear_wide_kernel<KIND, MT, NT, MODE>), dim3((unsigned)cdiv(p.N, 16 * NT), (unsigned)rows), dim3(512), 0, st, p);
 }
 
 // As many work-groups as run at once (one a CU with tiles of 256 x 256, whose
@@ -771,7 +862,7 @@ template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE>
 void launch_tiled(const Operands& p, hipStream_t st) {
     const int gm = (int)(MODE == kGrouped ? most_tiles(p.M, p.groups, 32 * WM * FM) : cdiv(p.M, 32 * WM * FM)), gn = (int)cdiv(p.N, 32 * WN * FN);
     const int64_t tiles = (int64_t)gm * gn;
-    constexpr int64_t at_once = WM * WN == 4 ? 512 : 256;
+    constexpr int64_t at_once = WM * WN == 8 ? 256 : WM * WN == 4 ? 512 : 1024;
     const unsigned grid = (unsigned)(tiles < at_once ? cdiv(tiles, 8) * 8 : at_once);
     hipLaunchKernelGGL((linear_tiled_kernel<KIND, WM, WN, FM, FN, BUF, MODE>), dim3(grid), dim3(64 * WM * WN), 0, st, p, gm, gn);
 }
@@ -812,27 +903,64 @@ int launch_linear(const Operands& p, hipStream_t st) {
     const int form = linear_form(KIND, p.M, p.N);
     if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4, MODE>(p, st);
     else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4, MODE>(p, st);
-    else if (p.M <= 16) launch_direct<KIND, 1, MODE>(p, st);
-    else if (p.M <= 32) launch_direct<KIND, 2, MODE>(p, st);
-    else launch_direct<KIND, 4, MODE>(p, st);
+    else if constexpr (MODE == kPlain) {
+        if (p.M <= 16) launch_direct<KIND, 1>(p, st);
+        else if (p.M <= 32) launch_direct<KIND, 2>(p, st);
+        else launch_direct<KIND, 4>(p, st);
+    } else {
+        if (p.M <= 16) launch_wide<KIND, 1, 2, MODE>(p, st);
+        else launch_wide<KIND, 2, 2, MODE>(p, st);
+    }
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
 
-// Which form a grouped product takes, by the rows that a group has on average.
-int expert_form(int64_t rows, int64_t groups) {      // 16, 32 or 64 (rows directly from memory), 128 or 256
+// Which form a grouped product takes.  The groups' sizes are on the GPU, so it
+// goes by their average, and by whether a row of 64 x 256 tiles of every group
+// fills the CUs (`many`).  Measured, weights from HBM, rows spread at random
+// over 8 (few) and 64 groups (many) of 2816 x 4096 (us):
+//                            wide      32 x 128   64 x 256   128 x 128   256 x 256
+//   INT4   8 groups,   1 row a group   10.3       16.6       24.5        25.1        53
+//                      4               14.6       19.1       25.9        26.6        53
+//                     16               17.9       19.1       26.1        26.6        53
+//                     64               31.8       22.4       26.3        26.7        53
+//                    128               50.8       38.0       28.4        29.2        53
+//   INT4  64 groups,   1               44.0       53.9       48.6        70.6       109
+//                      4               74.7       72.5       77.0        112        163
+//                     16               97.0       75.5       79.1        114        166
+//                     32              135.6      100.6       80.7        116        168
+//                    128               316        240        141         167        185
+//                    256                                     246         261        293
+//                   1024                                     851         873        790
+//   INT8   8 groups,  16               26.9       25.3       36.9        29.4        53
+//                     32               31.2       25.7       38.2        30.1        54
+//                     64               43.5       35.5       39.8        31.4        53
+//                   1024                                     142         135         124
+//   INT8  64 groups,   4              124        128        128         140         184
+//                     16              149        135        133         144         188
+//                     64              308        230        173         162         197
+//                    128              521        350        218         244         204
+//                   1024                                    1155        1165         848
+int expert_form(int kind, int64_t rows, int64_t groups, int64_t N) {      // 16 (wide), 32, 64, 128 or 256 rows a tile
     const int64_t each = cdiv(rows, groups);
-    return each <= 16 ? 16 : each <= 32 ? 32 : each <= 128 ? 64 : each <= 512 ? 128 : 256;
+    const bool many = groups * cdiv(N, 256) >= 256;
+    if (each <= (many ? 4 : 12)) return 16;
+    if (each <= (many ? 16 : kind == kInt8 ? 32 : 64)) return 32;
+    if (many && each >= (kind == kInt8 ? 128 : 768)) return 256;
+    return kind == kInt8 ? 128 : 64;
 }
 
 template <int KIND>
 int launch_experts(const Operands& p, hipStream_t st) {
-    const int form = expert_form(p.M, p.groups);
-    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4, kGrouped>(p, st);
-    else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4, kGrouped>(p, st);
-    else if (form == 64) launch_direct<KIND, 4, kGrouped>(p, st);
-    else if (form == 32) launch_direct<KIND, 2, kGrouped>(p, st);
-    else launch_direct<KIND, 1, kGrouped>(p, st);
+    const int form = expert_form(KIND, p.M, p.groups, p.N);
+    constexpr int BUF = KIND == kInt4 ? 3 : 4;
+    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, BUF, kGrouped>(p, st);
+    else if (form == 32) launch_tiled<KIND, 1, 2, 1, 2, BUF, kGrouped>(p, st);
+    else if (form != 16) {
+        if constexpr (KIND == kInt8) launch_tiled<KIND, 2, 2, 2, 2, BUF, kGrouped>(p, st);
+        else launch_tiled<KIND, 1, 4, 2, 2, BUF, kGrouped>(p, st);
+    } else if (KIND == kInt4 && p.groups * cdiv(p.N, 256) >= 256) launch_wide<KIND, 1, 4, kGrouped>(p, st);
+    else launch_wide<KIND, 1, 2, kGrouped>(p, st);
     IC_CHECK_LAUNCH();
     return IC_OK;
 }
@@ -919,9 +1047,9 @@ extern "C" int ic_quantized_linear(const int8_t* a, int64_t ld_a, const float* s
     return bits == 8 ? launch_linear<kInt8>(p, st) : launch_linear<kInt4>(p, st);
 }
 
-extern "C" int ic_expert_form(int64_t rows, int64_t groups) {
-    IC_REQUIRE(rows >= 0 && groups >= 1, "ic_expert_form: rows must be >= 0, groups >= 1");
-    return expert_form(rows, groups);
+extern "C" int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N) {
+    IC_REQUIRE((bits == 4 || bits == 8) && rows >= 0 && groups >= 1 && N >= 1, "ic_expert_form: bits must be 4 or 8, rows >= 0, groups and N >= 1");
+    return expert_form(bits == 8 ? kInt8 : kInt4, rows, groups, N);
 }
 
 extern "C" int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t a_rows,

@@ -230,4 +230,4 @@ def test_refusals_of_the_library(L):
                                          k.get("up", one), None)
     assert pack(a=None) == -1 and pack(n=0) == -1 and pack(K=0) == -1 and pack(up=ctypes.c_void_p(8)) == -1
     assert pack(n=1025) == -3 and pack(rank=129) == -3 and pack(K=65537) == -3
-    assert L.ic_expert_form(-1, 4) == -1 and L.ic_expert_form(4, 0) == -1
+    assert L.ic_expert_form(4, -1, 4, 8) == -1 and L.ic_expert_form(4, 4, 0, 8) == -1 and L.ic_expert_form(3, 4, 4, 8) == -1
