@@ -561,8 +561,8 @@ int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32
                      const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,
                      int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out, void* stream);
 
-/* Which form ic_expert_linear takes for these sizes: 16 (16 rows at a time,
- * directly from memory), or tiles of 32, 64, 128 or 256 rows. */
+/* Which form ic_expert_linear takes for these sizes: 1 or 2 (so many times 16
+ * rows, directly from memory), or tiles of 32, 64, 128 or 256 rows. */
 int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N);
 
 /* Low-rank adapters, bf16 or fp16: a [adapters, rank, K] and b [adapters, N,

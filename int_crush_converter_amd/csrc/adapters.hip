@@ -62,52 +62,91 @@ __device__ __forceinline__ lb_f32x4 mma16(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc) 
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lb_bf16x8, w), __builtin_bit_cast(lb_bf16x8, x), acc, 0, 0, 0);
 }
 
-// A work-group of 8 waves takes 16 ranks and 16 rows of one adapter, its waves
-// a share of K each; the sums are joined in LDS in a fixed order.
-template <int DT>
+// A work-group of 8 waves takes 16 RT ranks and 16 MT rows of one adapter, its
+// waves a share of K each; the sums are joined in LDS in a fixed order.
+template <int DT, int MT, int RT>
 __global__ __launch_bounds__(512) void shrink_kernel(const int8_t* __restrict__ a, int64_t ld_a, const float* __restrict__ sa, int M,
                                                      const lb_u32x4* __restrict__ down, int64_t tiles, int rank, int adapters,
                                                      const float* __restrict__ scaling, const int32_t* __restrict__ offsets,
                                                      const int32_t* __restrict__ order, float* __restrict__ t) {
     constexpr int WAVES = 8;
-    __shared__ lb_f32x4 part[WAVES][64];
+    __shared__ lb_f32x4 part[WAVES][MT * RT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-    const int padded = padded_rank(rank), rts = padded / 16, rt = blockIdx.x % rts;
-    const GroupTile tile = find_tile(offsets, adapters, M, 16, blockIdx.x / rts);
+    const int padded = padded_rank(rank), rts = padded / 16, groups = (rts + RT - 1) / RT, rt0 = blockIdx.x % groups * RT;
+    const GroupTile tile = find_tile(offsets, adapters, M, 16 * MT, blockIdx.x / groups);
     if (tile.group < 0) return;
-    const int at = tile.first + r < tile.end ? tile.first + r : tile.end - 1;
-    int m = order[at];
-    m = m < 0 ? 0 : m < M ? m : M - 1;
-    const lb_u32x4* x = reinterpret_cast<const lb_u32x4*>(a + m * ld_a) + g;
-    const lb_u32x4* w = down + ((int64_t)tile.group * rts + rt) * tiles * 128 + lane;
-    lb_f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int64_t t0 = tiles * wave / WAVES, t1 = tiles * (wave + 1) / WAVES;
-    for (int64_t k = t0; k < t1; ++k) {
-        const lb_u32x4 q = x[k * 4];
-        acc = mma16<DT>(w[k * 128], code_values<DT>(q[0], q[1]), acc);
-        acc = mma16<DT>(w[k * 128 + 64], code_values<DT>(q[2], q[3]), acc);
+    auto row_of = [&](int i) {             // (rows past the last repeat the last)
+        const int at = tile.first + i * 16 + r < tile.end ? tile.first + i * 16 + r : tile.end - 1, m = order[at];
+        return m < 0 ? 0 : m < M ? m : M - 1;
+    };
+    const lb_u32x4* x[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = reinterpret_cast<const lb_u32x4*>(a + row_of(i) * ld_a) + g;
+    const lb_u32x4* w[RT];
+#pragma unroll
+    for (int k = 0; k < RT; ++k) w[k] = down + ((int64_t)tile.group * rts + (rt0 + k < rts ? rt0 + k : rts - 1)) * tiles * 128 + lane;
+    lb_f32x4 acc[MT][RT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int k = 0; k < RT; ++k) acc[i][k] = lb_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int t0 = (int)(tiles * wave / WAVES), t1 = (int)(tiles * (wave + 1) / WAVES);
+    for (int c = t0; c < t1; ++c) {
+        lb_u32x4 q[MT], lo[RT], hi[RT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) q[i] = x[i][c * 4];
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            lo[k] = w[k][c * 128];
+            hi[k] = w[k][c * 128 + 64];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const lb_u32x4 u = code_values<DT>(q[i][0], q[i][1]), v = code_values<DT>(q[i][2], q[i][3]);
+#pragma unroll
+            for (int k = 0; k < RT; ++k) acc[i][k] = mma16<DT>(hi[k], v, mma16<DT>(lo[k], u, acc[i][k]));
+        }
     }
-    part[wave][lane] = acc;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int k = 0; k < RT; ++k) part[wave][i * RT + k][lane] = acc[i][k];
     __syncthreads();
-    if (wave) return;
-    lb_f32x4 s = part[0][lane];
+    for (int u = wave; u < MT * RT; u += WAVES) {
+        const int i = u / RT, rt = rt0 + u % RT;
+        if (tile.first + i * 16 + r >= tile.end || rt >= rts) continue;
+        lb_f32x4 s = part[0][u][lane];
 #pragma unroll
-    for (int k = 1; k < WAVES; ++k) s += part[k][lane];
-    const float f = sa[m] * scaling[tile.group];
+        for (int k = 1; k < WAVES; ++k) s += part[k][u][lane];
+        const int m = row_of(i);
+        const float f = sa[m] * scaling[tile.group];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = rt * 16 + g * 4 + i < rank ? s[i] * f : 0.0f;
-    if (tile.first + r < tile.end) *reinterpret_cast<lb_f32x4*>(t + (int64_t)m * padded + rt * 16 + g * 4) = s;
+        for (int k = 0; k < 4; ++k) s[k] = rt * 16 + g * 4 + k < rank ? s[k] * f : 0.0f;
+        *reinterpret_cast<lb_f32x4*>(t + (int64_t)m * padded + rt * 16 + g * 4) = s;
+    }
 }
 
 }  // namespace
 
 int launch_shrink(const Adapted& ad, const int8_t* a, int64_t ld_a, const float* sa, int64_t M, int64_t K, const void* down, int rank,
                   const float* scaling, const int32_t* offsets, const int32_t* order, hipStream_t st) {
-    const dim3 grid((unsigned)(most_tiles(M, ad.adapters, 16) * (ad.rank / 16)));
     const lb_u32x4* d = static_cast<const lb_u32x4*>(down);
     const int64_t tiles = cdiv(K, kActPad) * 2;
-    if (ad.f16) hipLaunchKernelGGL(shrink_kernel<IC_DTYPE_F16>, grid, dim3(512), 0, st, a, ld_a, sa, (int)M, d, tiles, rank, ad.adapters, scaling, offsets, order, ad.t);
-    else hipLaunchKernelGGL(shrink_kernel<IC_DTYPE_BF16>, grid, dim3(512), 0, st, a, ld_a, sa, (int)M, d, tiles, rank, ad.adapters, scaling, offsets, order, ad.t);
+    auto go = [&](auto dt, auto mt, auto rt) {
+        constexpr int MT = decltype(mt)::value, RT = decltype(rt)::value;
+        const dim3 grid((unsigned)(most_tiles(M, ad.adapters, 16 * MT) * cdiv(ad.rank / 16, RT)));
+        hipLaunchKernelGGL((shrink_kernel<decltype(dt)::value, MT, RT>), grid, dim3(512), 0, st, a, ld_a, sa, (int)M, d, tiles, rank, ad.adapters,
+                           scaling, offsets, order, ad.t);
+    };
+    auto shape = [&](auto dt) {
+        typedef std::integral_constant<int, 1> one;
+        if (M <= 1024) go(dt, one{}, one{});
+        else if (ad.rank <= 16) go(dt, std::integral_constant<int, 2>{}, one{});
+        else if (ad.rank <= 32) go(dt, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+        else go(dt, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+    };
+    if (ad.f16) shape(std::integral_constant<int, IC_DTYPE_F16>{});
+    else shape(std::integral_constant<int, IC_DTYPE_BF16>{});
     IC_CHECK_LAUNCH();
     return IC_OK;
 }

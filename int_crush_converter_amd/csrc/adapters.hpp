@@ -55,24 +55,24 @@ __device__ __forceinline__ lb_f32x4 adapter_dot4(const Adapted& ad, int64_t N, i
 }
 
 // The adapters' part of a block of 32 columns x 32 rows of y on the matrix
-// cores: lane (h, r) has row `m` (row r of the block) and, as the operand of B,
-// column n; the result is laid out like the product's own.  t is split into
-// two 16-bit values, t = hi + lo to 2^-16 of it at least (bf16: hi by truncation,
-// which cannot overflow; fp16: 22 bits, of the row brought to a magnitude of 1
-// by a power of two, since t may lie outside fp16's range).  Rows of one block
-// may have different adapters: each adapter's products are formed with all 32
-// rows and kept for its own.
-__device__ __forceinline__ lb_f32x16 adapter_block(const Adapted& ad, int64_t N, int m, int64_t n, int h) {
-    lb_f32x16 sum = {};
+// cores, added to v: lane (h, r) has row `m` (row r of the block) and, as the
+// operand of B, column n; v is laid out like the product's own result.  t is
+// split into two 16-bit values, t = hi + lo to 2^-16 of it at least (bf16: hi by
+// truncation, which cannot overflow; fp16: 22 bits, of the row brought to a
+// magnitude of 1 by a power of two, since t may lie outside fp16's range).  Rows
+// of one block may have different adapters: each adapter's products are formed
+// with all 32 rows and added to its own.
+__device__ __forceinline__ void add_adapters(const Adapted& ad, int64_t N, int m, int64_t n, int h, lb_f32x16& v) {
     int id = ad.ids[m];
     if (id >= ad.adapters) id = -1;
     const lb_f32x4* t = reinterpret_cast<const lb_f32x4*>(ad.t + (int64_t)m * ad.rank) + h * 2;
-    const int64_t column = (n < N ? n : N - 1) * ad.rank;
+    const int64_t column = (n < N ? n : N - 1) * ad.rank + h * 8;
     unsigned long long left = __ballot(id >= 0);
     float down = 1.0f, up = 1.0f;
     if (ad.f16 && left) {
         unsigned top = 0;
         if (id >= 0) {
+#pragma unroll 1
             for (int c = 0; c < ad.rank / 16; ++c)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -92,38 +92,37 @@ __device__ __forceinline__ lb_f32x16 adapter_block(const Adapted& ad, int64_t N,
         const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
         const bool mine = id == a;
         left &= ~__ballot(mine);
-        const uint16_t* b = ad.up + a * N * ad.rank + column + h * 8;
+        const uint16_t* b = ad.up + a * N * ad.rank + column;
         lb_f32x16 part = {};
+#pragma unroll 1
         for (int c = 0; c < ad.rank / 16; ++c) {
-            float v[8];
             const lb_f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
             const lb_f32x4 t0 = mine ? t[4 * c] : zero, t1 = mine ? t[4 * c + 1] : zero;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { v[k] = t0[k] * down; v[4 + k] = t1[k] * down; }
             const lb_u32x4 w = *reinterpret_cast<const lb_u32x4*>(b + c * 16);
             lb_u32x4 hi, lo;
             if (ad.f16) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    hi[k] = pack_half_words<IC_DTYPE_F16>(v[2 * k], v[2 * k + 1]);
-                    lo[k] = pack_half_words<IC_DTYPE_F16>(v[2 * k] - half_word<IC_DTYPE_F16>(hi[k], 0), v[2 * k + 1] - half_word<IC_DTYPE_F16>(hi[k], 1));
+                    const float u0 = (k < 2 ? t0[2 * k & 3] : t1[2 * k & 3]) * down, u1 = (k < 2 ? t0[(2 * k + 1) & 3] : t1[(2 * k + 1) & 3]) * down;
+                    hi[k] = pack_half_words<IC_DTYPE_F16>(u0, u1);
+                    lo[k] = pack_half_words<IC_DTYPE_F16>(u0 - half_word<IC_DTYPE_F16>(hi[k], 0), u1 - half_word<IC_DTYPE_F16>(hi[k], 1));
                 }
                 part = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lb_f16x8, w), __builtin_bit_cast(lb_f16x8, hi), part, 0, 0, 0);
                 part = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lb_f16x8, w), __builtin_bit_cast(lb_f16x8, lo), part, 0, 0, 0);
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    hi[k] = __builtin_amdgcn_perm(__float_as_uint(v[2 * k + 1]), __float_as_uint(v[2 * k]), 0x07060302);
-                    lo[k] = pack_half_words<IC_DTYPE_BF16>(v[2 * k] - half_word<IC_DTYPE_BF16>(hi[k], 0), v[2 * k + 1] - half_word<IC_DTYPE_BF16>(hi[k], 1));
+                    const float u0 = k < 2 ? t0[2 * k & 3] : t1[2 * k & 3], u1 = k < 2 ? t0[(2 * k + 1) & 3] : t1[(2 * k + 1) & 3];
+                    hi[k] = __builtin_amdgcn_perm(__float_as_uint(u1), __float_as_uint(u0), 0x07060302);
+                    lo[k] = pack_half_words<IC_DTYPE_BF16>(u0 - half_word<IC_DTYPE_BF16>(hi[k], 0), u1 - half_word<IC_DTYPE_BF16>(hi[k], 1));
                 }
                 part = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lb_bf16x8, w), __builtin_bit_cast(lb_bf16x8, hi), part, 0, 0, 0);
                 part = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lb_bf16x8, w), __builtin_bit_cast(lb_bf16x8, lo), part, 0, 0, 0);
             }
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) sum[k] = mine ? part[k] * up : sum[k];
+        for (int k = 0; k < 16; ++k) v[k] = mine ? v[k] + part[k] * up : v[k];
     }
-    return sum;
 }
 
 }  // namespace icq

@@ -371,7 +371,7 @@ __device__ __forceinline__ void meet() {
 // those that meet() counts.  It lets the newest N stay outstanding; with spills
 // among these it waits for more copies than it needs, never for fewer.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE = kPlain>
-__global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
+__global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
     typedef typename Acc32<KIND>::T acc_t;
     constexpr int WAVES = WM * WN, BM = 32 * WM * FM, BN = 32 * WN * FN;
     constexpr int X_KB = BM / 16 * (KIND == kInt4 ? 2 : 1), W_KB = BN / 16;      // a stage's KB
@@ -697,6 +697,23 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
                 return (float)(int)d * (sa * sw) + bias;
             }
         };
+        // block (i, j) as whole values with their adapters' part, in place of its sums
+        auto adapted = [&](int i, int j, int m0, int n0, int m_end) {
+            const float sa = row[wm * FM * 32 + i * 32 + r], sum = row[BM + wm * FM * 32 + i * 32 + r];
+            f32x16 v;
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+                const int c = wn * FN * 32 + j * 32 + (k >> 3) * 16 + h * 8 + (k & 7);
+                const lb_f32x4 bias = *reinterpret_cast<const lb_f32x4*>(col + c), sw = *reinterpret_cast<const lb_f32x4*>(col + BN + c);
+                const lb_f32x4 zero = *reinterpret_cast<const lb_f32x4*>(col + 2 * BN + c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k + e] = value(acc[i][j][k + e], sw[e], zero[e], bias[e], sa, sum);
+            }
+            const int m = m0 + i * 32 + r;
+            add_adapters(p.ad, p.N, m < m_end ? m : m_end - 1, n0 + j * 32 + w_column, h, v);
+            acc[i][j] = __builtin_bit_cast(acc_t, v);
+            __builtin_amdgcn_sched_barrier(0);
+        };
         if (p.wide) {
             if (more) start();
             // 32 rows of 128 bytes at a time through the wave's part of the last buffer, so that 8 lanes store a line;
@@ -723,8 +740,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
                 const float sa = KIND == kMx ? 0.0f : row[rw + i * 32 + r], sum = KIND == kMx ? 0.0f : row[BM + rw + i * 32 + r];
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
-                    f32x16 added;
-                    if constexpr (MODE == kAdapted) added = adapter_block(p.ad, p.N, m0 + i * 32 + r < m_end ? m0 + i * 32 + r : m_end - 1, n0 + j * 32 + w_column, h);
+                    if constexpr (MODE == kAdapted) adapted(i, j, m0, n0, m_end);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         lb_f32x4 v[2];
@@ -733,14 +749,14 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
                             const int c = cw + j * 32 + q * 16 + h * 8 + k * 4;
                             const lb_f32x4 bias = *reinterpret_cast<const lb_f32x4*>(col + c);
                             lb_f32x4 sw = {}, zero = {};
-                            if (KIND != kMx) {
+                            if (KIND != kMx && MODE != kAdapted) {
                                 sw = *reinterpret_cast<const lb_f32x4*>(col + BN + c);
                                 zero = *reinterpret_cast<const lb_f32x4*>(col + 2 * BN + c);
                             }
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                v[k][e] = value(acc[i][j][8 * q + 4 * k + e], sw[e], zero[e], bias[e], sa, sum);
-                                if constexpr (MODE == kAdapted) v[k][e] += added[8 * q + 4 * k + e];
+                                if constexpr (MODE == kAdapted) v[k][e] = __int_as_float(acc[i][j][8 * q + 4 * k + e]);
+                                else v[k][e] = value(acc[i][j][8 * q + 4 * k + e], sw[e], zero[e], bias[e], sa, sum);
                             }
                         }
                         if (p.out_dtype == IC_DTYPE_F32) {
@@ -772,25 +788,13 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tiled_kernel(Operands p, 
             sum_t* area = reinterpret_cast<sum_t*>(lds) + wave * 32 * PITCH;
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                if constexpr (MODE == kAdapted) {
-                    // whole values, in place of the sums
-                    const float sa = row[wm * FM * 32 + i * 32 + r], sum = row[BM + wm * FM * 32 + i * 32 + r];
 #pragma unroll
-                    for (int j = 0; j < FN; ++j) {
-                        const f32x16 added = adapter_block(p.ad, p.N, m0 + i * 32 + r < m_end ? m0 + i * 32 + r : m_end - 1, n0 + j * 32 + w_column, h);
+                for (int j = 0; j < FN; ++j) {
+                    if constexpr (MODE == kAdapted) adapted(i, j, m0, n0, m_end);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const int n = j * 32 + (k >> 3) * 16 + h * 8 + (k & 7), c = wn * FN * 32 + n;
-                            area[r * PITCH + n] = __builtin_bit_cast(sum_t, value(acc[i][j][k], col[BN + c], col[2 * BN + c], col[c], sa, sum) + added[k]);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < FN; ++j)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            *reinterpret_cast<sum4_t*>(area + r * PITCH + j * 32 + (k >> 1) * 16 + h * 8 + (k & 1) * 4) =
-                                sum4_t{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<sum4_t*>(area + r * PITCH + j * 32 + (k >> 1) * 16 + h * 8 + (k & 1) * 4) =
+                            sum4_t{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
                 }
                 lds_wave_fence();
                 const int rows = m_end - (m0 + i * 32) < 32 ? m_end - (m0 + i * 32) : 32;
@@ -908,7 +912,9 @@ int launch_linear(const Operands& p, hipStream_t st) {
         else if (p.M <= 32) launch_direct<KIND, 2>(p, st);
         else launch_direct<KIND, 4>(p, st);
     } else {
+        // (64 rows, INT4 12288 x 4096: 17.2 us with 2 x 2, 14.2 with 4 x 4; 4096 x 4096, 64 work-groups: 8.1 and 12.6)
         if (p.M <= 16) launch_wide<KIND, 1, 2, MODE>(p, st);
+        else if (p.M > 32 && cdiv(p.M, 64) * cdiv(p.N, 64) >= 128) launch_wide<KIND, 4, 4, MODE>(p, st);
         else launch_wide<KIND, 2, 2, MODE>(p, st);
     }
     IC_CHECK_LAUNCH();
@@ -941,10 +947,15 @@ int launch_linear(const Operands& p, hipStream_t st) {
 //                     64              308        230        173         162         197
 //                    128              521        350        218         244         204
 //                   1024                                    1155        1165         848
-int expert_form(int kind, int64_t rows, int64_t groups, int64_t N) {      // 16 (wide), 32, 64, 128 or 256 rows a tile
-    const int64_t each = cdiv(rows, groups);
-    const bool many = groups * cdiv(N, 256) >= 256;
-    if (each <= (many ? 4 : 12)) return 16;
+// Where 32 x 128 tiles would leave a third of the CUs idle, the wide form with
+// 32 rows: INT8 10 groups of 60 rows, 1000 x 2901, 15.1 against 16.8; INT4 one
+// group of 64 rows, 4096 x 4096, 8.1 against 16.8, 4096 x 12288 12.3 against
+// 35.5; of 8 groups of 32 rows, 2816 x 4096 (176 tiles) 23.9 against 22.2.
+int expert_form(int kind, int64_t rows, int64_t groups, int64_t N) {      // 1, 2 (wide, so many times 16 rows), 32, 64, 128 or 256
+    const int64_t met = rows < groups ? rows : groups, each = met ? cdiv(rows, met) : 0;
+    const bool many = met * cdiv(N, 256) >= 256;
+    if (each <= (many ? 4 : 12)) return 1;
+    if (met * cdiv(each, 32) * cdiv(N, 128) < 170) return 2;
     if (each <= (many ? 16 : kind == kInt8 ? 32 : 64)) return 32;
     if (many && each >= (kind == kInt8 ? 128 : 768)) return 256;
     return kind == kInt8 ? 128 : 64;
@@ -956,10 +967,13 @@ int launch_experts(const Operands& p, hipStream_t st) {
     constexpr int BUF = KIND == kInt4 ? 3 : 4;
     if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, BUF, kGrouped>(p, st);
     else if (form == 32) launch_tiled<KIND, 1, 2, 1, 2, BUF, kGrouped>(p, st);
-    else if (form != 16) {
+    else if (form > 32) {
         if constexpr (KIND == kInt8) launch_tiled<KIND, 2, 2, 2, 2, BUF, kGrouped>(p, st);
         else launch_tiled<KIND, 1, 4, 2, 2, BUF, kGrouped>(p, st);
-    } else if (KIND == kInt4 && p.groups * cdiv(p.N, 256) >= 256) launch_wide<KIND, 1, 4, kGrouped>(p, st);
+    } else if (form == 2) launch_wide<KIND, 2, 2, kGrouped>(p, st);
+    // four column tiles for INT4 where work-groups abound: 64 groups of 4096 x 1408, 1 row each, 35.4 against 40.3 us
+    // (INT8 50.7 against 53.0, but 2816 x 4096 95 against 83); few: 8 groups of 4 rows, 2816 x 4096, 16.2 against 14.6
+    else if (KIND == kInt4 && (p.M < p.groups ? p.M : p.groups) * cdiv(p.N, 256) >= 256) launch_wide<KIND, 1, 4, kGrouped>(p, st);
     else launch_wide<KIND, 1, 2, kGrouped>(p, st);
     IC_CHECK_LAUNCH();
     return IC_OK;
