@@ -526,7 +526,7 @@ int ic_linear_form(int kind, int64_t M, int64_t N);
  *   order    int32 [rows * per_row]: the pair at a place, -1 behind the last
  *   position int32 [rows, per_row]: the pair's place, -1 = none
  * At most 1024 groups, 64 choices a row, 1048560 pairs.  Workspace:
- * ic_group_workspace_bytes(rows, groups). */
+ * ic_group_workspace_bytes(rows, groups), 16-byte aligned. */
 int64_t ic_group_workspace_bytes(int64_t rows, int64_t groups);
 
 /* The order of given ids (int32, or int64 with wide 1) [rows, per_row],

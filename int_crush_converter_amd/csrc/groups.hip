@@ -20,15 +20,6 @@ namespace {
 constexpr int kThreads = 1024;          // of a work-group that counts or places
 constexpr int kMaxTop = 64;
 
-__device__ __forceinline__ unsigned wave_max_u32(unsigned v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned u = (unsigned)__shfl_xor((int)v, o, 64);
-        v = v > u ? v : u;
-    }
-    return v;
-}
-
 // Keys order like the values, a NaN above all of them and the two zeros equal;
 // 0 is what a mask (-inf) took out, or what has been chosen already.
 __device__ __forceinline__ unsigned logit_key(float x) {
@@ -52,7 +43,7 @@ __device__ __forceinline__ void choose(const void* logits, int64_t at, int exper
     unsigned own = 0;                    // the lane's largest
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) own = own > key[i] ? own : key[i];
-    unsigned best = wave_max_u32(own);
+    unsigned best = wave_top(own);
     const float peak = key_logit(best);
     float total = 0.0f;
     if (!renormalize) {
@@ -61,7 +52,7 @@ __device__ __forceinline__ void choose(const void* logits, int64_t at, int exper
         total = wave_sum(total);
     }
     id = -1;
-    float e = 0.0f;
+    unsigned own_best = 0;               // lane j: the value of choice j
     for (int j = 0; j < top && best; ++j) {
         int slot = 0;
         unsigned long long at_best = 0;
@@ -73,7 +64,7 @@ __device__ __forceinline__ void choose(const void* logits, int64_t at, int exper
         const int first = __builtin_ctzll(at_best);
         if (lane == j) {
             id = slot * 64 + first;
-            e = expf(key_logit(best) - peak);
+            own_best = best;
         }
         own = 0;
 #pragma unroll
@@ -81,8 +72,9 @@ __device__ __forceinline__ void choose(const void* logits, int64_t at, int exper
             if (i == slot && lane == first) key[i] = 0;
             own = own > key[i] ? own : key[i];
         }
-        best = wave_max_u32(own);
+        best = wave_top(own);
     }
+    const float e = id < 0 ? 0.0f : expf(key_logit(own_best) - peak);
     if (renormalize) total = wave_sum(e);
     weight = id < 0 ? 0.0f : e / total;
 }
@@ -91,37 +83,47 @@ __device__ __forceinline__ void choose(const void* logits, int64_t at, int exper
 struct Units {
     int64_t pairs;       // of all units
     int per_unit, units, groups;
-    int32_t* counts;     // [units, groups]
+    uint16_t* counts;    // [units, pitch]: a unit has fewer than 2^16 pairs
+    __host__ __device__ int pitch() const { return (groups + 7) / 8 * 8; }
 };
 
 // Places this unit's pairs: groups' ids from `ids` (-1: none, ordered behind
-// all groups), edges and earlier units' shares from the counts.  lds: 3 x 1024
-// ints and a few.
+// all groups), edges and earlier units' shares from the counts.
 struct PlaceLds {
     int total[kMaxGroups], before[kMaxGroups], base[kMaxGroups + 1], waves[2][kThreads / 64];
 };
+__device__ __forceinline__ void write_counts(const Units& u, int unit, const int* count) {
+    for (int g = threadIdx.x; g < u.pitch(); g += kThreads) u.counts[(int64_t)unit * u.pitch() + g] = (uint16_t)(g < u.groups ? count[g] : 0);
+}
 __device__ __forceinline__ void place_unit(const Units& u, int unit, const int32_t* ids, PlaceLds& s, int32_t* offsets,
                                            int32_t* order, int32_t* position) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // threads in rows of `width`: column = group, each row sums every so manieth unit
-    const int width = u.groups <= 64 ? 64 : u.groups <= 128 ? 128 : u.groups <= 256 ? 256 : u.groups <= 512 ? 512 : 1024;
-    const int g = tid & (width - 1), row = tid / width, rows = kThreads / width;
     s.total[tid] = 0;
     s.before[tid] = 0;
     __syncthreads();
-    if (g < u.groups) {
-        int total = 0, before = 0;
+    // rows of `width` threads, 8 groups a thread; each row sums every so manieth unit (at most 32 rows meet in LDS)
+    const int eights = u.pitch() / 8, width = eights <= 8 ? 8 : eights <= 16 ? 16 : eights <= 32 ? 32 : eights <= 64 ? 64 : 128;
+    const int col = tid & (width - 1), row = tid / width, rows = kThreads / width < 32 ? kThreads / width : 32;
+    if (col < eights && row < rows) {
+        int total[8] = {}, before[8] = {};
 #pragma unroll 8
         for (int k = row; k < u.units; k += rows) {
-            const int c = u.counts[(int64_t)k * u.groups + g];
-            total += c;
-            before += k < unit ? c : 0;
+            const lb_u32x4 c = *reinterpret_cast<const lb_u32x4*>(u.counts + (int64_t)k * u.pitch() + col * 8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int n = (int)(i & 1 ? c[i >> 1] >> 16 : c[i >> 1] & 0xffffu);
+                total[i] += n;
+                before[i] += k < unit ? n : 0;
+            }
         }
-        atomicAdd(&s.total[g], total);       // integers: any order gives the same sum
-        atomicAdd(&s.before[g], before);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {        // (group col * 8 + i at i * 128 + col: lanes on different banks)
+            atomicAdd(&s.total[i * 128 + col], total[i]);        // integers: any order gives the same sum
+            atomicAdd(&s.before[i * 128 + col], before[i]);
+        }
     }
     __syncthreads();
-    const int total = s.total[tid], before = s.before[tid];      // (zeros behind the last group)
+    const int at_lds = (tid & 7) * 128 + (tid >> 3), total = s.total[at_lds], before = s.before[at_lds];      // (zeros behind the last group)
     const int upto = wave_scan(total), earlier = wave_scan(before);
     if (lane == 63) {
         s.waves[0][wave] = upto;
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const void* __restrict_
         }
     }
     __syncthreads();
-    for (int g = tid; g < u.groups; g += kThreads) u.counts[(int64_t)unit * u.groups + g] = count[g];
+    write_counts(u, unit, count);
     if (u.units == 1) {
         __syncthreads();
         place_unit(u, 0, ids, s, offsets, order, position);
@@ -213,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void count_kernel(const ID* __restrict__ 
         if (is) atomicAdd(&count[(int)id], 1);
     }
     __syncthreads();
-    for (int g = tid; g < u.groups; g += kThreads) u.counts[(int64_t)unit * u.groups + g] = count[g];
+    write_counts(u, unit, count);
     if (u.units == 1) {
         __syncthreads();
         place_unit(u, 0, ids, s, offsets, order, position);
@@ -233,8 +235,7 @@ int rows_per_unit(int64_t rows) {
     return (int)(n < 16 ? 16 : n);
 }
 
-// Rows back to their tokens: a lane has 8 columns, and the k rows' loads in
-// flight together (8 at a time).
+// Rows back to their tokens: a lane has 8 columns, and four rows' loads in flight.
 template <int DT>
 __device__ __forceinline__ void load8(const void* p, int64_t base, int c0, int cols, float (&v)[8]) {
     if (c0 + 8 <= cols) {
@@ -271,14 +272,22 @@ __global__ __launch_bounds__(256) void combine_kernel(const void* __restrict__ y
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
     }
-    for (int j = 0; j < top; ++j) {
-        const int at = position[t * top + j];
-        if (at < 0 || at >= pairs) continue;
-        const float w = weights[t * top + j];
-        float v[8];
-        load8<DT>(y, at * ld_y, c0, cols, v);
+    for (int j0 = 0; j0 < top; j0 += 4) {
+        float v[4][8];
+        int at[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(w, v[i], sum[i]);
+        for (int j = 0; j < 4; ++j) {
+            at[j] = j0 + j < top ? position[t * top + j0 + j] : -1;
+            if (at[j] >= pairs) at[j] = -1;
+            if (at[j] >= 0) load8<DT>(y, at[j] * ld_y, c0, cols, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (at[j] < 0) continue;
+            const float w = weights[t * top + j0 + j];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(w, v[j][i], sum[i]);
+        }
     }
     store_cols<DT, 8>(out, t * ld_out, c0, cols, sum);
 }
@@ -312,7 +321,7 @@ using namespace icq;
 
 extern "C" int64_t ic_group_workspace_bytes(int64_t rows, int64_t groups) {
     if (rows < 0 || groups < 1 || groups > kMaxGroups || rows > kMaxRows) return 0;
-    return cdiv(rows, rows_per_unit(rows)) * groups * 4;
+    return cdiv(rows, rows_per_unit(rows)) * cdiv(groups, 8) * 16;
 }
 
 extern "C" int ic_route_tokens(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t ld, int top, int renormalize,
@@ -323,12 +332,13 @@ extern "C" int ic_route_tokens(const void* logits, int dtype, int64_t tokens, in
     IC_REQUIRE(top <= experts, "ic_route_tokens: more choices than experts");
     IC_REQUIRE(offsets && (tokens == 0 || (logits && ids && weights && order && position && workspace)),
                "ic_route_tokens: null pointer");
+    IC_REQUIRE(aligned16(workspace), "ic_route_tokens: workspace not 16-byte aligned");
     IC_REQUIRE(tokens <= 1 || ld >= experts, "ic_route_tokens: leading dimension below the number of experts");
     hipStream_t st = as_stream(stream);
     const int per = rows_per_unit(tokens);
     const int units = tokens ? (int)cdiv(tokens, per) : 1;
     ProfScope prof(st, PT_OTHER, 0.0, (double)tokens * experts * (dtype == IC_DTYPE_F32 ? 4 : 2) + 16.0 * tokens * top);
-    const Units u{tokens * top, per * top, units, (int)experts, static_cast<int32_t*>(workspace)};
+    const Units u{tokens * top, per * top, units, (int)experts, static_cast<uint16_t*>(workspace)};
     if (tokens == 0) {
         hipLaunchKernelGGL(place_kernel, dim3(1), dim3(kThreads), 0, st, Units{0, 1, 0, (int)experts, nullptr}, ids, offsets, order, position);
         IC_CHECK_LAUNCH();
@@ -346,11 +356,12 @@ extern "C" int ic_group_rows(const void* given, int wide, int64_t rows, int64_t 
                              int32_t* order, int32_t* position, void* workspace, void* stream) {
     if (const int rc = check_groups("ic_group_rows", rows, per_row, groups)) return rc;
     IC_REQUIRE(offsets && (rows == 0 || (given && ids && order && position && workspace)), "ic_group_rows: null pointer");
+    IC_REQUIRE(aligned16(workspace), "ic_group_rows: workspace not 16-byte aligned");
     hipStream_t st = as_stream(stream);
     const int per = rows_per_unit(rows);
     const int units = rows ? (int)cdiv(rows, per) : 1;
     ProfScope prof(st, PT_OTHER, 0.0, (wide ? 20.0 : 16.0) * rows * per_row);
-    const Units u{rows * per_row, (int)(per * per_row), units, (int)groups, static_cast<int32_t*>(workspace)};
+    const Units u{rows * per_row, (int)(per * per_row), units, (int)groups, static_cast<uint16_t*>(workspace)};
     if (rows == 0) {
         hipLaunchKernelGGL(place_kernel, dim3(1), dim3(kThreads), 0, st, Units{0, 1, 0, (int)groups, nullptr}, ids, offsets, order, position);
         IC_CHECK_LAUNCH();

@@ -7,15 +7,35 @@ namespace icq {
 
 constexpr int kMaxGroups = 1024;
 
-// Inclusive sum over the 64 lanes.
+// v of another lane by DPP, `none` where there is no such lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or(int none, int v) {
+    return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
+}
+constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118;     // within 16 lanes
+constexpr int kLast15 = 0x142, kLast31 = 0x143;     // the last lane of 16 to the next 16, of 32 to the upper 32
+
+// Inclusive sum over the 64 lanes: within 16 lanes, then across them.
 __device__ __forceinline__ int wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
+    v += dpp_or<kShr1, 0xf>(0, v);
+    v += dpp_or<kShr2, 0xf>(0, v);
+    v += dpp_or<kShr4, 0xf>(0, v);
+    v += dpp_or<kShr8, 0xf>(0, v);
+    v += dpp_or<kLast15, 0xa>(0, v);
+    v += dpp_or<kLast31, 0xc>(0, v);
     return v;
+}
+
+// The largest of the 64 lanes, the same scalar for all.
+__device__ __forceinline__ unsigned wave_top(unsigned v) {
+    auto larger = [](unsigned a, int b) { return a > (unsigned)b ? a : (unsigned)b; };
+    v = larger(v, dpp_or<kShr1, 0xf>(0, (int)v));
+    v = larger(v, dpp_or<kShr2, 0xf>(0, (int)v));
+    v = larger(v, dpp_or<kShr4, 0xf>(0, (int)v));
+    v = larger(v, dpp_or<kShr8, 0xf>(0, (int)v));
+    v = larger(v, dpp_or<kLast15, 0xa>(0, (int)v));
+    v = larger(v, dpp_or<kLast31, 0xc>(0, (int)v));
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // Rows [first, end) of group g; ends past `rows` count as `rows`.

@@ -24,7 +24,7 @@ class RowGroups:
     """The (row, choice) pairs of a batch ordered by group, in int32 on the GPU; pair p is choice ``p % per_row`` of row
     ``p // per_row``.  Made by ``group_rows`` and ``route_tokens``."""
 
-    __slots__ = ("data", "rows", "per_row", "groups")
+    __slots__ = ("data", "scratch", "rows", "per_row", "groups")
 
     def __init__(self, *args, **kwargs):
         raise TypeError("RowGroups are made by group_rows and route_tokens")
@@ -34,19 +34,22 @@ class RowGroups:
         if not 1 <= groups <= MAX_GROUPS or not 1 <= per_row <= MAX_CHOICES or rows * per_row > MAX_PAIRS:
             raise ValueError(f"at most {MAX_GROUPS} groups, {MAX_CHOICES} choices a row and {MAX_PAIRS} pairs, got {groups}, "
                              f"{per_row} and {rows} rows")
-        g = cls.__new__(cls)                 # one allocation: ids, order, position, offsets
-        g.data = torch.empty(3 * rows * per_row + groups + 1, dtype=torch.int32, device=dev)
+        # one allocation: workspace (ic_group_workspace_bytes: 16-bit counts of at most 256 units of at least 16 rows), ids,
+        # order, position, offsets
+        g = cls.__new__(cls)
+        g.scratch = min(256, (rows + 15) // 16) * ((groups + 7) // 8) * 4
+        g.data = torch.empty(g.scratch + 3 * rows * per_row + groups + 1, dtype=torch.int32, device=dev)
         g.rows, g.per_row, g.groups = rows, per_row, groups
         return g
 
     def pointers(self) -> tuple[int, int, int, int]:
         """Addresses of ids, offsets, order and position."""
-        at, n = self.data.data_ptr(), 4 * self.rows * self.per_row
+        at, n = self.data.data_ptr() + 4 * self.scratch, 4 * self.rows * self.per_row
         return at, at + 3 * n, at + n, at + 2 * n
 
     def _part(self, i: int) -> torch.Tensor:
-        n = self.rows * self.per_row
-        return self.data[i * n: (i + 1) * n]
+        at, n = self.scratch, self.rows * self.per_row
+        return self.data[at + i * n: at + (i + 1) * n]
 
     @property
     def ids(self) -> torch.Tensor:
@@ -56,7 +59,7 @@ class RowGroups:
     @property
     def offsets(self) -> torch.Tensor:
         """int32 [groups + 1]: group g has the places offsets[g] to offsets[g + 1] - 1 of the order."""
-        return self.data[3 * self.rows * self.per_row:]
+        return self.data[self.scratch + 3 * self.rows * self.per_row:]
 
     @property
     def order(self) -> torch.Tensor:
@@ -69,11 +72,6 @@ class RowGroups:
         return self._part(2).view(self.rows, self.per_row)
 
 
-def _workspace(g: RowGroups) -> torch.Tensor:
-    # ic_group_workspace_bytes: counts of at most 256 units of at least 16 rows
-    return torch.empty(min(256, -(-g.rows // 16)) * g.groups, dtype=torch.int32, device=g.data.device)
-
-
 def group_rows(ids: torch.Tensor, groups: int) -> RowGroups:
     """The order of ids [rows] or [rows, per_row] (int32 or int64) by group; equal ones keep their order.  Numbers outside
     [0, groups) mean none: such pairs are in no group."""
@@ -81,9 +79,9 @@ def group_rows(ids: torch.Tensor, groups: int) -> RowGroups:
         raise ValueError(f"expected int32 or int64 ids [rows] or [rows, per_row], got {ids.dtype} {tuple(ids.shape)}")
     given = nat.on_gpu("ids", ids).contiguous()
     g = RowGroups._empty(ids.shape[0], ids.shape[1] if ids.dim() == 2 else 1, groups, given.device)
-    ws, (to, offsets, order, position) = _workspace(g), g.pointers()
+    to, offsets, order, position = g.pointers()
     call("ic_group_rows", given.data_ptr(), int(given.dtype == torch.int64), g.rows, g.per_row, groups, to, offsets, order,
-         position, ws.data_ptr(), nat.stream_for(given))
+         position, g.data.data_ptr(), nat.stream_for(given))
     return g
 
 
@@ -105,9 +103,9 @@ def route_tokens(logits: torch.Tensor, top: int, *, renormalize: bool = True) ->
     g = RowGroups._empty(tokens, top, experts, x.device)
     x = as_rows(x) if tokens else x
     weights = torch.empty((tokens, top), dtype=torch.float32, device=x.device)
-    ws, (ids, offsets, order, position) = _workspace(g), g.pointers()
+    ids, offsets, order, position = g.pointers()
     call("ic_route_tokens", x.data_ptr(), code, tokens, experts, x.stride(0) if tokens > 1 else experts, top,
-         int(renormalize), ids, weights.data_ptr(), offsets, order, position, ws.data_ptr(), nat.stream_for(x))
+         int(renormalize), ids, weights.data_ptr(), offsets, order, position, g.data.data_ptr(), nat.stream_for(x))
     return g, weights
 
 

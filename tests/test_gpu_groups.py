@@ -210,7 +210,7 @@ def test_other_stream_and_graph(gpu_dev):
         def chain():
             groups, w = icq.route_tokens(x, 4)
             again = icq.group_rows(groups.ids, 60)
-            return groups.data, w, again.data, icq.combine_experts(y, groups, w)
+            return groups.ids, groups.order, groups.offsets, groups.position, w, again.order, icq.combine_experts(y, groups, w)
 
         eager = [t.clone() for t in chain()]
         side = torch.cuda.Stream()
@@ -235,14 +235,14 @@ def test_two_graphs_at_once(gpu_dev):
     import int_crush_converter_amd as icq
     g = torch.Generator().manual_seed(6)
     xs = [torch.randn(3000, 100, generator=g).to(gpu_dev) for _ in range(2)]
-    want = [[t.clone() for t in (lambda r: (r[0].data, r[1]))(icq.route_tokens(x, 5))] for x in xs]
+    want = [[t.clone() for t in (lambda r: (r[0].ids, r[0].order, r[0].offsets, r[0].position, r[1]))(icq.route_tokens(x, 5))] for x in xs]
     graphs, held, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
     for x in xs:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             r = icq.route_tokens(x, 5)
         graphs.append(graph)
-        held.append((r[0].data, r[1]))
+        held.append((r[0].ids, r[0].order, r[0].offsets, r[0].position, r[1]))
     torch.cuda.synchronize()
     for k in range(3):
         for s, graph in zip(streams, graphs):

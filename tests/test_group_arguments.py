@@ -187,11 +187,11 @@ def test_operands_elsewhere(monkeypatch):
 
 
 def test_sizes_of_the_library(L):
-    assert L.ic_group_workspace_bytes(0, 5) == 0 and L.ic_group_workspace_bytes(1, 5) == 20
-    assert L.ic_group_workspace_bytes(17, 64) == 2 * 64 * 4 and L.ic_group_workspace_bytes(1048560, 1024) <= 256 * 1024 * 4
+    assert L.ic_group_workspace_bytes(0, 5) == 0 and L.ic_group_workspace_bytes(1, 5) == 16
+    assert L.ic_group_workspace_bytes(17, 64) == 2 * 64 * 2 and L.ic_group_workspace_bytes(1048560, 1024) <= 256 * 1024 * 2
     assert L.ic_group_workspace_bytes(10, 1025) == 0
     for rows in (1, 16, 17, 4000, 4096, 4097, 8191, 100000, 1048560):
-        assert L.ic_group_workspace_bytes(rows, 7) <= min(256, -(-rows // 16)) * 7 * 4        # what the package allocates
+        assert L.ic_group_workspace_bytes(rows, 7) <= 4 * groups.RowGroups._empty(rows, 1, 7, torch.device("cpu")).scratch
     assert L.ic_adapter_down_bytes(3, 12, 130) == 3 * 16 * 256 * 2 and L.ic_adapter_up_bytes(3, 10, 17) == 3 * 10 * 32 * 2
     assert L.ic_adapted_linear_workspace_bytes(7, 12) == 7 * 16 * 4
     assert L.ic_adapter_up_bytes(1024, 1048560, 128) == 1024 * 1048560 * 128 * 2              # past 32 bits
@@ -207,6 +207,7 @@ def test_refusals_of_the_library(L):
     rows = lambda **k: L.ic_group_rows(k.get("ids", one), 0, k.get("rows", 4), k.get("per", 2), k.get("groups", 8), one, one, one, one,     # noqa: E731
                                        k.get("ws", one), None)
     assert rows(ids=None) == -1 and rows(ws=None) == -1 and rows(per=0) == -1 and rows(groups=0) == -1 and rows(groups=2000) == -3
+    assert rows(ws=ctypes.c_void_p(8)) == -1
     assert rows(rows=1 << 62, per=64) == -3
     comb = lambda **k: L.ic_combine_rows(k.get("y", one), k.get("dtype", 1), k.get("tokens", 4), k.get("top", 2), k.get("cols", 64),         # noqa: E731
                                          k.get("ldy", 64), one, one, k.get("res"), k.get("ldr", 0), one, k.get("ldo", 64), None)
