@@ -28,54 +28,56 @@ __device__ __forceinline__ unsigned logit_key(float x) {
 }
 __device__ __forceinline__ float key_logit(unsigned k) { return k == 0xffffffffu ? __uint_as_float(0x7fc00000u) : key_float(k); }
 
-// The choice of one token by one wave: expert i * 64 + lane in slot i.  Each
-// choice is a maximum over the lanes and a search for its first place.
+// The choice of one token by one wave.  A lane has SLOTS consecutive experts and
+// sorts them, largest first and of equals the lowest, so that a choice is a
+// maximum over the lanes' first ones, and of lanes with that maximum the lowest.
 template <int DT, int SLOTS>
 __device__ __forceinline__ void choose(const void* logits, int64_t at, int experts, int top, int renormalize,
                                        int& id, float& weight) {
     const int lane = threadIdx.x & 63;
     unsigned key[SLOTS];
+    int expert[SLOTS];
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
-        const int e = i * 64 + lane;
-        key[i] = e < experts ? logit_key(load_as_f32(logits, DT, at + e)) : 0u;
+        expert[i] = lane * SLOTS + i;
+        key[i] = expert[i] < experts ? logit_key(load_as_f32(logits, DT, at + expert[i])) : 0u;
     }
-    unsigned own = 0;                    // the lane's largest
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) own = own > key[i] ? own : key[i];
-    unsigned best = wave_top(own);
+    for (int n = SLOTS - 1; n > 0; --n)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {          // neighbours change places only if the second is larger: equals keep their order
+            const bool swap = key[i + 1] > key[i];
+            const unsigned k = key[i];
+            const int e = expert[i];
+            key[i] = swap ? key[i + 1] : k;
+            expert[i] = swap ? expert[i + 1] : e;
+            key[i + 1] = swap ? k : key[i + 1];
+            expert[i + 1] = swap ? e : expert[i + 1];
+        }
+    unsigned best = wave_top(key[0]);
     const float peak = key_logit(best);
     float total = 0.0f;
     if (!renormalize) {
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) total += key[i] ? expf(key_logit(key[i]) - peak) : 0.0f;
-        total = wave_sum(total);
+        total = wave_total(total);
     }
     id = -1;
-    unsigned own_best = 0;               // lane j: the value of choice j
+    unsigned own = 0;                          // lane j: the value of choice j
     for (int j = 0; j < top && best; ++j) {
-        int slot = 0;
-        unsigned long long at_best = 0;
-#pragma unroll
-        for (int i = SLOTS - 1; i >= 0; --i) {
-            const unsigned long long here = __ballot(key[i] == best);
-            if (here) { at_best = here; slot = i; }
-        }
-        const int first = __builtin_ctzll(at_best);
-        if (lane == j) {
-            id = slot * 64 + first;
-            own_best = best;
-        }
-        own = 0;
+        const unsigned long long at_best = __ballot(key[0] == best), taken = at_best & (0 - at_best);
+        const unsigned long long mine = 1ull << j;
+        id = (int)lanes_of(mine, (unsigned)__builtin_amdgcn_readlane(expert[0], __builtin_ctzll(at_best)), (unsigned)id);
+        own = lanes_of(mine, best, own);
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) {
-            if (i == slot && lane == first) key[i] = 0;
-            own = own > key[i] ? own : key[i];
+            key[i] = lanes_of(taken, i + 1 < SLOTS ? key[i + 1 < SLOTS ? i + 1 : i] : 0u, key[i]);
+            if (i + 1 < SLOTS) expert[i] = (int)lanes_of(taken, (unsigned)expert[i + 1 < SLOTS ? i + 1 : i], (unsigned)expert[i]);
         }
-        best = wave_top(own);
+        best = wave_top(key[0]);
     }
-    const float e = id < 0 ? 0.0f : expf(key_logit(own_best) - peak);
-    if (renormalize) total = wave_sum(e);
+    const float e = id < 0 ? 0.0f : expf(key_logit(own) - peak);
+    if (renormalize) total = wave_total(e);
     weight = id < 0 ? 0.0f : e / total;
 }
 
@@ -90,7 +92,8 @@ struct Units {
 // Places this unit's pairs: groups' ids from `ids` (-1: none, ordered behind
 // all groups), edges and earlier units' shares from the counts.
 struct PlaceLds {
-    int total[kMaxGroups], before[kMaxGroups], base[kMaxGroups + 1], waves[2][kThreads / 64];
+    int total[kMaxGroups + 1], before[kMaxGroups], base[kMaxGroups + 1], waves[2][kThreads / 64];
+    uint16_t share[kThreads / 64][kMaxGroups + 1];       // of a wave's 64 pairs, then of the waves before it
 };
 __device__ __forceinline__ void write_counts(const Units& u, int unit, const int* count) {
     for (int g = threadIdx.x; g < u.pitch(); g += kThreads) u.counts[(int64_t)unit * u.pitch() + g] = (uint16_t)(g < u.groups ? count[g] : 0);
@@ -98,6 +101,8 @@ __device__ __forceinline__ void write_counts(const Units& u, int unit, const int
 __device__ __forceinline__ void place_unit(const Units& u, int unit, const int32_t* ids, PlaceLds& s, int32_t* offsets,
                                            int32_t* order, int32_t* position) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t first = (int64_t)unit * u.per_unit, last = first + u.per_unit < u.pairs ? first + u.per_unit : u.pairs;
+    int next = first + tid < last ? ids[first + tid] : -1;
     s.total[tid] = 0;
     s.before[tid] = 0;
     __syncthreads();
@@ -136,7 +141,6 @@ __device__ __forceinline__ void place_unit(const Units& u, int unit, const int32
         all += s.waves[0][w];
         mine += s.waves[1][w];
     }
-    const int64_t first = (int64_t)unit * u.per_unit;
     if (tid < u.groups) s.base[tid] = start + before;
     if (tid == 0) s.base[u.groups] = all + (int)(first - mine);          // pairs of no group
     if (unit == 0) {
@@ -144,27 +148,41 @@ __device__ __forceinline__ void place_unit(const Units& u, int unit, const int32
         if (tid == 0) offsets[u.groups] = all;
     }
     __syncthreads();
-    if (wave) return;
-    // one wave goes through the unit in order, 64 pairs at a time
-    const int64_t last = first + u.per_unit < u.pairs ? first + u.per_unit : u.pairs;
-    for (int64_t p0 = first; p0 < last; p0 += 64) {
-        const int64_t p = p0 + lane;
+    // 1024 pairs at a time: each wave ranks its 64, and the groups' shares of the 16 waves are summed in order
+    for (int64_t p1 = first;; p1 += kThreads) {
+        const int64_t p = p1 + tid;
         const bool have = p < last;
-        const int id = have ? ids[p] : -1, key = id < 0 ? u.groups : id;
+        const int id = next, key = id < 0 ? u.groups : id;
+        next = p + kThreads < last ? ids[p + kThreads] : -1;
+        for (int g = lane; g <= u.groups; g += 64) s.share[wave][g] = 0;
         unsigned long long same = __ballot(have);
         for (int b = 0; (u.groups >> b) != 0; ++b) {
             const unsigned long long m = __ballot((key >> b) & 1);
             same &= (key >> b) & 1 ? m : ~m;
         }
         const int rank = (int)__builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
-        const int at = s.base[key] + rank;
         lds_wave_fence();
-        if (have && rank == 0) s.base[key] += __builtin_popcountll(same);
-        lds_wave_fence();
+        if (have && rank == 0) s.share[wave][key] = (uint16_t)__builtin_popcountll(same);
+        __syncthreads();
+        for (int g = tid; g <= u.groups; g += kThreads) {
+            int sum = 0;
+#pragma unroll
+            for (int w = 0; w < kThreads / 64; ++w) {
+                const int own = s.share[w][g];
+                s.share[w][g] = (uint16_t)sum;
+                sum += own;
+            }
+            s.total[g] = sum;
+        }
+        __syncthreads();
         if (have) {
+            const int at = s.base[key] + s.share[wave][key] + rank;
             order[at] = id < 0 ? -1 : (int32_t)p;
             position[p] = id < 0 ? -1 : at;
         }
+        if (p1 + kThreads >= last) break;
+        __syncthreads();
+        for (int g = tid; g <= u.groups; g += kThreads) s.base[g] += s.total[g];
     }
 }
 

@@ -26,16 +26,40 @@ __device__ __forceinline__ int wave_scan(int v) {
     return v;
 }
 
-// The largest of the 64 lanes, the same scalar for all.
+// The largest of the 64 lanes, the same scalar for all.  One instruction a
+// step, which the compiler makes three of (a lane without a partner keeps its
+// value; a DPP operand needs two wait states behind its own writing).
 __device__ __forceinline__ unsigned wave_top(unsigned v) {
-    auto larger = [](unsigned a, int b) { return a > (unsigned)b ? a : (unsigned)b; };
-    v = larger(v, dpp_or<kShr1, 0xf>(0, (int)v));
-    v = larger(v, dpp_or<kShr2, 0xf>(0, (int)v));
-    v = larger(v, dpp_or<kShr4, 0xf>(0, (int)v));
-    v = larger(v, dpp_or<kShr8, 0xf>(0, (int)v));
-    v = larger(v, dpp_or<kLast15, 0xa>(0, (int)v));
-    v = larger(v, dpp_or<kLast31, 0xc>(0, (int)v));
+    asm("s_nop 1\n\tv_max_u32_dpp %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_u32_dpp %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_u32_dpp %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_u32_dpp %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_u32_dpp %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_u32_dpp %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf"
+        : "+v"(v));
     return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// a in the lanes of the mask, else b.
+__device__ __forceinline__ unsigned lanes_of(unsigned long long mask, unsigned a, unsigned b) {
+    unsigned d;
+    asm("v_cndmask_b32_e64 %0, %1, %2, %3" : "=v"(d) : "v"(b), "v"(a), "s"(mask));
+    return d;
+}
+
+// The sum of the 64 lanes in one order, the same scalar for all.
+__device__ __forceinline__ float wave_total(float v) {
+    auto part = [](float x, auto ctrl, auto rows) {
+        return __int_as_float(dpp_or<decltype(ctrl)::value, decltype(rows)::value>(0, __float_as_int(x)));
+    };
+    typedef std::integral_constant<int, 0xf> all;
+    v += part(v, std::integral_constant<int, kShr1>{}, all{});
+    v += part(v, std::integral_constant<int, kShr2>{}, all{});
+    v += part(v, std::integral_constant<int, kShr4>{}, all{});
+    v += part(v, std::integral_constant<int, kShr8>{}, all{});
+    v += part(v, std::integral_constant<int, kLast15>{}, std::integral_constant<int, 0xa>{});
+    v += part(v, std::integral_constant<int, kLast31>{}, std::integral_constant<int, 0xc>{});
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // Rows [first, end) of group g; ends past `rows` count as `rows`.
