@@ -565,13 +565,15 @@ int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32
  * rows, directly from memory), or tiles of 32, 64, 128 or 256 rows. */
 int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N);
 
-/* Low-rank adapters, bf16 or fp16: a [adapters, rank, K] and b [adapters, N,
- * rank], contiguous, laid out once for ic_adapted_linear (ic_adapter_down_bytes
- * and ic_adapter_up_bytes, 16-byte aligned).  At most 1024 of rank 128. */
+/* Low-rank adapters, both of bf16 or of fp16: a [adapters, rank, K] and b
+ * [adapters, N, rank], contiguous, laid out once for ic_adapted_linear
+ * (ic_adapter_down_bytes and ic_adapter_up_bytes, 16-byte aligned).  b is
+ * finite: Inf or NaN in it may reach rows of other adapters.  At most 1024 of
+ * rank 128. */
 int64_t ic_adapter_down_bytes(int64_t adapters, int rank, int64_t K);
-int64_t ic_adapter_up_bytes(int64_t adapters, int64_t N, int rank);
-int ic_adapter_pack(const void* a, const void* b, int64_t adapters, int rank, int64_t N, int64_t K, void* down,
-                    void* up, void* stream);
+int64_t ic_adapter_up_bytes(int64_t adapters, int64_t N, int rank, int dtype);
+int ic_adapter_pack(const void* a, const void* b, int dtype, int64_t adapters, int rank, int64_t N, int64_t K,
+                    void* down, void* up, void* stream);
 
 /* ic_quantized_linear beside which row m adds the adapter ids[m] of its own
  * (none for ids outside [0, adapters)):

@@ -112,8 +112,8 @@ _SIGS = {
                                 _i32, _i64, _i64, _vp, _i32, _i64, _vp]),
     "ic_expert_form": (_i32, [_i32, _i64, _i64, _i64]),
     "ic_adapter_down_bytes": (_i64, [_i64, _i32, _i64]),
-    "ic_adapter_up_bytes": (_i64, [_i64, _i64, _i32]),
-    "ic_adapter_pack": (_i32, [_vp, _vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp]),
+    "ic_adapter_up_bytes": (_i64, [_i64, _i64, _i32, _i32]),
+    "ic_adapter_pack": (_i32, [_vp, _vp, _i32, _i64, _i32, _i64, _i64, _vp, _vp, _vp]),
     "ic_adapted_linear_workspace_bytes": (_i64, [_i64, _i32]),
     "ic_adapted_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _i64, _i64, _vp, _vp,
                                  _i32, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _vp]),

@@ -21,7 +21,8 @@ class LowRankAdapters:
     float16, and their scaling (a number, or [count]).
 
     Beside a rotated weight the activations are rotated too: give ``rotate_weights(a, rot_size)`` there, whose rows are
-    padded like the activations'.  Adapters of smaller rank are padded with zeros to the largest."""
+    padded like the activations'.  Adapters of smaller rank are padded with zeros to the largest.  b has to be finite; Inf
+    or NaN in a reaches the adapter's own rows."""
 
     __slots__ = ("down", "up", "scaling", "code", "count", "rank", "in_features", "out_features")
 
@@ -34,6 +35,8 @@ class LowRankAdapters:
         N = b.shape[1]
         if not 1 <= n <= MAX_GROUPS or not 1 <= r <= MAX_RANK or not 1 <= K <= MAX_FEATURES or N < 1:
             raise ValueError(f"1 to {MAX_GROUPS} adapters of rank 1 to {MAX_RANK} and in_features up to {MAX_FEATURES}, got {n}, {r}, {K}")
+        if not torch.isfinite(b).all():
+            raise ValueError("b holds Inf or NaN, which would reach rows of other adapters")
         a, b = nat.on_gpu("a", a).contiguous(), nat.on_gpu("b", b).contiguous()
         if isinstance(scaling, torch.Tensor):
             if scaling.numel() not in (1, n):
@@ -46,6 +49,6 @@ class LowRankAdapters:
         self.code = nat.dtype_code(a)
         L = nat.lib()
         self.down = nat.workspace(L.ic_adapter_down_bytes(n, r, K), a.device)
-        self.up = nat.workspace(L.ic_adapter_up_bytes(n, N, r), a.device)
-        call("ic_adapter_pack", a.data_ptr(), b.data_ptr(), n, r, N, K, self.down.data_ptr(), self.up.data_ptr(),
+        self.up = nat.workspace(L.ic_adapter_up_bytes(n, N, r, self.code), a.device)
+        call("ic_adapter_pack", a.data_ptr(), b.data_ptr(), self.code, n, r, N, K, self.down.data_ptr(), self.up.data_ptr(),
              nat.stream_for(a, b))

@@ -10,11 +10,13 @@ namespace {
 // A [adapters, rank, K] -> tiles of 16 ranks x 64 columns, [adapter][rank / 16][K / 64]: two words of 16 bytes a lane,
 // lane 16 g + r holding columns 16 g .. 16 g + 7 and + 8 .. + 15 of rank r, as a lane holds 16 consecutive codes of
 // a row.  Zeros behind the last rank and column.
+__host__ __device__ inline int down_tiles(int rank) { return (rank + 15) / 16; }
+
 __global__ __launch_bounds__(256) void pack_down_kernel(const uint16_t* __restrict__ src, int64_t adapters, int rank, int64_t K,
                                                         lb_u32x4* __restrict__ dst, int64_t tiles) {
     const int lane = threadIdx.x & 63, r = lane & 15;
     const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);     // [adapter][rank tile][column tile]
-    const int rt = padded_rank(rank) / 16;
+    const int rt = down_tiles(rank);
     if (at >= adapters * rt * tiles) return;
     const int64_t a = at / (rt * tiles);
     const int row = (int)(at / tiles % rt) * 16 + r;
@@ -30,15 +32,29 @@ __global__ __launch_bounds__(256) void pack_down_kernel(const uint16_t* __restri
     dst[at * 128 + 64 + lane] = w[1];
 }
 
-// B [adapters, N, rank] -> rows padded with zeros to whole 16 ranks.
-__global__ __launch_bounds__(256) void pack_up_kernel(const uint16_t* __restrict__ src, int64_t rows, int rank, uint16_t* __restrict__ dst) {
-    const int padded = padded_rank(rank);
-    const int64_t total = rows * padded, stride = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
-        const int64_t row = i / padded;
-        const int c = (int)(i - row * padded);
-        dst[i] = c < rank ? src[row * rank + c] : (uint16_t)0;
+// B [adapters, N, rank] -> tiles (adapters.hpp), a lane one column's 8 ranks.
+__global__ __launch_bounds__(256) void pack_up_kernel(const uint16_t* __restrict__ src, int64_t adapters, int64_t N, int rank, int f16,
+                                                      lb_u32x4* __restrict__ dst) {
+    const int lane = threadIdx.x & 63, parts = rank_parts(rank), planes = f16 ? 2 : 1;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n_tiles = cdiv(N, 16);     // [adapter][column tile][part][plane]
+    if (at >= adapters * n_tiles * parts * planes) return;
+    const int64_t n = at / (parts * planes) % n_tiles * 16 + (lane & 15), a = at / (parts * planes) / n_tiles;
+    const int rank0 = (int)(at / planes % parts) * kRankPart + (lane >> 4) * 8, plane = (int)(at % planes);
+    lb_u32x4 w = {0, 0, 0, 0};
+    if (n < N) {
+        const uint16_t* s = src + (a * N + n) * rank;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (rank0 + k >= rank) continue;
+            unsigned v = s[rank0 + k];
+            if (f16) {
+                const float x = f16_bits_to_f32((uint16_t)v), hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+                v = __float_as_uint(plane ? x - hi : hi) >> 16;
+            }
+            w[k >> 1] |= v << (16 * (k & 1));
+        }
     }
+    dst[at * 64 + lane] = w;
 }
 
 // 8 codes of a lane as the 16-bit values of an operand (exact: |q| <= 128).
@@ -68,11 +84,12 @@ template <int DT, int MT, int RT>
 __global__ __launch_bounds__(512) void shrink_kernel(const int8_t* __restrict__ a, int64_t ld_a, const float* __restrict__ sa, int M,
                                                      const lb_u32x4* __restrict__ down, int64_t tiles, int rank, int adapters,
                                                      const float* __restrict__ scaling, const int32_t* __restrict__ offsets,
-                                                     const int32_t* __restrict__ order, float* __restrict__ t) {
+                                                     const int32_t* __restrict__ order, uint16_t* __restrict__ t) {
     constexpr int WAVES = 8;
     __shared__ lb_f32x4 part[WAVES][MT * RT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-    const int padded = padded_rank(rank), rts = padded / 16, groups = (rts + RT - 1) / RT, rt0 = blockIdx.x % groups * RT;
+    const int parts = rank_parts(rank), rts = down_tiles(rank), groups = (rts + RT - 1) / RT, rt0 = blockIdx.x % groups * RT;
+    if (blockIdx.x == 0 && threadIdx.x < parts * 64) t[(int64_t)M * parts * 64 + threadIdx.x] = 0;       // the row of zeros
     const GroupTile tile = find_tile(offsets, adapters, M, 16 * MT, blockIdx.x / groups);
     if (tile.group < 0) return;
     auto row_of = [&](int i) {             // (rows past the last repeat the last)
@@ -120,9 +137,21 @@ __global__ __launch_bounds__(512) void shrink_kernel(const int8_t* __restrict__ 
         for (int k = 1; k < WAVES; ++k) s += part[k][u][lane];
         const int m = row_of(i);
         const float f = sa[m] * scaling[tile.group];
+        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] = rt * 16 + g * 4 + k < rank ? s[k] * f : 0.0f;
-        *reinterpret_cast<lb_f32x4*>(t + (int64_t)m * padded + rt * 16 + g * 4) = s;
+        for (int k = 0; k < 4; ++k) {
+            const float v = rt * 16 + g * 4 + k < rank ? s[k] * f : 0.0f;
+            const uint32_t top = __float_as_uint(v) & 0xffff0000u, rest = pack_half_words<IC_DTYPE_BF16>(v - __uint_as_float(top), 0.0f);
+            hi[k >> 1] |= top >> (16 * (1 - (k & 1)));
+            lo[k >> 1] |= rest << (16 * (k & 1));
+        }
+        uint16_t* to = t + ((int64_t)m * parts + rt / 2) * 64 + rt % 2 * 16 + g * 4;
+        *reinterpret_cast<lb_u32x2*>(to) = lb_u32x2{hi[0], hi[1]};
+        *reinterpret_cast<lb_u32x2*>(to + kRankPart) = lb_u32x2{lo[0], lo[1]};
+        if (rt == rts - 1 && rts % 2) {                // the rest of the last part
+            *reinterpret_cast<lb_u32x2*>(to + 16) = lb_u32x2{0, 0};
+            *reinterpret_cast<lb_u32x2*>(to + kRankPart + 16) = lb_u32x2{0, 0};
+        }
     }
 }
 
@@ -134,18 +163,18 @@ int launch_shrink(const Adapted& ad, const int8_t* a, int64_t ld_a, const float*
     const int64_t tiles = cdiv(K, kActPad) * 2;
     auto go = [&](auto dt, auto mt, auto rt) {
         constexpr int MT = decltype(mt)::value, RT = decltype(rt)::value;
-        const dim3 grid((unsigned)(most_tiles(M, ad.adapters, 16 * MT) * cdiv(ad.rank / 16, RT)));
+        const dim3 grid((unsigned)(most_tiles(M, ad.adapters, 16 * MT) * cdiv(down_tiles(rank), RT)));
         hipLaunchKernelGGL((shrink_kernel<decltype(dt)::value, MT, RT>), grid, dim3(512), 0, st, a, ld_a, sa, (int)M, d, tiles, rank, ad.adapters,
                            scaling, offsets, order, ad.t);
     };
     auto shape = [&](auto dt) {
         typedef std::integral_constant<int, 1> one;
         if (M <= 1024) go(dt, one{}, one{});
-        else if (ad.rank <= 16) go(dt, std::integral_constant<int, 2>{}, one{});
-        else if (ad.rank <= 32) go(dt, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+        else if (rank <= 16) go(dt, std::integral_constant<int, 2>{}, one{});
+        else if (rank <= 32) go(dt, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
         else go(dt, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
     };
-    if (ad.f16) shape(std::integral_constant<int, IC_DTYPE_F16>{});
+    if (ad.planes == 2) shape(std::integral_constant<int, IC_DTYPE_F16>{});
     else shape(std::integral_constant<int, IC_DTYPE_BF16>{});
     IC_CHECK_LAUNCH();
     return IC_OK;
@@ -157,32 +186,34 @@ using namespace icq;
 
 extern "C" int64_t ic_adapter_down_bytes(int64_t adapters, int rank, int64_t K) {
     if (adapters < 0 || rank < 1 || rank > kMaxRank || K < 0) return 0;
-    return adapters * padded_rank(rank) * cdiv(K, kActPad) * kActPad * 2;
+    return adapters * down_tiles(rank) * 16 * cdiv(K, kActPad) * kActPad * 2;
 }
 
-extern "C" int64_t ic_adapter_up_bytes(int64_t adapters, int64_t N, int rank) {
-    if (adapters < 0 || rank < 1 || rank > kMaxRank || N < 0) return 0;
-    return adapters * N * padded_rank(rank) * 2;
+extern "C" int64_t ic_adapter_up_bytes(int64_t adapters, int64_t N, int rank, int dtype) {
+    if (adapters < 0 || rank < 1 || rank > kMaxRank || N < 0 || (dtype != IC_DTYPE_BF16 && dtype != IC_DTYPE_F16)) return 0;
+    return adapters * cdiv(N, 16) * rank_parts(rank) * (dtype == IC_DTYPE_F16 ? 2048 : 1024);
 }
 
 extern "C" int64_t ic_adapted_linear_workspace_bytes(int64_t M, int rank) {
     if (M < 0 || rank < 1 || rank > kMaxRank) return 0;
-    return M * padded_rank(rank) * 4;
+    return (M + 1) * rank_parts(rank) * 128;
 }
 
-extern "C" int ic_adapter_pack(const void* a, const void* b, int64_t adapters, int rank, int64_t N, int64_t K, void* down, void* up,
+extern "C" int ic_adapter_pack(const void* a, const void* b, int dtype, int64_t adapters, int rank, int64_t N, int64_t K, void* down, void* up,
                                void* stream) {
     IC_REQUIRE(adapters >= 1 && rank >= 1 && N >= 1 && K >= 1, "ic_adapter_pack: sizes must be >= 1");
+    IC_REQUIRE(dtype == IC_DTYPE_BF16 || dtype == IC_DTYPE_F16, "ic_adapter_pack: adapters are bf16 or fp16");
     if (adapters > kMaxGroups || rank > kMaxRank || K > 65536 || N > kMaxRows)
         return fail(IC_ERR_RANGE, "ic_adapter_pack: at most 1024 adapters, rank 128, 65536 for K, 1048560 for N");
     IC_REQUIRE(a && b && down && up && aligned16(down) && aligned16(up), "ic_adapter_pack: null pointer, or results not 16-byte aligned");
-    const int64_t tiles = cdiv(K, kActPad) * 2, n = adapters * (padded_rank(rank) / 16) * tiles;
+    const int64_t tiles = cdiv(K, kActPad) * 2, n = adapters * down_tiles(rank) * tiles;
+    const int64_t u = adapters * cdiv(N, 16) * rank_parts(rank) * (dtype == IC_DTYPE_F16 ? 2 : 1);
+    if (u > 1 << 25) return fail(IC_ERR_RANGE, "ic_adapter_pack: b takes more than 2^25 KB");
     hipStream_t st = as_stream(stream);
     hipLaunchKernelGGL(pack_down_kernel, dim3((unsigned)cdiv(n, 4)), dim3(256), 0, st, static_cast<const uint16_t*>(a), adapters, rank, K,
                        static_cast<lb_u32x4*>(down), tiles);
-    const int64_t blocks = cdiv(adapters * N * padded_rank(rank), 256);
-    hipLaunchKernelGGL(pack_up_kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st, static_cast<const uint16_t*>(b),
-                       adapters * N, rank, static_cast<uint16_t*>(up));
+    hipLaunchKernelGGL(pack_up_kernel, dim3((unsigned)cdiv(u, 4)), dim3(256), 0, st, static_cast<const uint16_t*>(b), adapters, N, rank,
+                       dtype == IC_DTYPE_F16, static_cast<lb_u32x4*>(up));
     IC_CHECK_LAUNCH();
     return IC_OK;
 }

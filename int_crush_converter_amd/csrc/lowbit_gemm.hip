@@ -11,7 +11,7 @@
 //   grouped   rows of y are ordered by group, each group has a weight of its
 //             own, and row i of y may come from another row of x;
 //   adapted   y[m, n] += sum_r t[m, r] B_a[n, r], a the adapter of row m and
-//             t = scale_a A_a x in fp32 (adapters.hip).
+//             t = scale_a A_a x (adapters.hip).
 #include "common.hpp"
 #include "prof.hpp"
 #include "lowbit.hpp"
@@ -132,6 +132,11 @@ __device__ __forceinline__ lb_f32x4 mma_mx(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc,
 // The same products of 32 rows and 32 columns, with twice the operations an
 // instruction (a wave alone on its SIMD reaches 4.7 POP/s and 8.9 PFLOP/s with
 // these over the card, 2.9 and 5.1 with the smaller ones).
+template <typename T>
+__device__ __forceinline__ T mma32_ranks(lb_u32x4 w, lb_u32x4 x, T acc) {      // (acc: fp32 values)
+    return __builtin_bit_cast(T, __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lb_bf16x8, w), __builtin_bit_cast(lb_bf16x8, x),
+                                                                                     __builtin_bit_cast(lb_f32x16, acc), 0, 0, 0));
+}
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <int KIND> struct Acc32 { typedef i32x16 T; };
@@ -386,7 +391,10 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
     // BUF stages; two sets of scale words; a column's bias, scale and zero-point; a row's scale and code sum
     // (and a group's first row of tiles)
     constexpr int SCALES = BUF * STAGE, COLS = SCALES + 2 * S_WORDS, ROWS = COLS + BN * 3 / 4, GROUPS = ROWS + (KIND == kMx ? 0 : BM / 2);
-    __shared__ lb_u32x4 lds[GROUPS + (MODE == kGrouped ? kMaxGroups / 4 + 1 : 0)];
+    // (kAdapted: each row's adapter, and which of the adapters the rows have, a bit each, for two tiles in turn)
+    __shared__ lb_u32x4 lds[GROUPS + (MODE == kGrouped ? kMaxGroups / 4 + 1 : MODE == kAdapted ? BM / 4 + kMaxGroups / 64 : 0)];
+    int* const row_id = reinterpret_cast<int*>(lds + GROUPS);
+    unsigned* const present = reinterpret_cast<unsigned*>(lds + GROUPS + BM / 4);
     float* const col = reinterpret_cast<float*>(lds + COLS);
     float* const row = reinterpret_cast<float*>(lds + ROWS);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, r = lane & 31;
@@ -409,7 +417,8 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
 
     const int k_tiles = (int)cdiv(p.K, 128), words = (int)cdiv(p.K, 512);
     const int n_tiles = (int)cdiv(p.N, 16), m_tiles = (int)cdiv(p.M, 16);
-    const int stages = KIND == kInt8 ? (int)cdiv(p.K, 64) : k_tiles;
+    const int k_stages = KIND == kInt8 ? (int)cdiv(p.K, 64) : k_tiles;
+    int stages = k_stages;                                 // (kAdapted: and those of the adapters of the tile's rows)
     constexpr int W_STEP = 1024, X_STEP = KIND == kMx ? 1024 : KIND == kInt4 ? 128 : 64;
     const int w_pitch = k_tiles * (KIND == kInt8 ? 2048 : 1024);                  // bytes of a row of tiles
 
@@ -487,7 +496,49 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
     auto copy = [&](__amdgpu_buffer_rsrc_t from, int lane_off, int off, lb_u32x4* to) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, lane_off, off, 0, 0);
     };
+    // kAdapted.  Behind the stages of K come those of each adapter that the tile's rows have: an operand of t lies like one
+    // of the activations (INT4: 32 ranks of hi and of lo in a stage, INT8: of one of them), one of B like one of the
+    // weights.  Rows with another adapter or none take the row of zeros.  Fetched one after another: adapter `ad_now`,
+    // its stage `ad_stage`.
+    const int ad_stages = p.ad.parts * p.ad.planes * (KIND == kInt8 ? 2 : 1);
+    int ad_now = -1, ad_stage = 0, ad_set = 0;
+    auto next_adapter = [&]() {                            // the lowest in the set above ad_now (there is one)
+        const unsigned* set = present + ad_set * (kMaxGroups / 32);
+        const int at = ad_now + 1, l = lane & 31;
+        unsigned w = set[l];
+        w &= l < at >> 5 ? 0u : l == at >> 5 ? ~0u << (at & 31) : ~0u;
+        const int first = __builtin_ctzll(__ballot(w != 0));
+        ad_now = first * 32 + __builtin_ctz((unsigned)__builtin_amdgcn_readlane((int)w, first));
+    };
+    auto fetch_adapter = [&](int buf) {
+        if constexpr (MODE == kAdapted) {
+            if (ad_stage == 0) next_adapter();
+            lb_u32x4* to = lds + buf * STAGE + wave * 64;
+            const int half = KIND == kInt8 ? ad_stage & 1 : 0, tile_of = KIND == kInt8 ? ad_stage >> 1 : ad_stage;   // (tile_of: part and plane)
+            const int pitch = p.ad.parts * 128, from = tile_of / p.ad.planes * 128 + half * 64;
+            const int lane_row = KIND == kInt4 ? lane >> 3 : lane >> 2;
+            const int chunk = KIND == kInt4 ? (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4)) : (lane & 3) ^ (lane >> 4);
+            const __amdgpu_buffer_rsrc_t t_buf = buffer(p.ad.t);
+#pragma unroll
+            for (int i = 0; i < X_LOADS; ++i) {
+                const int at = (i * WAVES + wave) * (KIND == kInt4 ? 8 : 16) + lane_row;
+                copy(t_buf, (row_id[at] == ad_now ? row0 + at : (int)p.M) * pitch + chunk * 16, from, to + i * WAVES * 64);
+            }
+            const int nt = bn * (BN / 16), nl = n_tiles - 1 - nt, up_pitch = p.ad.parts * p.ad.planes * 1024;
+            const __amdgpu_buffer_rsrc_t up_buf = buffer(p.ad.up + ((int64_t)ad_now * n_tiles + nt) * up_pitch);
+#pragma unroll
+            for (int i = 0; i < W_LOADS; ++i) {
+                const int at = i * WAVES + wave < nl ? i * WAVES + wave : nl;
+                copy(up_buf, lane16, at * up_pitch + tile_of * 1024, to + (X_LOADS + i) * WAVES * 64);
+            }
+            ad_stage = ad_stage + 1 == ad_stages ? 0 : ad_stage + 1;
+        }
+    };
     auto fetch = [&](int t, int buf) {
+        if (MODE == kAdapted && t >= k_stages) {
+            fetch_adapter(buf);
+            return;
+        }
         lb_u32x4* to = lds + buf * STAGE + wave * 64;
         if constexpr (KIND == kMx) {
             if ((t & 3) == 0) {
@@ -513,7 +564,6 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
     // of 8 consecutive outputs.
     lb_u32x4 xv[2][FM], wv[2][FN];
     int xs[KIND == kMx ? FM : 1][2], ws[KIND == kMx ? FN : 1][2];
-    const int w_column = (r >> 4) * 16 + (r >> 2 & 1) * 8 + (r >> 3 & 1) * 4 + (r & 3);
     const int w_lane = (r >> 4) * 64 + h * 16 + (r >> 2 & 1) * 8 + (r >> 3 & 1) * 4 + (r & 3);
     auto read_x = [&](const lb_u32x4* s, lb_u32x4 (&to)[FM], int c) {
 #pragma unroll
@@ -559,9 +609,16 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
             }
         }
         if (p.bias) c_bias = load_as_f32(p.bias, p.bias_dtype, n);
+        if constexpr (MODE == kAdapted) {                  // (K has BUF - 1 stages at least; the set is read behind the next barrier)
+            int id = tid < BM && row0 + tid < row_end ? p.ad.ids[row0 + tid] : -1;
+            if (id >= p.ad.adapters) id = -1;
+            if (tid < BM) row_id[tid] = id;
+            ad_set ^= 1;
+            if (id >= 0) atomicOr(&present[ad_set * (kMaxGroups / 32) + (id >> 5)], 1u << (id & 31));
+        }
 #pragma unroll
         for (int b = 0; b < BUF - 1; ++b)
-            if (b < stages) fetch(b, b);
+            if (b < k_stages) fetch(b, b);
     };
     // in stage t, when this wave has read the last of it: stage t + 1 has landed, and all waves are done with stage t's
     // buffer.  Behind the last stage whatever the next buffer holds is read, and not used: no branch parts the reads
@@ -585,9 +642,51 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
         static_for<0, READS>(one);
     };
 
+    // y from the accumulated sum: INT4 operands are held as 16 q, and the shift is exact.  |zp| <= 2^7 and
+    // |sum| <= 2^23 for K <= 65536, so the 24-bit product is exact, and |sum_k a (q - zp)| < 2^31, so the
+    // difference is right even where a term has wrapped.
+    auto value = [&](auto s, float sw, float zero, float bias, float sa, float sum) {
+        if constexpr (KIND == kMx) return s + bias;
+        else {
+            const unsigned d = (unsigned)(KIND == kInt4 ? s >> 4 : s) - (unsigned)__mul24(__float_as_int(zero), __float_as_int(sum));
+            return (float)(int)d * (sa * sw) + bias;
+        }
+    };
+    // kAdapted: whole values in place of the sums, before the adapters' stages
+    auto whole_values = [&]() {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const float sa = row[wm * FM * 32 + i * 32 + r], sum = row[BM + wm * FM * 32 + i * 32 + r];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                f32x16 v;
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    const int c = wn * FN * 32 + j * 32 + (k >> 3) * 16 + h * 8 + (k & 7);
+                    const lb_f32x4 bias = *reinterpret_cast<const lb_f32x4*>(col + c), sw = *reinterpret_cast<const lb_f32x4*>(col + BN + c);
+                    const lb_f32x4 zero = *reinterpret_cast<const lb_f32x4*>(col + 2 * BN + c);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[k + e] = value(acc[i][j][k + e], sw[e], zero[e], bias[e], sa, sum);
+                }
+                acc[i][j] = __builtin_bit_cast(acc_t, v);
+            }
+        }
+    };
+
+    if constexpr (MODE == kAdapted) {
+        if (threadIdx.x < kMaxGroups / 16) present[threadIdx.x] = 0;
+        lds_barrier();
+    }
     start();
     meet<0>();
     for (;;) {
+        if constexpr (MODE == kAdapted) {
+            const int own = lane < 32 ? __builtin_popcount(present[ad_set * (kMaxGroups / 32) + lane]) : 0;
+            stages = k_stages + __builtin_amdgcn_readlane(wave_scan(own), 63) * ad_stages;
+            ad_now = -1;
+            ad_stage = 0;
+            if (threadIdx.x < kMaxGroups / 32) present[(ad_set ^ 1) * (kMaxGroups / 32) + threadIdx.x] = 0;      // for the next tile
+        }
         if (threadIdx.x < BN) {
             col[threadIdx.x] = c_bias;
             if (KIND != kMx) {
@@ -606,14 +705,19 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
         buf = 0;
         if constexpr (KIND == kInt4) {
             // four sets a stage: the low nibbles of both words of weights, then the high ones
-            auto stage = [&](int t, auto first_) {
-                constexpr bool FIRST = decltype(first_)::value;
+            auto stage = [&](int t, auto first_, auto of_k) {
+                constexpr bool FIRST = decltype(first_)::value, OF_K = decltype(of_k)::value;
                 auto products = [&](int word, bool high, const lb_u32x4 (&x)[FM], bool fresh) {
 #pragma unroll
                     for (int j = 0; j < FN; ++j) {
-                        const lb_u32x4 w = high ? high_nibbles(wv[word][j]) : low_nibbles(wv[word][j]);
+                        if constexpr (OF_K) {
+                            const lb_u32x4 w = high ? high_nibbles(wv[word][j]) : low_nibbles(wv[word][j]);
 #pragma unroll
-                        for (int i = 0; i < FM; ++i) acc[i][j] = mma32_i8(w, x[i], fresh ? acc_t{} : acc[i][j]);
+                            for (int i = 0; i < FM; ++i) acc[i][j] = mma32_i8(w, x[i], fresh ? acc_t{} : acc[i][j]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < FM; ++i) acc[i][j] = mma32_ranks(wv[word][j], x[i], acc[i][j]);
+                        }
                     }
                 };
                 const lb_u32x4* here = lds + buf * STAGE;
@@ -635,14 +739,19 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
                 products(1, true, xv[1], false);
                 interleave(std::integral_constant<int, FM + FN>{});
             };
-            stage(0, std::true_type{});
+            stage(0, std::true_type{}, std::true_type{});
 #pragma unroll 1
-            for (int t = 1; t < stages; ++t) stage(t, std::false_type{});
+            for (int t = 1; t < k_stages; ++t) stage(t, std::false_type{}, std::true_type{});
+            if constexpr (MODE == kAdapted) {
+                whole_values();
+#pragma unroll 1
+                for (int t = k_stages; t < stages; ++t) stage(t, std::false_type{}, std::false_type{});
+            }
         } else {
             // (stage t with t % 4 = B: the byte of its scales)
-            auto stage = [&](int t, auto byte, auto first_) {
+            auto stage = [&](int t, auto byte, auto first_, auto of_k) {
                 constexpr int B = decltype(byte)::value;
-                constexpr bool FIRST = decltype(first_)::value;
+                constexpr bool FIRST = decltype(first_)::value, OF_K = decltype(of_k)::value;
                 auto products = [&](auto set, bool fresh) {
                     constexpr int C = decltype(set)::value;
 #pragma unroll
@@ -651,6 +760,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
                         for (int i = 0; i < FM; ++i) {
                             const acc_t a = fresh ? acc_t{} : acc[i][j];
                             if constexpr (KIND == kMx) acc[i][j] = mma32_mx<B>(wv[C][j], xv[C][i], a, ws[j][C], xs[i][C]);
+                            else if constexpr (!OF_K) acc[i][j] = mma32_ranks(wv[C][j], xv[C][i], acc[i][j]);
                             else acc[i][j] = mma32_i8(wv[C][j], xv[C][i], a);
                         }
                 };
@@ -667,18 +777,23 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
                 products(std::integral_constant<int, 1>{}, false);
                 interleave(std::integral_constant<int, FM + FN>{});
             };
-            stage(0, std::integral_constant<int, 0>{}, std::true_type{});
+            stage(0, std::integral_constant<int, 0>{}, std::true_type{}, std::true_type{});
             if constexpr (KIND == kMx) {
 #pragma unroll 1
                 for (int t = 1; t < stages; t += 4) {
-                    stage(t, std::integral_constant<int, 1>{}, std::false_type{});
-                    if (t + 1 < stages) stage(t + 1, std::integral_constant<int, 2>{}, std::false_type{});
-                    if (t + 2 < stages) stage(t + 2, std::integral_constant<int, 3>{}, std::false_type{});
-                    if (t + 3 < stages) stage(t + 3, std::integral_constant<int, 0>{}, std::false_type{});
+                    stage(t, std::integral_constant<int, 1>{}, std::false_type{}, std::true_type{});
+                    if (t + 1 < stages) stage(t + 1, std::integral_constant<int, 2>{}, std::false_type{}, std::true_type{});
+                    if (t + 2 < stages) stage(t + 2, std::integral_constant<int, 3>{}, std::false_type{}, std::true_type{});
+                    if (t + 3 < stages) stage(t + 3, std::integral_constant<int, 0>{}, std::false_type{}, std::true_type{});
                 }
             } else {
 #pragma unroll 1
-                for (int t = 1; t < stages; ++t) stage(t, std::integral_constant<int, 1>{}, std::false_type{});
+                for (int t = 1; t < k_stages; ++t) stage(t, std::integral_constant<int, 1>{}, std::false_type{}, std::true_type{});
+                if constexpr (MODE == kAdapted) {
+                    whole_values();
+#pragma unroll 1
+                    for (int t = k_stages; t < stages; ++t) stage(t, std::integral_constant<int, 1>{}, std::false_type{}, std::false_type{});
+                }
             }
         }
 
@@ -687,33 +802,6 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
         const bool whole = p.wide && p.out_dtype != IC_DTYPE_F32 && row0 + BM <= m_end && (bn + 1) * BN <= p.N;
         tile += gridDim.x >> 3;
         const bool more = tile < last;                     // (all waves are done with the buffers)
-        // y from the accumulated sum: INT4 operands are held as 16 q, and the shift is exact.  |zp| <= 2^7 and
-        // |sum| <= 2^23 for K <= 65536, so the 24-bit product is exact, and |sum_k a (q - zp)| < 2^31, so the
-        // difference is right even where a term has wrapped.
-        auto value = [&](auto s, float sw, float zero, float bias, float sa, float sum) {
-            if constexpr (KIND == kMx) return s + bias;
-            else {
-                const unsigned d = (unsigned)(KIND == kInt4 ? s >> 4 : s) - (unsigned)__mul24(__float_as_int(zero), __float_as_int(sum));
-                return (float)(int)d * (sa * sw) + bias;
-            }
-        };
-        // block (i, j) as whole values with their adapters' part, in place of its sums
-        auto adapted = [&](int i, int j, int m0, int n0, int m_end) {
-            const float sa = row[wm * FM * 32 + i * 32 + r], sum = row[BM + wm * FM * 32 + i * 32 + r];
-            f32x16 v;
-#pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-                const int c = wn * FN * 32 + j * 32 + (k >> 3) * 16 + h * 8 + (k & 7);
-                const lb_f32x4 bias = *reinterpret_cast<const lb_f32x4*>(col + c), sw = *reinterpret_cast<const lb_f32x4*>(col + BN + c);
-                const lb_f32x4 zero = *reinterpret_cast<const lb_f32x4*>(col + 2 * BN + c);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[k + e] = value(acc[i][j][k + e], sw[e], zero[e], bias[e], sa, sum);
-            }
-            const int m = m0 + i * 32 + r;
-            add_adapters(p.ad, p.N, m < m_end ? m : m_end - 1, n0 + j * 32 + w_column, h, v);
-            acc[i][j] = __builtin_bit_cast(acc_t, v);
-            __builtin_amdgcn_sched_barrier(0);
-        };
         if (p.wide) {
             if (more) start();
             // 32 rows of 128 bytes at a time through the wave's part of the last buffer, so that 8 lanes store a line;
@@ -740,7 +828,6 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
                 const float sa = KIND == kMx ? 0.0f : row[rw + i * 32 + r], sum = KIND == kMx ? 0.0f : row[BM + rw + i * 32 + r];
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
-                    if constexpr (MODE == kAdapted) adapted(i, j, m0, n0, m_end);
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         lb_f32x4 v[2];
@@ -790,7 +877,6 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
             for (int i = 0; i < FM; ++i) {
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
-                    if constexpr (MODE == kAdapted) adapted(i, j, m0, n0, m_end);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         *reinterpret_cast<sum4_t*>(area + r * PITCH + j * 32 + (k >> 1) * 16 + h * 8 + (k & 1) * 4) =
@@ -904,9 +990,12 @@ int linear_form(int kind, int64_t M, int64_t N) {      // 0, 128 or 256
 
 template <int KIND, int MODE = kPlain>
 int launch_linear(const Operands& p, hipStream_t st) {
-    const int form = linear_form(KIND, p.M, p.N);
-    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, KIND == kInt4 ? 3 : 4, MODE>(p, st);
-    else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, KIND == kInt4 ? 3 : 4, MODE>(p, st);
+    constexpr int BUF = KIND == kInt4 ? 3 : 4;
+    int form = linear_form(KIND, p.M, p.N);
+    // (a tile's adapters are known when BUF - 1 stages of it have been asked for)
+    if (MODE == kAdapted && cdiv(p.K, KIND == kInt8 ? 64 : 128) < BUF - 1) form = 0;
+    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, BUF, MODE>(p, st);
+    else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, BUF, MODE>(p, st);
     else if constexpr (MODE == kPlain) {
         if (p.M <= 16) launch_direct<KIND, 1>(p, st);
         else if (p.M <= 32) launch_direct<KIND, 2>(p, st);
@@ -1101,7 +1190,7 @@ extern "C" int ic_adapted_linear(const int8_t* a, int64_t ld_a, const float* sa,
     IC_REQUIRE(aligned16(down) && aligned16(up) && aligned16(workspace), "ic_adapted_linear: adapters and workspace need 16-byte alignment");
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 2.0 * M * N * K + 2.0 * M * rank * (N + K), (double)M * K + (double)N * K * bits / 8);
-    p.ad = Adapted{ids, static_cast<float*>(workspace), static_cast<const uint16_t*>(up), adapter_dtype == IC_DTYPE_F16, padded_rank(rank), (int)adapters};
+    p.ad = Adapted{ids, static_cast<uint16_t*>(workspace), static_cast<const uint8_t*>(up), adapter_dtype == IC_DTYPE_F16 ? 2 : 1, rank_parts(rank), (int)adapters};
     if (const int rc = launch_shrink(p.ad, a, ld_a, sa, M, K, down, rank, scaling, offsets, order, st)) return rc;
     return bits == 8 ? launch_linear<kInt8, kAdapted>(p, st) : launch_linear<kInt4, kAdapted>(p, st);
 }

@@ -124,7 +124,7 @@ def quantized_linear(x: QuantizedActivations, weight: QuantizedWeight, bias: tor
                          f"{rows} rows with one among {ad.count} adapters")
     nat.stream_for(ad.down, ad.up, ad.scaling, groups.data)
     out = torch.empty((*x.lead, N), dtype=out_dtype, device=data.device)
-    ws = torch.empty((rows, -(-ad.rank // 16) * 16), dtype=torch.float32, device=data.device)
+    ws = torch.empty((rows + 1) * -(-ad.rank // 32) * 32, dtype=torch.float32, device=data.device)    # ic_adapted_linear_workspace_bytes
     ids, offsets, order, _ = groups.pointers()
     call("ic_adapted_linear", data.data_ptr(), data.shape[1], m, m + 4 * rows, rows, w.tiles.data_ptr(), w.bits,
          w.scales.data_ptr(), w.scale_kind, None if z is None else z.data_ptr(), None if b is None else b.data_ptr(),

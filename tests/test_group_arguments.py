@@ -152,6 +152,11 @@ def test_refused_adapters(calls):
     for n, r, N, K in ((0, 4, 16, 64), (2, 0, 16, 64), (2, 129, 16, 64), (2, 4, 16, 0), (2, 4, 16, 65537), (2, 4, 0, 64), (1025, 1, 1, 1)):
         with pytest.raises(ValueError, match="adapters of rank"):
             icq.LowRankAdapters(torch.zeros(n, r, K, dtype=BF16), torch.zeros(n, N, r, dtype=BF16))
+    for value in (float("nan"), float("inf")):
+        odd = ok_b.clone()
+        odd[1, 3, 2] = value
+        with pytest.raises(ValueError, match="Inf or NaN"):
+            icq.LowRankAdapters(ok_a, odd)
     with pytest.raises(ValueError, match="scalings"):
         icq.LowRankAdapters(ok_a, ok_b, torch.ones(3))
     w, ad = weight(16, 64), adapter(2, 4, 16, 64)
@@ -192,9 +197,10 @@ def test_sizes_of_the_library(L):
     assert L.ic_group_workspace_bytes(10, 1025) == 0
     for rows in (1, 16, 17, 4000, 4096, 4097, 8191, 100000, 1048560):
         assert L.ic_group_workspace_bytes(rows, 7) <= 4 * groups.RowGroups._empty(rows, 1, 7, torch.device("cpu")).scratch
-    assert L.ic_adapter_down_bytes(3, 12, 130) == 3 * 16 * 256 * 2 and L.ic_adapter_up_bytes(3, 10, 17) == 3 * 10 * 32 * 2
-    assert L.ic_adapted_linear_workspace_bytes(7, 12) == 7 * 16 * 4
-    assert L.ic_adapter_up_bytes(1024, 1048560, 128) == 1024 * 1048560 * 128 * 2              # past 32 bits
+    assert L.ic_adapter_down_bytes(3, 12, 130) == 3 * 16 * 256 * 2 and L.ic_adapter_up_bytes(3, 17, 33, 1) == 3 * 2 * 2 * 1024
+    assert L.ic_adapter_up_bytes(3, 17, 33, 2) == 3 * 2 * 2 * 2048 and L.ic_adapter_up_bytes(3, 17, 33, 0) == 0
+    assert L.ic_adapted_linear_workspace_bytes(7, 12) == 8 * 128
+    assert L.ic_adapter_up_bytes(1024, 1048560, 128, 1) == 1024 * 1048560 * 128 * 2           # past 32 bits
 
 
 def test_refusals_of_the_library(L):
@@ -227,8 +233,9 @@ def test_refusals_of_the_library(L):
                                          k.get("ws", one), one, 1, k.get("ldo", 8), None)
     assert ad(down=None) == -1 and ad(dtype=0) == -1 and ad(n=0) == -1 and ad(n=1025) == -1 and ad(rank=0) == -1 and ad(rank=129) == -1
     assert ad(ids=None) == -1 and ad(ws=None) == -1 and ad(ws=ctypes.c_void_p(8)) == -1 and ad(ldo=7) == -1 and ad(M=0) == 0
-    pack = lambda **k: L.ic_adapter_pack(k.get("a", one), one, k.get("n", 2), k.get("rank", 4), k.get("N", 8), k.get("K", 8), one,             # noqa: E731
+    pack = lambda **k: L.ic_adapter_pack(k.get("a", one), one, k.get("dtype", 1), k.get("n", 2), k.get("rank", 4), k.get("N", 8), k.get("K", 8), one,             # noqa: E731
                                          k.get("up", one), None)
     assert pack(a=None) == -1 and pack(n=0) == -1 and pack(K=0) == -1 and pack(up=ctypes.c_void_p(8)) == -1
+    assert pack(dtype=0) == -1 and pack(n=1024, N=1048560) == -3
     assert pack(n=1025) == -3 and pack(rank=129) == -3 and pack(K=65537) == -3
     assert L.ic_expert_form(4, -1, 4, 8) == -1 and L.ic_expert_form(4, 4, 0, 8) == -1 and L.ic_expert_form(3, 4, 4, 8) == -1
