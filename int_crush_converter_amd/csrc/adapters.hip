@@ -78,19 +78,21 @@ __device__ __forceinline__ lb_f32x4 mma16(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc) 
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lb_bf16x8, w), __builtin_bit_cast(lb_bf16x8, x), acc, 0, 0, 0);
 }
 
-// A work-group of 8 waves takes 16 RT ranks and 16 MT rows of one adapter, its
+// A work-group takes 16 RT ranks and 16 MT rows of one adapter, its
 // waves a share of K each; the sums are joined in LDS in a fixed order.
-template <int DT, int MT, int RT>
-__global__ __launch_bounds__(512) void shrink_kernel(const int8_t* __restrict__ a, int64_t ld_a, const float* __restrict__ sa, int M,
+template <int DT, int MT, int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const int8_t* __restrict__ a, int64_t ld_a, const float* __restrict__ sa, int M,
                                                      const lb_u32x4* __restrict__ down, int64_t tiles, int rank, int adapters,
                                                      const float* __restrict__ scaling, const int32_t* __restrict__ offsets,
                                                      const int32_t* __restrict__ order, uint16_t* __restrict__ t) {
-    constexpr int WAVES = 8;
     __shared__ lb_f32x4 part[WAVES][MT * RT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
-    const int parts = rank_parts(rank), rts = down_tiles(rank), groups = (rts + RT - 1) / RT, rt0 = blockIdx.x % groups * RT;
+    const int parts = rank_parts(rank), rts = down_tiles(rank), groups = (rts + RT - 1) / RT;
+    // work-groups are dealt to the 8 XCDs in turn: each gets one run of rows, whose adapter its L2 keeps
+    const int per = gridDim.x >> 3, extra = gridDim.x & 7, xcd = blockIdx.x & 7;
+    const int at_run = xcd * per + (xcd < extra ? xcd : extra) + (blockIdx.x >> 3), rt0 = at_run % groups * RT;
     if (blockIdx.x == 0 && threadIdx.x < parts * 64) t[(int64_t)M * parts * 64 + threadIdx.x] = 0;       // the row of zeros
-    const GroupTile tile = find_tile(offsets, adapters, M, 16 * MT, blockIdx.x / groups);
+    const GroupTile tile = find_tile(offsets, adapters, M, 16 * MT, at_run / groups);
     if (tile.group < 0) return;
     auto row_of = [&](int i) {             // (rows past the last repeat the last)
         const int at = tile.first + i * 16 + r < tile.end ? tile.first + i * 16 + r : tile.end - 1, m = order[at];
@@ -161,18 +163,25 @@ int launch_shrink(const Adapted& ad, const int8_t* a, int64_t ld_a, const float*
                   const float* scaling, const int32_t* offsets, const int32_t* order, hipStream_t st) {
     const lb_u32x4* d = static_cast<const lb_u32x4*>(down);
     const int64_t tiles = cdiv(K, kActPad) * 2;
-    auto go = [&](auto dt, auto mt, auto rt) {
-        constexpr int MT = decltype(mt)::value, RT = decltype(rt)::value;
+    auto go = [&](auto dt, auto mt, auto rt, auto waves) {
+        constexpr int MT = decltype(mt)::value, RT = decltype(rt)::value, WAVES = decltype(waves)::value;
         const dim3 grid((unsigned)(most_tiles(M, ad.adapters, 16 * MT) * cdiv(down_tiles(rank), RT)));
-        hipLaunchKernelGGL((shrink_kernel<decltype(dt)::value, MT, RT>), grid, dim3(512), 0, st, a, ld_a, sa, (int)M, d, tiles, rank, ad.adapters,
-                           scaling, offsets, order, ad.t);
+        hipLaunchKernelGGL((shrink_kernel<decltype(dt)::value, MT, RT, WAVES>), grid, dim3(64 * WAVES), 0, st, a, ld_a, sa, (int)M, d, tiles, rank,
+                           ad.adapters, scaling, offsets, order, ad.t);
     };
     auto shape = [&](auto dt) {
-        typedef std::integral_constant<int, 1> one;
-        if (M <= 1024) go(dt, one{}, one{});
-        else if (rank <= 16) go(dt, std::integral_constant<int, 2>{}, one{});
-        else if (rank <= 32) go(dt, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
-        else go(dt, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+        typedef std::integral_constant<int, 1> c1;
+        typedef std::integral_constant<int, 2> c2;
+        typedef std::integral_constant<int, 3> c3;
+        typedef std::integral_constant<int, 4> c4;
+        typedef std::integral_constant<int, 8> c8;
+        if (M <= 1024) return go(dt, c1{}, c1{}, std::integral_constant<int, 16>{});
+        // 32 or 48 rows: what takes fewer rounds of the CUs for its height
+        auto cost = [&](int mt) { return mt * cdiv(most_tiles(M, ad.adapters, 16 * mt) * cdiv(rank, 64), 256); };
+        const bool high = cost(3) < cost(2);
+        if (rank <= 16) high ? go(dt, c3{}, c1{}, c8{}) : go(dt, c2{}, c1{}, c8{});
+        else if (rank <= 32) high ? go(dt, c3{}, c2{}, c8{}) : go(dt, c2{}, c2{}, c8{});
+        else high ? go(dt, c3{}, c4{}, c8{}) : go(dt, c2{}, c4{}, c8{});
     };
     if (ad.planes == 2) shape(std::integral_constant<int, IC_DTYPE_F16>{});
     else shape(std::integral_constant<int, IC_DTYPE_BF16>{});

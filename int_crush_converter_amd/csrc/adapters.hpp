@@ -23,6 +23,7 @@ struct Adapted {
     uint16_t* t;             // [M + 1, parts, 64]
     const uint8_t* up;
     int planes, parts, adapters;
+    int eights;              // of ranks that are not all padding
 };
 
 // t for every row that has an adapter.
@@ -42,7 +43,8 @@ __device__ __forceinline__ lb_f32x4 adapter_dot4(const Adapted& ad, int64_t N, i
     if (id < 0 || id >= ad.adapters) return s;
     const lb_u32x4* t = reinterpret_cast<const lb_u32x4*>(ad.t + m * ad.parts * 64);
     const lb_u32x4* b = reinterpret_cast<const lb_u32x4*>(ad.up + (id * cdiv(N, 16) + n / 16) * (ad.parts * ad.planes) * 1024) + n % 16;
-    for (int c = 0; c < ad.parts * 4; ++c) {
+#pragma unroll 2
+    for (int c = 0; c < ad.eights; ++c) {
         const lb_u32x4 hi = t[(c >> 2) * 8 + (c & 3)], lo = t[(c >> 2) * 8 + (c & 3) + 4];
         float v[8];
 #pragma unroll

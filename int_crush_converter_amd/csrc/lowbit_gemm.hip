@@ -290,6 +290,16 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
         }
     };
     if (t0 < t1) load(t0);
+    // the adapters' part of the wave's outputs, whose loads wait together with the first of the product
+    constexpr int OWN = (MT * NT + WAVES - 1) / WAVES;
+    lb_f32x4 added[OWN];
+    if constexpr (MODE == kAdapted) {
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            const int u = wave + k * WAVES, m = m0 + u / NT * 16 + r, n = (nt0 + u % NT) * 16 + g * 4;
+            added[k] = u < MT * NT && m < m_end && n < p.N ? adapter_dot4(p.ad, p.N, m, n) : lb_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
     for (int k = threadIdx.x; k < MT * NT * 256; k += 64 * WAVES) (&sum[0][0][0])[k] = 0;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -325,7 +335,10 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) atomicAdd(&sum[i * NT + j][k][lane], acc[i][j][k]);
     __syncthreads();
-    for (int u = wave; u < MT * NT; u += WAVES) {
+#pragma unroll
+    for (int own = 0; own < OWN; ++own) {
+        const int u = wave + own * WAVES;
+        if (u >= MT * NT) break;
         const int i = u / NT, j = u % NT, m = m0 + i * 16 + r, n = (nt0 + j) * 16 + g * 4;
         if (m >= m_end || n >= p.N) continue;
         Columns<KIND> cols;
@@ -333,7 +346,7 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
         const int from = source_row<MODE>(p, m);
         const i32x4 s = {sum[u][0][lane], sum[u][1][lane], sum[u][2][lane], sum[u][3][lane]};
         lb_f32x4 y = cols.finish(s, p.sa[from], p.zp ? p.sums[from] : 0);
-        if constexpr (MODE == kAdapted) y += adapter_dot4(p.ad, p.N, m, n);
+        if constexpr (MODE == kAdapted) y += added[own];
         store4(p, y, m, n, m_end);
     }
 }
@@ -654,17 +667,24 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
     };
     // kAdapted: whole values in place of the sums, before the adapters' stages
     auto whole_values = [&]() {
+        // (two addresses, made here: the compiler would keep 80 of them over the K loop, spilled)
+        const float* my_col = col + wn * FN * 32 + h * 8;
+        const float* my_row = row + wm * FM * 32 + r;
+        int at_col = (int)(my_col - reinterpret_cast<const float*>(lds)), at_row = (int)(my_row - reinterpret_cast<const float*>(lds));
+        asm volatile("" : "+v"(at_col), "+v"(at_row));
+        my_col = reinterpret_cast<const float*>(lds) + at_col;
+        my_row = reinterpret_cast<const float*>(lds) + at_row;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            const float sa = row[wm * FM * 32 + i * 32 + r], sum = row[BM + wm * FM * 32 + i * 32 + r];
+            const float sa = my_row[i * 32], sum = my_row[BM + i * 32];
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 f32x16 v;
 #pragma unroll
                 for (int k = 0; k < 16; k += 4) {
-                    const int c = wn * FN * 32 + j * 32 + (k >> 3) * 16 + h * 8 + (k & 7);
-                    const lb_f32x4 bias = *reinterpret_cast<const lb_f32x4*>(col + c), sw = *reinterpret_cast<const lb_f32x4*>(col + BN + c);
-                    const lb_f32x4 zero = *reinterpret_cast<const lb_f32x4*>(col + 2 * BN + c);
+                    const float* c = my_col + j * 32 + (k >> 3) * 16 + (k & 7);
+                    const lb_f32x4 bias = *reinterpret_cast<const lb_f32x4*>(c), sw = *reinterpret_cast<const lb_f32x4*>(c + BN);
+                    const lb_f32x4 zero = *reinterpret_cast<const lb_f32x4*>(c + 2 * BN);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[k + e] = value(acc[i][j][k + e], sw[e], zero[e], bias[e], sa, sum);
                 }
@@ -1190,7 +1210,8 @@ extern "C" int ic_adapted_linear(const int8_t* a, int64_t ld_a, const float* sa,
     IC_REQUIRE(aligned16(down) && aligned16(up) && aligned16(workspace), "ic_adapted_linear: adapters and workspace need 16-byte alignment");
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 2.0 * M * N * K + 2.0 * M * rank * (N + K), (double)M * K + (double)N * K * bits / 8);
-    p.ad = Adapted{ids, static_cast<uint16_t*>(workspace), static_cast<const uint8_t*>(up), adapter_dtype == IC_DTYPE_F16 ? 2 : 1, rank_parts(rank), (int)adapters};
+    p.ad = Adapted{ids, static_cast<uint16_t*>(workspace), static_cast<const uint8_t*>(up), adapter_dtype == IC_DTYPE_F16 ? 2 : 1, rank_parts(rank), (int)adapters,
+                   (rank + 7) / 8};
     if (const int rc = launch_shrink(p.ad, a, ld_a, sa, M, K, down, rank, scaling, offsets, order, st)) return rc;
     return bits == 8 ? launch_linear<kInt8, kAdapted>(p, st) : launch_linear<kInt4, kAdapted>(p, st);
 }
