@@ -1032,41 +1032,50 @@ int launch_linear(const Operands& p, hipStream_t st) {
 
 // Which form a grouped product takes.  The groups' sizes are on the GPU, so it
 // goes by their average, and by whether a row of 64 x 256 tiles of every group
-// fills the CUs (`many`).  Measured, weights from HBM, rows spread at random
-// over 8 (few) and 64 groups (many) of 2816 x 4096 (us):
-//                            wide      32 x 128   64 x 256   128 x 128   256 x 256
-//   INT4   8 groups,   1 row a group   10.3       16.6       24.5        25.1        53
-//                      4               14.6       19.1       25.9        26.6        53
-//                     16               17.9       19.1       26.1        26.6        53
-//                     64               31.8       22.4       26.3        26.7        53
-//                    128               50.8       38.0       28.4        29.2        53
-//   INT4  64 groups,   1               44.0       53.9       48.6        70.6       109
-//                      4               74.7       72.5       77.0        112        163
-//                     16               97.0       75.5       79.1        114        166
-//                     32              135.6      100.6       80.7        116        168
-//                    128               316        240        141         167        185
-//                    256                                     246         261        293
-//                   1024                                     851         873        790
-//   INT8   8 groups,  16               26.9       25.3       36.9        29.4        53
-//                     32               31.2       25.7       38.2        30.1        54
-//                     64               43.5       35.5       39.8        31.4        53
-//                   1024                                     142         135         124
-//   INT8  64 groups,   4              124        128        128         140         184
-//                     16              149        135        133         144         188
-//                     64              308        230        173         162         197
-//                    128              521        350        218         244         204
-//                   1024                                    1155        1165         848
+// that can have rows fills the CUs (`many`).  Measured, weights from HBM, rows
+// at random over 8 (few) and 64 groups (many), us:
+//                  2816 x 4096                              4096 x 1408
+//   rows a group   wide 16  wide 32  32x128  64x256  256^2  wide 16  wide 32  32x128  64x256  256^2
+//   INT4,  8,   1    10.9     11.8    17.6    25.3             8.7     11.2    11.1    14.8
+//               8    14.2     17.8    17.9    25.0             9.4     12.8    11.3    15.0
+//              16    14.6     18.3    17.9    25.4            11.6     13.0    11.4    15.1
+//              32    18.7     19.2    18.3    25.4            16.2     17.4    13.5    15.1
+//              64    28.5     30.0    22.3    25.7            25.1     25.8    14.3    16.1
+//             128                     36.2    27.0    54                       23.9    19.8    30
+//            1024                              112   120                               73     88
+//            2048                              218   193                              138    148
+//   INT4, 64,   1    47.7     61.6    56.2    50.0            31.5     56.8    30.7    33.8
+//               2    63.8     87.4    64.9    80.8            43.7     77.0    40.9    43.2
+//               4    73.8     96.9    71.3    78.8            51.4     90.7    51.7    45.7
+//              16    98.7    102.4    75.8    79.5            68.1     94.1    54.7    50.7
+//              64     197      207     136    97.4             162      198     103    67.9
+//             256                              248   267                              165    217
+//             512                              455   451                              304    313
+//            1024                              864   813                              572    576
+//                  wide 16  wide 32  128x128  256^2            wide 16  wide 32  128x128  256^2
+//   INT8,  8,   8    21.1     25.5    29.0                      13.4     15.6    16.4
+//              16    25.6     26.4    28.8                      15.3     15.9    17.1
+//              32    29.9     28.8    29.2                      20.4     20.5    16.7
+//              64    41.0     37.6    30.8                      32.0     29.6    17.6
+//             128                     36.9    55.7                               22.6   29.2
+//            1024                      139     129                               86.1   89.4
+//   INT8, 64,   1    85.7     86.9    96.0                      49.1     65.0    56.2
+//               4     124      133     137                      90.9      113    85.9
+//              16     147      148     145                       116      122    89.7
+//             128                      235     215                                143    147
+//             256                      355     327                                216    214
+//            1024                     1179     865                                678    571
 // Where 32 x 128 tiles would leave a third of the CUs idle, the wide form with
-// 32 rows: INT8 10 groups of 60 rows, 1000 x 2901, 15.1 against 16.8; INT4 one
-// group of 64 rows, 4096 x 4096, 8.1 against 16.8, 4096 x 12288 12.3 against
-// 35.5; of 8 groups of 32 rows, 2816 x 4096 (176 tiles) 23.9 against 22.2.
+// 32 rows: INT8 10 groups of 60 rows, 1000 x 2901, 15.1 against 21.9 (128 x 128);
+// INT4 one group of 64 rows, 4096 x 4096, 8.1 against 16.8, 4096 x 12288 12.3
+// against 35.5.
 int expert_form(int kind, int64_t rows, int64_t groups, int64_t N) {      // 1, 2 (wide, so many times 16 rows), 32, 64, 128 or 256
     const int64_t met = rows < groups ? rows : groups, each = met ? cdiv(rows, met) : 0;
     const bool many = met * cdiv(N, 256) >= 256;
-    if (each <= (many ? 4 : 12)) return 1;
+    if (each <= (many ? 2 : 16)) return 1;
     if (met * cdiv(each, 32) * cdiv(N, 128) < 170) return 2;
-    if (each <= (many ? 16 : kind == kInt8 ? 32 : 64)) return 32;
-    if (many && each >= (kind == kInt8 ? 128 : 768)) return 256;
+    if (kind == kInt4 && !many && each <= 64) return 32;
+    if (many && each >= (kind == kInt8 ? 128 : 1024)) return 256;
     return kind == kInt8 ? 128 : 64;
 }
 
@@ -1075,9 +1084,9 @@ int launch_experts(const Operands& p, hipStream_t st) {
     const int form = expert_form(KIND, p.M, p.groups, p.N);
     constexpr int BUF = KIND == kInt4 ? 3 : 4;
     if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, BUF, kGrouped>(p, st);
-    else if (form == 32) launch_tiled<KIND, 1, 2, 1, 2, BUF, kGrouped>(p, st);
-    else if (form > 32) {
+    else if (form >= 32) {
         if constexpr (KIND == kInt8) launch_tiled<KIND, 2, 2, 2, 2, BUF, kGrouped>(p, st);
+        else if (form == 32) launch_tiled<KIND, 1, 2, 1, 2, BUF, kGrouped>(p, st);
         else launch_tiled<KIND, 1, 4, 2, 2, BUF, kGrouped>(p, st);
     } else if (form == 2) launch_wide<KIND, 2, 2, kGrouped>(p, st);
     // four column tiles for INT4 where work-groups abound: 64 groups of 4096 x 1408, 1 row each, 35.4 against 40.3 us
