@@ -31,16 +31,15 @@ __device__ __forceinline__ float key_logit(unsigned k) { return k == 0xffffffffu
 // The choice of one token by one wave.  A lane has SLOTS consecutive experts and
 // sorts them, largest first and of equals the lowest, so that a choice is a
 // maximum over the lanes' first ones, and of lanes with that maximum the lowest.
-template <int DT, int SLOTS>
-__device__ __forceinline__ void choose(const void* logits, int64_t at, int experts, int top, int renormalize,
-                                       int& id, float& weight) {
+template <int SLOTS>
+__device__ __forceinline__ void choose(const float (&logit)[SLOTS], int top, int renormalize, int& id, float& weight) {
     const int lane = threadIdx.x & 63;
     unsigned key[SLOTS];
     int expert[SLOTS];
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {
         expert[i] = lane * SLOTS + i;
-        key[i] = expert[i] < experts ? logit_key(load_as_f32(logits, DT, at + expert[i])) : 0u;
+        key[i] = logit_key(logit[i]);
     }
 #pragma unroll
     for (int n = SLOTS - 1; n > 0; --n)
@@ -198,10 +197,20 @@ __global__ __launch_bounds__(kThreads) void route_kernel(const void* __restrict_
     count[tid] = 0;
     __syncthreads();
     const int64_t t0 = (int64_t)unit * tokens_per_unit, t1 = t0 + tokens_per_unit < tokens ? t0 + tokens_per_unit : tokens;
+    float next[SLOTS];                       // of the wave's next token
+    auto load = [&](int64_t t) {
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) next[i] = t < t1 && lane * SLOTS + i < u.groups ? load_as_f32(logits, DT, t * ld + lane * SLOTS + i) : -INFINITY;
+    };
+    load(t0 + (tid >> 6));
     for (int64_t t = t0 + (tid >> 6); t < t1; t += kThreads / 64) {
+        float logit[SLOTS];
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) logit[i] = next[i];
+        load(t + kThreads / 64);
         int id;
         float w;
-        choose<DT, SLOTS>(logits, t * ld, u.groups, top, renormalize, id, w);
+        choose<SLOTS>(logit, top, renormalize, id, w);
         if (lane < top) {
             ids[t * top + lane] = id;
             weights[t * top + lane] = w;
@@ -376,7 +385,9 @@ extern "C" int ic_group_rows(const void* given, int wide, int64_t rows, int64_t 
     IC_REQUIRE(offsets && (rows == 0 || (given && ids && order && position && workspace)), "ic_group_rows: null pointer");
     IC_REQUIRE(aligned16(workspace), "ic_group_rows: workspace not 16-byte aligned");
     hipStream_t st = as_stream(stream);
-    const int per = rows_per_unit(rows);
+    // up to 2048 pairs need no second launch (64 rows 5.2 us in a graph, 7.2 with two; a router's tokens do: a wave takes
+    // some microseconds for each, 64 tokens 9.5 us with two launches and 15.9 with one)
+    const int per = rows * per_row <= 2048 ? (int)(rows ? rows : 1) : rows_per_unit(rows);
     const int units = rows ? (int)cdiv(rows, per) : 1;
     ProfScope prof(st, PT_OTHER, 0.0, (wide ? 20.0 : 16.0) * rows * per_row);
     const Units u{rows * per_row, (int)(per * per_row), units, (int)groups, static_cast<uint16_t*>(workspace)};

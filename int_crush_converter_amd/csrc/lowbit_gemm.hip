@@ -1022,7 +1022,8 @@ int launch_linear(const Operands& p, hipStream_t st) {
         else launch_direct<KIND, 4>(p, st);
     } else {
         // (64 rows, INT4 12288 x 4096: 17.2 us with 2 x 2, 14.2 with 4 x 4; 4096 x 4096, 64 work-groups: 8.1 and 12.6)
-        if (p.M <= 16) launch_wide<KIND, 1, 2, MODE>(p, st);
+        if (p.M <= 16 && cdiv(p.N, 32) < 256) launch_wide<KIND, 1, 1, MODE>(p, st);
+        else if (p.M <= 16) launch_wide<KIND, 1, 2, MODE>(p, st);
         else if (p.M > 32 && cdiv(p.M, 64) * cdiv(p.N, 64) >= 128) launch_wide<KIND, 4, 4, MODE>(p, st);
         else launch_wide<KIND, 2, 2, MODE>(p, st);
     }

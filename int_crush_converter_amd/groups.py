@@ -47,14 +47,15 @@ class RowGroups:
         at, n = self.data.data_ptr() + 4 * self.scratch, 4 * self.rows * self.per_row
         return at, at + 3 * n, at + n, at + 2 * n
 
-    def _part(self, i: int) -> torch.Tensor:
-        at, n = self.scratch, self.rows * self.per_row
-        return self.data[at + i * n: at + (i + 1) * n]
+    def _part(self, i: int, flat: bool) -> torch.Tensor:
+        n = self.rows * self.per_row
+        shape, strides = ((n,), (1,)) if flat else ((self.rows, self.per_row), (self.per_row, 1))
+        return self.data.as_strided(shape, strides, self.scratch + i * n)
 
     @property
     def ids(self) -> torch.Tensor:
         """int32 [rows, per_row]: each pair's group, -1 for none."""
-        return self._part(0).view(self.rows, self.per_row)
+        return self._part(0, False)
 
     @property
     def offsets(self) -> torch.Tensor:
@@ -64,12 +65,12 @@ class RowGroups:
     @property
     def order(self) -> torch.Tensor:
         """int32 [rows * per_row]: the pair at each place, -1 behind the last group's."""
-        return self._part(1)
+        return self._part(1, True)
 
     @property
     def position(self) -> torch.Tensor:
         """int32 [rows, per_row]: each pair's place, -1 for none."""
-        return self._part(2).view(self.rows, self.per_row)
+        return self._part(2, False)
 
 
 def group_rows(ids: torch.Tensor, groups: int) -> RowGroups:
