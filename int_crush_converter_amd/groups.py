@@ -20,6 +20,10 @@ from .activations import as_rows, call
 MAX_GROUPS, MAX_CHOICES, MAX_PAIRS = 1024, 64, 1048560
 
 
+def _gpu(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_cuda else nat.to_gpu(t)          # (which GPU: nat.stream_for asks, of all operands at once)
+
+
 class RowGroups:
     """The (row, choice) pairs of a batch ordered by group, in int32 on the GPU; pair p is choice ``p % per_row`` of row
     ``p // per_row``.  Made by ``group_rows`` and ``route_tokens``."""
@@ -78,7 +82,7 @@ def group_rows(ids: torch.Tensor, groups: int) -> RowGroups:
     [0, groups) mean none: such pairs are in no group."""
     if ids.dim() not in (1, 2) or ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"expected int32 or int64 ids [rows] or [rows, per_row], got {ids.dtype} {tuple(ids.shape)}")
-    given = nat.on_gpu("ids", ids).contiguous()
+    given = _gpu(ids).contiguous()
     g = RowGroups._empty(ids.shape[0], ids.shape[1] if ids.dim() == 2 else 1, groups, given.device)
     to, offsets, order, position = g.pointers()
     call("ic_group_rows", given.data_ptr(), int(given.dtype == torch.int64), g.rows, g.per_row, groups, to, offsets, order,
@@ -99,7 +103,7 @@ def route_tokens(logits: torch.Tensor, top: int, *, renormalize: bool = True) ->
     tokens, experts = logits.shape
     if not 1 <= top <= experts:
         raise ValueError(f"top must be in [1, {experts}] (the experts), got {top}")
-    x = nat.on_gpu("logits", logits)
+    x = _gpu(logits)
     code = nat.dtype_code(x)
     g = RowGroups._empty(tokens, top, experts, x.device)
     x = as_rows(x) if tokens else x
@@ -107,7 +111,7 @@ def route_tokens(logits: torch.Tensor, top: int, *, renormalize: bool = True) ->
     ids, offsets, order, position = g.pointers()
     call("ic_route_tokens", x.data_ptr(), code, tokens, experts, x.stride(0) if tokens > 1 else experts, top,
          int(renormalize), ids, weights.data_ptr(), offsets, order, position, g.data.data_ptr(), nat.stream_for(x))
-    return g, weights
+    return g, weights if logits.is_cuda else weights.to(logits.device)
 
 
 def combine_experts(y: torch.Tensor, groups: RowGroups, weights: torch.Tensor, residual: torch.Tensor | None = None
@@ -121,14 +125,16 @@ def combine_experts(y: torch.Tensor, groups: RowGroups, weights: torch.Tensor, r
     cols = y.shape[1]
     if tuple(weights.shape) != (groups.rows, groups.per_row) or not weights.is_floating_point():
         raise ValueError(f"expected weights ({groups.rows}, {groups.per_row}), got {weights.dtype} {tuple(weights.shape)}")
-    yr = nat.on_gpu("y", y)
+    yr = _gpu(y)
     code = nat.dtype_code(yr)
-    w = nat.on_gpu("weights", weights).float().contiguous()
+    w = _gpu(weights)
+    if w.dtype != torch.float32 or not w.is_contiguous():
+        w = w.float().contiguous()
     r = None
     if residual is not None:
         if tuple(residual.shape) != (groups.rows, cols) or residual.dtype != y.dtype:
             raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} does not match ({groups.rows}, {cols}) {y.dtype}")
-        r = nat.on_gpu("residual", residual)
+        r = _gpu(residual)
     stream = nat.stream_for(yr, w, r, groups.data)
     if groups.rows:
         yr, r = as_rows(yr), None if r is None else as_rows(r)
@@ -136,4 +142,4 @@ def combine_experts(y: torch.Tensor, groups: RowGroups, weights: torch.Tensor, r
     call("ic_combine_rows", yr.data_ptr(), code, groups.rows, groups.per_row, cols, yr.stride(0) if pairs > 1 else cols,
          groups.pointers()[3], w.data_ptr(), None if r is None else r.data_ptr(),
          0 if r is None else r.stride(0) if groups.rows > 1 else cols, out.data_ptr(), cols, stream)
-    return out
+    return out if y.is_cuda else out.to(y.device)

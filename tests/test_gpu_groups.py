@@ -199,6 +199,18 @@ def test_combine_strides_and_bad_rows(gpu_dev):
         assert torch.equal(got, want)
 
 
+def test_host_tensors(gpu_dev):
+    """Host tensors are copied to the GPU and floating-point results back; the order stays there."""
+    import int_crush_converter_amd as icq
+    g = torch.Generator().manual_seed(8)
+    x, y, r = torch.randn(9, 20, generator=g), torch.randn(27, 40, generator=g), torch.randn(9, 40, generator=g)
+    groups, w = icq.route_tokens(x, 3)
+    on, won = icq.route_tokens(x.to(gpu_dev), 3)
+    assert not w.is_cuda and torch.equal(w, won.cpu()) and torch.equal(groups.order, on.order)
+    out = icq.combine_experts(y, groups, w, r)
+    assert not out.is_cuda and torch.equal(out, icq.combine_experts(y.to(gpu_dev), on, won, r.to(gpu_dev)).cpu())
+
+
 def test_other_stream_and_graph(gpu_dev):
     """Calls follow the current stream; a captured router and its way back give the eager result on every replay."""
     import int_crush_converter_amd as icq

@@ -32,6 +32,7 @@ def calls(monkeypatch):
     for mod in (activations, adapters, experts, groups, linear):
         monkeypatch.setattr(mod, "call", lambda name, *args: made.append(name))
     monkeypatch.setattr(nat, "on_gpu", lambda name, t: t)
+    monkeypatch.setattr(nat, "to_gpu", lambda t: t)
     monkeypatch.setattr(nat, "stream_for", lambda *t: 0)
     return made
 
@@ -185,7 +186,11 @@ def test_operands_elsewhere(monkeypatch):
     w = icq.ExpertWeight([weight(16, 64)] * 4)
     monkeypatch.undo()
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(nat, "to_gpu", lambda t: t)
     for f in (lambda: icq.expert_linear(act(5, 64), w, g, gather=True),
+              lambda: icq.group_rows(torch.zeros(3, dtype=torch.int32), 4),
+              lambda: icq.route_tokens(torch.zeros(3, 8), 2),
+              lambda: icq.combine_experts(torch.zeros(10, 8), g, torch.zeros(5, 2)),
               lambda: icq.quantized_linear(act(5, 64), weight(16, 64), adapters=adapter(2, 4, 16, 64), groups=rows_of(5, 1, 2))):
         with pytest.raises(ValueError, match="current device is cuda:0"):
             f()
