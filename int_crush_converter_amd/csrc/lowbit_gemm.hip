@@ -247,6 +247,12 @@ __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
 // have been loaded and exchanged serve NT tiles of weights.  The next step's
 // loads are on their way during a step's products.  Sums are integers: waves
 // add theirs in LDS in any order.
+//
+// One token's four experts of 64, INT4 2816 x 4096: traced 6.6 to 7.4 us, 9.0 to
+// 9.6 a launch in a graph with weights from HBM (23 MB: 2.5 TB/s); 8 experts 10.9
+// us (4.2 TB/s).  Latency bounds it: the launch, the tile's place, then 4 steps of
+// a wave.  With two or four steps' loads in flight it was slower (12 and 22 %
+// with 64 groups of 4 rows), as fewer waves fit.
 template <int KIND, int MT, int NT, int MODE>
 __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
     constexpr int WAVES = 8, W = KIND == kInt8 ? 2 : 1;
@@ -384,10 +390,24 @@ __device__ __forceinline__ void meet() {
 // kernel with 16 x 16 instructions, a work-group a tile, was faster: 318 to 323
 // us where this one took 341 to 345 in turn on the same card.
 //
-// The 256 x 256 forms of INT4 and INT8 spill 22 and 8 registers, at a tile's
-// start and end, none in the K loop.  Spills are vector-memory operations like
+// The 256 x 256 forms of INT4 and INT8 spill 16 and 4 registers (grouped 19 and
+// 3, adapted 81 and 93), at a tile's start and end, none in the K loop.  Spills are vector-memory operations like
 // those that meet() counts.  It lets the newest N stay outstanding; with spills
 // among these it waits for more copies than it needs, never for fewer.
+//
+// Grouped: tiles are numbered group by group, whatever their number of rows; a
+// work-group finds its tile's group by bisection in LDS.  8192 tokens x 4 of 32
+// experts 2816 x 4096 INT4 408 to 416 us, 1.8 POP/s (K = 4096 gives 2.2 in whole
+// tiles; a group's last tile is half empty on average).  Running only the blocks
+// of 32 rows that a last tile has took as long (425 against 424): rows that
+// repeat cost little of the power that bounds the rest.  512 tokens x 4 of 64
+// experts, 32 rows each, 64 x 256 tiles: 83 to 87 us, 4.3 to 4.5 TB/s of weights
+// (a large copy: 4.7 to 5.1).
+//
+// Adapted: 8192 x 4096 x 12288 INT4 with rank 64 traced 367 to 374 us where the
+// plain product takes 343 to 349, 8192 x 4096 x 4096 149 and 124.  Adding the
+// adapters' products block by block behind the K loop, each waiting for its
+// operands from L2, took 437 us.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE = kPlain>
 __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
     typedef typename Acc32<KIND>::T acc_t;
@@ -965,9 +985,8 @@ void launch_wide(const Operands& p, hipStream_t st) {
 }
 
 // As many work-groups as run at once (one a CU with tiles of 256 x 256, whose
-// buffers take most of its LDS, two with 128 x 128), each of which walks its
-// XCD's tiles.  (INT4's 128 x 128 takes 260 registers, four too many for two a
-// CU: its second half starts as the first ends.)
+// buffers take most of its LDS, two with 128 x 128 and 64 x 256, three or four
+// with 32 x 128), each of which walks its XCD's tiles.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE>
 void launch_tiled(const Operands& p, hipStream_t st) {
     const int gm = (int)(MODE == kGrouped ? most_tiles(p.M, p.groups, 32 * WM * FM) : cdiv(p.M, 32 * WM * FM)), gn = (int)cdiv(p.N, 32 * WN * FN);
@@ -991,16 +1010,17 @@ void launch_tiled(const Operands& p, hipStream_t st) {
 //   1344 ( 192 x 7168)     11/32/98    9.9/23/60    7.3/17/44
 // Then tiles of 256 x 256, one a CU, where they fill more than half of a first
 // round over the 256 CUs (up to there 128 x 128 tiles need one round too), or of
-// two and more rounds three quarters, with INT4 two thirds; else of 128 x 128.
+// two and more rounds three quarters, with INT4 two thirds (between these two the
+// forms are within 4 %); else of 128 x 128.
 // 128 x 128 against 256 x 256, y of 4096 columns, K = 1024 / 4096 / 12288:
 //   rows (256-tiles)            INT8                        INT4                         MXFP4
-//   2048 (1/2 round)     17/44/115 - 23/55/139      22/49/119 - 25/56/137      12/25/59  - 16/34/82
-//   2304 (0.56)          24/62/160 - 25/59/143      30/69/168 - 26/57/135      16/34/86  - 16/34/84
-//   4096 (1 round)       31/82/225 - 28/69/178      40/94/237 - 29/66/164      25/46/111 - 22/41/99
-//   5120 (0.63 of two)  36/101/279 - 44/117/305    49/114/288 - 47/112/285     32/57/143 - 28/66/171
-//   5632 (0.69 of two)  42/115/328 - 45/118/309    57/135/343 - 48/115/285     34/63/155 - 28/67/171
-//   6144 (0.75 of two)  43/120/336 - 46/121/319    58/138/345 - 50/118/288     35/65/163 - 29/68/174
-//   8192 (2 rounds)     55/157/446 - 53/133/348    77/188/479 - 54/126/320     37/85/216 - 48/77/191
+//   2048 (1/2 round)     17/44/115 - 23/55/139      16/41/101 - 24/52/127      12/25/59  - 16/34/82
+//   2304 (0.56)          24/62/160 - 25/59/143      22/53/136 - 24/53/128      16/34/86  - 16/34/84
+//   4096 (1 round)       31/82/225 - 28/69/178      29/76/196 - 27/65/166      25/46/111 - 22/41/99
+//   5120 (0.63 of two)  36/101/279 - 44/117/305    36/91/236 - 44/109/286      32/57/143 - 28/66/171
+//   5632 (0.69 of two)  42/115/328 - 45/118/309    40/106/283 - 44/110/286     34/63/155 - 28/67/171
+//   6144 (0.75 of two)  43/120/336 - 46/121/319    41/111/291 - 45/113/291     35/65/163 - 29/68/174
+//   8192 (2 rounds)     55/157/446 - 53/133/348    52/145/385 - 51/127/327     37/85/216 - 48/77/191
 int linear_form(int kind, int64_t M, int64_t N) {      // 0, 128 or 256
     const int64_t groups = cdiv(N, 16) * cdiv(M, 64), tiles = cdiv(M, 256) * cdiv(N, 256), rounds = cdiv(tiles, 256);
     if (M <= 64 || groups < (kind == kInt8 ? 1000 : kind == kInt4 ? 1300 : 1150)) return 0;

@@ -199,6 +199,30 @@ def test_combine_strides_and_bad_rows(gpu_dev):
         assert torch.equal(got, want)
 
 
+def test_as_many_pairs_as_there_may_be(gpu_dev):
+    """1048560 pairs: units of thousands of rows, and rows whose offsets pass 32 bits."""
+    import int_crush_converter_amd as icq
+    n = 1048560
+    g = torch.Generator(device=gpu_dev).manual_seed(1)
+    x = torch.randn(n, 5, generator=g, device=gpu_dev)
+    groups, w = icq.route_tokens(x, 1)
+    ids = x.argmax(1)
+    order = torch.argsort(ids, stable=True)
+    assert torch.equal(groups.ids[:, 0].long(), ids) and torch.equal(groups.order.long(), order) and (w == 1).all()
+    assert torch.equal(groups.offsets.long(), torch.searchsorted(ids[order], torch.arange(6, device=gpu_dev)))
+    assert torch.equal(groups.position[order, 0].long(), torch.arange(n, device=gpu_dev))
+    again = icq.group_rows(torch.arange(n, device=gpu_dev).reshape(-1, 60) % 1023, 1023)
+    want = torch.argsort(torch.arange(n, device=gpu_dev) % 1023, stable=True)
+    assert torch.equal(again.order.long(), want)
+    cols = 2056                                                    # 2 pieces of a row, 2.2e9 elements
+    y = torch.zeros(n, cols, dtype=torch.float16, device=gpu_dev)
+    y[:, 7] = (order % 64).half()
+    y[:, -1] = 3.0
+    out = icq.combine_experts(y, groups, w)
+    assert torch.equal(out[:, 7], (torch.arange(n, device=gpu_dev) % 64).half()) and (out[:, -1] == 3).all()
+    assert not out[:, 8:-1].any()
+
+
 def test_host_tensors(gpu_dev):
     """Host tensors are copied to the GPU and floating-point results back; the order stays there."""
     import int_crush_converter_amd as icq

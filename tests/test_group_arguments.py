@@ -224,7 +224,7 @@ def test_refusals_of_the_library(L):
                                          k.get("ldy", 64), one, one, k.get("res"), k.get("ldr", 0), one, k.get("ldo", 64), None)
     assert comb(y=None) == -1 and comb(dtype=4) == -1 and comb(cols=0) == -1 and comb(ldy=63) == -1 and comb(ldo=63) == -1
     assert comb(res=one, ldr=63) == -1 and comb(top=65) == -3 and comb(tokens=1048560) == -3 and comb(tokens=0) == 0
-    assert comb(tokens=524280, cols=1 << 16, ldy=1 << 16, ldo=1 << 16) == -3
+    assert comb(tokens=1 << 40, top=1) == -3 and comb(cols=1 << 21, ldy=1 << 21, ldo=1 << 21) == -3
     ex = lambda **k: L.ic_expert_linear(one, k.get("lda", 128), one, None, k.get("arows", 4), k.get("offsets", one), k.get("order", one),     # noqa: E731
                                         k.get("top", 2), k.get("groups", 3), k.get("rows", 8), one, k.get("bits", 4), one, 0, k.get("zp"),
                                         None, 0, k.get("N", 8), k.get("K", 64), one, k.get("out", 1), k.get("ldo", 8), None)
