@@ -563,7 +563,7 @@ int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32
 
 /* Which form ic_expert_linear takes for these sizes: 1 or 2 (so many times 16
  * rows, directly from memory), or tiles of 32, 64, 128 or 256 rows. */
-int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N);
+int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N, int64_t K);
 
 /* Low-rank adapters, both of bf16 or of fp16: a [adapters, rank, K] and b
  * [adapters, N, rank], contiguous, laid out once for ic_adapted_linear

@@ -110,7 +110,7 @@ _SIGS = {
     "ic_combine_rows": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp]),
     "ic_expert_linear": (_i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _vp,
                                 _i32, _i64, _i64, _vp, _i32, _i64, _vp]),
-    "ic_expert_form": (_i32, [_i32, _i64, _i64, _i64]),
+    "ic_expert_form": (_i32, [_i32, _i64, _i64, _i64, _i64]),
     "ic_adapter_down_bytes": (_i64, [_i64, _i32, _i64]),
     "ic_adapter_up_bytes": (_i64, [_i64, _i64, _i32, _i32]),
     "ic_adapter_pack": (_i32, [_vp, _vp, _i32, _i64, _i32, _i64, _i64, _vp, _vp, _vp]),

@@ -1089,20 +1089,23 @@ int launch_linear(const Operands& p, hipStream_t st) {
 // Where 32 x 128 tiles would leave a third of the CUs idle, the wide form with
 // 32 rows: INT8 10 groups of 60 rows, 1000 x 2901, 15.1 against 21.9 (128 x 128);
 // INT4 one group of 64 rows, 4096 x 4096, 8.1 against 16.8, 4096 x 12288 12.3
-// against 35.5.
-int expert_form(int kind, int64_t rows, int64_t groups, int64_t N) {      // 1, 2 (wide, so many times 16 rows), 32, 64, 128 or 256
+// against 35.5.  INT4 takes 32 x 128 tiles where there are up to 128 of 64 x 256:
+// 13 groups of 78 rows, 823 x 3662 (104), 22.9 against 29.6; 8 of 128 rows, 2816 x
+// 4096 (176), 36.2 against 27.0.  A K below 1024 has fewer steps than the wide
+// form has waves: 16 groups of one row, 9668 x 120, 16.6 against 10.5 (64 x 256).
+int expert_form(int kind, int64_t rows, int64_t groups, int64_t N, int64_t K) {      // 1, 2 (wide, so many times 16 rows), 32, 64, 128 or 256
     const int64_t met = rows < groups ? rows : groups, each = met ? cdiv(rows, met) : 0;
     const bool many = met * cdiv(N, 256) >= 256;
-    if (each <= (many ? 2 : 16)) return 1;
+    if (each <= (!many ? 16 : K >= 1024 ? 2 : 0)) return 1;
     if (met * cdiv(each, 32) * cdiv(N, 128) < 170) return 2;
-    if (kind == kInt4 && !many && each <= 64) return 32;
+    if (kind == kInt4 && met * cdiv(each, 64) * cdiv(N, 256) <= 128) return 32;
     if (many && each >= (kind == kInt8 ? 128 : 1024)) return 256;
     return kind == kInt8 ? 128 : 64;
 }
 
 template <int KIND>
 int launch_experts(const Operands& p, hipStream_t st) {
-    const int form = expert_form(KIND, p.M, p.groups, p.N);
+    const int form = expert_form(KIND, p.M, p.groups, p.N, p.K);
     constexpr int BUF = KIND == kInt4 ? 3 : 4;
     if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, BUF, kGrouped>(p, st);
     else if (form >= 32) {
@@ -1200,9 +1203,10 @@ extern "C" int ic_quantized_linear(const int8_t* a, int64_t ld_a, const float* s
     return bits == 8 ? launch_linear<kInt8>(p, st) : launch_linear<kInt4>(p, st);
 }
 
-extern "C" int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N) {
-    IC_REQUIRE((bits == 4 || bits == 8) && rows >= 0 && groups >= 1 && N >= 1, "ic_expert_form: bits must be 4 or 8, rows >= 0, groups and N >= 1");
-    return expert_form(bits == 8 ? kInt8 : kInt4, rows, groups, N);
+extern "C" int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N, int64_t K) {
+    IC_REQUIRE((bits == 4 || bits == 8) && rows >= 0 && groups >= 1 && N >= 1 && K >= 1,
+               "ic_expert_form: bits must be 4 or 8, rows >= 0, groups, N and K >= 1");
+    return expert_form(bits == 8 ? kInt8 : kInt4, rows, groups, N, K);
 }
 
 extern "C" int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t a_rows,

@@ -74,7 +74,8 @@ SIZES = [  # rows, top, E, N, K
     (33, 4, 3, 129, 384), (20, 2, 1000, 33, 129), (150, 2, 2, 64, 1000), (300, 1, 2, 130, 257), (500, 2, 3, 264, 640), (700, 2, 4, 300, 130),
     (900, 2, 3, 512, 100), (1200, 2, 2, 260, 1153), (2100, 1, 1, 1000, 64), (513, 3, 70, 96, 520), (1500, 2, 300, 24, 72),
     (1000, 2, 300, 40, 200), (9000, 4, 256, 130, 65), (70000, 4, 300, 17, 40), (1600, 1, 2, 33000, 128), (300, 2, 260, 72, 640),
-    (100, 2, 8, 3000, 130), (900, 1, 6, 2000, 260), (2000, 4, 40, 700, 128), (560, 2, 20, 1500, 200), (70000, 2, 100, 700, 72),
+    (100, 2, 8, 3000, 130), (900, 1, 6, 2000, 260), (2000, 4, 40, 700, 128), (560, 2, 20, 1500, 200), (70000, 2, 100, 700, 72), (20, 1, 54, 3900, 120),
+    (260, 1, 300, 200, 1100),
 ]
 
 
@@ -97,7 +98,7 @@ def test_against_64_bits(gpu_dev, rows, top, E, N, K, bits, asym):
 
 def test_sizes_reach_every_form(gpu_dev):
     import int_crush_converter_amd._native as nat
-    form = lambda bits: {nat.lib().ic_expert_form(bits, r * t, e, n) for r, t, e, n, _ in SIZES}      # noqa: E731
+    form = lambda bits: {nat.lib().ic_expert_form(bits, r * t, e, n, k) for r, t, e, n, k in SIZES}      # noqa: E731
     assert form(4) == {1, 2, 32, 64, 256} and form(8) == {1, 2, 128, 256}
 
 

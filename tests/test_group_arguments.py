@@ -243,4 +243,5 @@ def test_refusals_of_the_library(L):
     assert pack(a=None) == -1 and pack(n=0) == -1 and pack(K=0) == -1 and pack(up=ctypes.c_void_p(8)) == -1
     assert pack(dtype=0) == -1 and pack(n=1024, N=1048560) == -3
     assert pack(n=1025) == -3 and pack(rank=129) == -3 and pack(K=65537) == -3
-    assert L.ic_expert_form(4, -1, 4, 8) == -1 and L.ic_expert_form(4, 4, 0, 8) == -1 and L.ic_expert_form(3, 4, 4, 8) == -1
+    form = L.ic_expert_form
+    assert form(4, -1, 4, 8, 8) == -1 and form(4, 4, 0, 8, 8) == -1 and form(3, 4, 4, 8, 8) == -1 and form(4, 4, 4, 8, 0) == -1
