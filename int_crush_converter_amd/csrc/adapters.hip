@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void pack_down_kernel(const uint16_t* __restri
 // B [adapters, N, rank] -> tiles (adapters.hpp), a lane one column's 8 ranks.
 __global__ __launch_bounds__(256) void pack_up_kernel(const uint16_t* __restrict__ src, int64_t adapters, int64_t N, int rank, int f16,
                                                       lb_u32x4* __restrict__ dst) {
-    const int lane = threadIdx.x & 63, parts = rank_parts(rank), planes = f16 ? 2 : 1;
+    const int lane = threadIdx.x & 63, parts = rank_parts(rank), planes = up_planes(f16);
     const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n_tiles = cdiv(N, 16);     // [adapter][column tile][part][plane]
     if (at >= adapters * n_tiles * parts * planes) return;
     const int64_t n = at / (parts * planes) % n_tiles * 16 + (lane & 15), a = at / (parts * planes) / n_tiles;
@@ -47,9 +47,9 @@ __global__ __launch_bounds__(256) void pack_up_kernel(const uint16_t* __restrict
         for (int k = 0; k < 8; ++k) {
             if (rank0 + k >= rank) continue;
             unsigned v = s[rank0 + k];
-            if (f16) {
+            if (plane) {
                 const float x = f16_bits_to_f32((uint16_t)v), hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-                v = __float_as_uint(plane ? x - hi : hi) >> 16;
+                v = __float_as_uint(plane == 2 ? x - hi : hi) >> 16;
             }
             w[k >> 1] |= v << (16 * (k & 1));
         }
@@ -193,7 +193,7 @@ int launch_shrink(const Adapted& ad, const int8_t* a, int64_t ld_a, const float*
         else if (rank <= 32) high ? go(dt, c3{}, c2{}, c8{}) : go(dt, c2{}, c2{}, c8{});
         else high ? go(dt, c3{}, c4{}, c8{}) : go(dt, c2{}, c4{}, c8{});
     };
-    if (ad.planes == 2) shape(std::integral_constant<int, IC_DTYPE_F16>{});
+    if (ad.f16) shape(std::integral_constant<int, IC_DTYPE_F16>{});
     else shape(std::integral_constant<int, IC_DTYPE_BF16>{});
     IC_CHECK_LAUNCH();
     return IC_OK;
@@ -210,7 +210,7 @@ extern "C" int64_t ic_adapter_down_bytes(int64_t adapters, int rank, int64_t K) 
 
 extern "C" int64_t ic_adapter_up_bytes(int64_t adapters, int64_t N, int rank, int dtype) {
     if (adapters < 0 || rank < 1 || rank > kMaxRank || N < 0 || (dtype != IC_DTYPE_BF16 && dtype != IC_DTYPE_F16)) return 0;
-    return adapters * cdiv(N, 16) * rank_parts(rank) * (dtype == IC_DTYPE_F16 ? 2048 : 1024);
+    return adapters * cdiv(N, 16) * rank_parts(rank) * up_planes(dtype == IC_DTYPE_F16) * 1024;
 }
 
 extern "C" int64_t ic_adapted_linear_workspace_bytes(int64_t M, int rank) {
@@ -226,7 +226,7 @@ extern "C" int ic_adapter_pack(const void* a, const void* b, int dtype, int64_t 
         return fail(IC_ERR_RANGE, "ic_adapter_pack: at most 1024 adapters, rank 128, 65536 for K, 1048560 for N");
     IC_REQUIRE(a && b && down && up && aligned16(down) && aligned16(up), "ic_adapter_pack: null pointer, or results not 16-byte aligned");
     const int64_t tiles = cdiv(K, kActPad) * 2, n = adapters * down_tiles(rank) * tiles;
-    const int64_t u = adapters * cdiv(N, 16) * rank_parts(rank) * (dtype == IC_DTYPE_F16 ? 2 : 1);
+    const int64_t u = adapters * cdiv(N, 16) * rank_parts(rank) * up_planes(dtype == IC_DTYPE_F16);
     if (u > 1 << 25) return fail(IC_ERR_RANGE, "ic_adapter_pack: b takes more than 2^25 KB");
     hipStream_t st = as_stream(stream);
     hipLaunchKernelGGL(pack_down_kernel, dim3((unsigned)cdiv(n, 4)), dim3(256), 0, st, static_cast<const uint16_t*>(a), adapters, rank, K,

@@ -297,14 +297,17 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
     };
     if (t0 < t1) load(t0);
     // the adapters' part of the wave's outputs, whose loads wait together with the first of the product
-    constexpr int OWN = (MT * NT + WAVES - 1) / WAVES;
+    // (with fewer tiles than waves a tile's ranks are shared among waves)
+    constexpr int OWN = (MT * NT + WAVES - 1) / WAVES, SHARES = MT * NT < WAVES ? WAVES / (MT * NT) : 1;
+    __shared__ lb_f32x4 shared[MODE == kAdapted && SHARES > 1 ? WAVES : 1][64];
     lb_f32x4 added[OWN];
     if constexpr (MODE == kAdapted) {
 #pragma unroll
         for (int k = 0; k < OWN; ++k) {
-            const int u = wave + k * WAVES, m = m0 + u / NT * 16 + r, n = (nt0 + u % NT) * 16 + g * 4;
-            added[k] = u < MT * NT && m < m_end && n < p.N ? adapter_dot4(p.ad, p.N, m, n) : lb_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const int u = wave % (MT * NT < WAVES ? MT * NT : WAVES) + k * WAVES, m = m0 + u / NT * 16 + r, n = (nt0 + u % NT) * 16 + g * 4;
+            added[k] = m < m_end && n < p.N ? adapter_dot4(p.ad, p.N, m, n, SHARES > 1 ? wave / (MT * NT) : 0, SHARES) : lb_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+        if (SHARES > 1) shared[wave][lane] = added[0];
     }
     for (int k = threadIdx.x; k < MT * NT * 256; k += 64 * WAVES) (&sum[0][0][0])[k] = 0;
 #pragma unroll
@@ -352,7 +355,13 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
         const int from = source_row<MODE>(p, m);
         const i32x4 s = {sum[u][0][lane], sum[u][1][lane], sum[u][2][lane], sum[u][3][lane]};
         lb_f32x4 y = cols.finish(s, p.sa[from], p.zp ? p.sums[from] : 0);
-        if constexpr (MODE == kAdapted) y += added[own];
+        if constexpr (MODE == kAdapted && SHARES == 1) y += added[own];
+        else if constexpr (MODE == kAdapted) {
+            lb_f32x4 a = shared[u][lane];
+#pragma unroll
+            for (int k = 1; k < SHARES; ++k) a += shared[u + k * MT * NT][lane];
+            y += a;
+        }
         store4(p, y, m, n, m_end);
     }
 }
@@ -533,7 +542,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
     // of the activations (INT4: 32 ranks of hi and of lo in a stage, INT8: of one of them), one of B like one of the
     // weights.  Rows with another adapter or none take the row of zeros.  Fetched one after another: adapter `ad_now`,
     // its stage `ad_stage`.
-    const int ad_stages = p.ad.parts * p.ad.planes * (KIND == kInt8 ? 2 : 1);
+    const int ad_planes = p.ad.f16 ? 2 : 1, ad_stages = p.ad.parts * ad_planes * (KIND == kInt8 ? 2 : 1);
     int ad_now = -1, ad_stage = 0, ad_set = 0;
     auto next_adapter = [&]() {                            // the lowest in the set above ad_now (there is one)
         const unsigned* set = present + ad_set * (kMaxGroups / 32);
@@ -548,7 +557,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
             if (ad_stage == 0) next_adapter();
             lb_u32x4* to = lds + buf * STAGE + wave * 64;
             const int half = KIND == kInt8 ? ad_stage & 1 : 0, tile_of = KIND == kInt8 ? ad_stage >> 1 : ad_stage;   // (tile_of: part and plane)
-            const int pitch = p.ad.parts * 128, from = tile_of / p.ad.planes * 128 + half * 64;
+            const int pitch = p.ad.parts * 128, part = tile_of / ad_planes, from = part * 128 + half * 64;
             const int lane_row = KIND == kInt4 ? lane >> 3 : lane >> 2;
             const int chunk = KIND == kInt4 ? (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4)) : (lane & 3) ^ (lane >> 4);
             const __amdgpu_buffer_rsrc_t t_buf = buffer(p.ad.t);
@@ -557,12 +566,12 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
                 const int at = (i * WAVES + wave) * (KIND == kInt4 ? 8 : 16) + lane_row;
                 copy(t_buf, (row_id[at] == ad_now ? row0 + at : (int)p.M) * pitch + chunk * 16, from, to + i * WAVES * 64);
             }
-            const int nt = bn * (BN / 16), nl = n_tiles - 1 - nt, up_pitch = p.ad.parts * p.ad.planes * 1024;
+            const int nt = bn * (BN / 16), nl = n_tiles - 1 - nt, up_pitch = p.ad.parts * up_planes(p.ad.f16) * 1024;
             const __amdgpu_buffer_rsrc_t up_buf = buffer(p.ad.up + ((int64_t)ad_now * n_tiles + nt) * up_pitch);
 #pragma unroll
             for (int i = 0; i < W_LOADS; ++i) {
                 const int at = i * WAVES + wave < nl ? i * WAVES + wave : nl;
-                copy(up_buf, lane16, at * up_pitch + tile_of * 1024, to + (X_LOADS + i) * WAVES * 64);
+                copy(up_buf, lane16, at * up_pitch + (p.ad.f16 ? part * 3 + 1 + tile_of % 2 : part) * 1024, to + (X_LOADS + i) * WAVES * 64);
             }
             ad_stage = ad_stage + 1 == ad_stages ? 0 : ad_stage + 1;
         }
@@ -1032,8 +1041,16 @@ template <int KIND, int MODE = kPlain>
 int launch_linear(const Operands& p, hipStream_t st) {
     constexpr int BUF = KIND == kInt4 ? 3 : 4;
     int form = linear_form(KIND, p.M, p.N);
-    // (a tile's adapters are known when BUF - 1 stages of it have been asked for)
-    if (MODE == kAdapted && cdiv(p.K, KIND == kInt8 ? 64 : 128) < BUF - 1) form = 0;
+    if constexpr (MODE == kAdapted) {
+        // The end of a tile takes longer, which two work-groups a CU hide: 256 x 256 from K = 4096 on, and where they fill
+        // three quarters of their rounds.  128 against 256, INT4 / INT8, rank 16 where not said, us: 8192 x 4096 x 1024 68
+        // to 77 / 75 to 87; 2304 x 4096 x 2048 43 to 51 / 47 to 58; 4096 x 4096 x 4096 90 to 89 / 100 to 99; 8192 x 4096
+        // x 4096 rank 64 173 to 165 / 189 to 184; 8192 x 4100 x 4096 (0.71) 192 to 242.
+        const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256);
+        if (form == 256 && (p.K < 4096 || (tiles > 256 && tiles * 12 < cdiv(tiles, 256) * 256 * 9))) form = 128;
+        // (a tile's adapters are known when BUF - 1 stages of it have been asked for)
+        if (cdiv(p.K, KIND == kInt8 ? 64 : 128) < BUF - 1) form = 0;
+    }
     if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, BUF, MODE>(p, st);
     else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, BUF, MODE>(p, st);
     else if constexpr (MODE == kPlain) {
@@ -1244,7 +1261,7 @@ extern "C" int ic_adapted_linear(const int8_t* a, int64_t ld_a, const float* sa,
     IC_REQUIRE(aligned16(down) && aligned16(up) && aligned16(workspace), "ic_adapted_linear: adapters and workspace need 16-byte alignment");
     hipStream_t st = as_stream(stream);
     ProfScope prof(st, PT_OTHER, 2.0 * M * N * K + 2.0 * M * rank * (N + K), (double)M * K + (double)N * K * bits / 8);
-    p.ad = Adapted{ids, static_cast<uint16_t*>(workspace), static_cast<const uint8_t*>(up), adapter_dtype == IC_DTYPE_F16 ? 2 : 1, rank_parts(rank), (int)adapters,
+    p.ad = Adapted{ids, static_cast<uint16_t*>(workspace), static_cast<const uint8_t*>(up), adapter_dtype == IC_DTYPE_F16, rank_parts(rank), (int)adapters,
                    (rank + 7) / 8};
     if (const int rc = launch_shrink(p.ad, a, ld_a, sa, M, K, down, rank, scaling, offsets, order, st)) return rc;
     return bits == 8 ? launch_linear<kInt8, kAdapted>(p, st) : launch_linear<kInt4, kAdapted>(p, st);

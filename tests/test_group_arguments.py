@@ -203,7 +203,7 @@ def test_sizes_of_the_library(L):
     for rows in (1, 16, 17, 4000, 4096, 4097, 8191, 100000, 1048560):
         assert L.ic_group_workspace_bytes(rows, 7) <= 4 * groups.RowGroups._empty(rows, 1, 7, torch.device("cpu")).scratch
     assert L.ic_adapter_down_bytes(3, 12, 130) == 3 * 16 * 256 * 2 and L.ic_adapter_up_bytes(3, 17, 33, 1) == 3 * 2 * 2 * 1024
-    assert L.ic_adapter_up_bytes(3, 17, 33, 2) == 3 * 2 * 2 * 2048 and L.ic_adapter_up_bytes(3, 17, 33, 0) == 0
+    assert L.ic_adapter_up_bytes(3, 17, 33, 2) == 3 * 2 * 2 * 3072 and L.ic_adapter_up_bytes(3, 17, 33, 0) == 0
     assert L.ic_adapted_linear_workspace_bytes(7, 12) == 8 * 128
     assert L.ic_adapter_up_bytes(1024, 1048560, 128, 1) == 1024 * 1048560 * 128 * 2           # past 32 bits
 
