@@ -562,7 +562,8 @@ int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32
                      int bias_dtype, int64_t N, int64_t K, void* out, int out_dtype, int64_t ld_out, void* stream);
 
 /* Which form ic_expert_linear takes for these sizes: 1 or 2 (so many times 16
- * rows, directly from memory), or tiles of 32, 64, 128 or 256 rows. */
+ * rows, directly from memory), or tiles of 32 x 128, 64 x 256, 128 x 128 or
+ * 128 x 256 (32, 64, 128 and 256). */
 int ic_expert_form(int bits, int64_t rows, int64_t groups, int64_t N, int64_t K);
 
 /* Low-rank adapters, both of bf16 or of fp16: a [adapters, rank, K] and b

@@ -399,26 +399,27 @@ __device__ __forceinline__ void meet() {
 // kernel with 16 x 16 instructions, a work-group a tile, was faster: 318 to 323
 // us where this one took 341 to 345 in turn on the same card.
 //
-// The 256 x 256 forms of INT4 and INT8 spill 16 and 4 registers (grouped 19 and
-// 3, adapted 81 and 93), at a tile's start and end, none in the K loop.  Spills are vector-memory operations like
+// The 256 x 256 forms of INT4 and INT8 spill 16 and 4 registers (adapted 82 and
+// 93; the grouped ones of 128 x 256 20 and 3), at a tile's start and end, none in the K loop.  Spills are vector-memory operations like
 // those that meet() counts.  It lets the newest N stay outstanding; with spills
 // among these it waits for more copies than it needs, never for fewer.
 //
 // Grouped: tiles are numbered group by group, whatever their number of rows; a
 // work-group finds its tile's group by bisection in LDS.  8192 tokens x 4 of 32
-// experts 2816 x 4096 INT4 408 to 416 us, 1.8 POP/s (K = 4096 gives 2.2 in whole
-// tiles; a group's last tile is half empty on average).  Running only the blocks
-// of 32 rows that a last tile has took as long (425 against 424): rows that
-// repeat cost little of the power that bounds the rest.  512 tokens x 4 of 64
-// experts, 32 rows each, 64 x 256 tiles: 83 to 87 us, 4.3 to 4.5 TB/s of weights
-// (a large copy: 4.7 to 5.1).
+// experts 2816 x 4096 INT4 370 to 383 us, 2.0 POP/s (K = 4096 gives 2.2 in whole tiles;
+// a group's last tile is half empty on average): 128 x 256 by two work-groups of
+// 4 waves a CU, one at its products while the other is at a tile's end.  64 x 256
+// took 409, 256 x 256 414.  Running only the blocks of 32 rows that a last tile
+// has took as long (425 against 424, 256 x 256): rows that repeat cost little of
+// the power that bounds the rest.  512 tokens x 4 of 64 experts, 32 rows each, 64 x
+// 256 tiles: 83 to 87 us, 4.3 to 4.5 TB/s of weights (a large copy: 4.7 to 5.1).
 //
 // Adapted: 8192 x 4096 x 12288 INT4 with rank 64 traced 367 to 374 us where the
 // plain product takes 343 to 349, 8192 x 4096 x 4096 149 and 124.  Adding the
 // adapters' products block by block behind the K loop, each waiting for its
 // operands from L2, took 437 us.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE = kPlain>
-__global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
+__global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
     typedef typename Acc32<KIND>::T acc_t;
     constexpr int WAVES = WM * WN, BM = 32 * WM * FM, BN = 32 * WN * FN;
     constexpr int X_KB = BM / 16 * (KIND == kInt4 ? 2 : 1), W_KB = BN / 16;      // a stage's KB
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
     // (and a group's first row of tiles)
     constexpr int SCALES = BUF * STAGE, COLS = SCALES + 2 * S_WORDS, ROWS = COLS + BN * 3 / 4, GROUPS = ROWS + (KIND == kMx ? 0 : BM / 2);
     // (kAdapted: each row's adapter, and which of the adapters the rows have, a bit each, for two tiles in turn)
-    __shared__ lb_u32x4 lds[GROUPS + (MODE == kGrouped ? kMaxGroups / 4 + 1 : MODE == kAdapted ? BM / 4 + kMaxGroups / 64 : 0)];
+    __shared__ lb_u32x4 lds[GROUPS + (MODE == kGrouped ? kMaxGroups / 8 + 1 : MODE == kAdapted ? BM / 4 + kMaxGroups / 64 : 0)];
     int* const row_id = reinterpret_cast<int*>(lds + GROUPS);
     unsigned* const present = reinterpret_cast<unsigned*>(lds + GROUPS + BM / 4);
     float* const col = reinterpret_cast<float*>(lds + COLS);
@@ -443,11 +444,11 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
     const int wm = wave / WN, wn = wave % WN;
     const int lane16 = lane * 16;
 
-    int* const starts = reinterpret_cast<int*>(lds + GROUPS);
+    uint16_t* const starts = reinterpret_cast<uint16_t*>(lds + GROUPS);
     if constexpr (MODE == kGrouped) {
         if (wave == 0) group_starts(p.offsets, p.groups, (int)p.M, BM, starts);
         __syncthreads();
-        grid_m = __builtin_amdgcn_readfirstlane(starts[p.groups]);
+        grid_m = __builtin_amdgcn_readfirstlane((int)starts[p.groups]);
     }
 
     // work-groups are dealt to the 8 XCDs in turn: each XCD gets one run of tiles, walked in bands of 8 tile rows so
@@ -481,12 +482,12 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted ? 2 : 1) void linear
             group = 0;
             while (past - group > 1) {
                 const int mid = (group + past) >> 1;
-                if (starts[mid] <= tile_row) group = mid;
+                if ((int)starts[mid] <= tile_row) group = mid;
                 else past = mid;
             }
             group = __builtin_amdgcn_readfirstlane(group);
-            const int s0 = __builtin_amdgcn_readfirstlane(starts[group]);
-            rows_of = __builtin_amdgcn_readfirstlane(starts[group + 1]) - s0;
+            const int s0 = __builtin_amdgcn_readfirstlane((int)starts[group]);
+            rows_of = __builtin_amdgcn_readfirstlane((int)starts[group + 1]) - s0;
             at -= s0 * grid_n;
         }
         const int band = at / (8 * grid_n), rows_in = rows_of - band * 8 < 8 ? rows_of - band * 8 : 8;
@@ -994,8 +995,8 @@ void launch_wide(const Operands& p, hipStream_t st) {
 }
 
 // As many work-groups as run at once (one a CU with tiles of 256 x 256, whose
-// buffers take most of its LDS, two with 128 x 128 and 64 x 256, three or four
-// with 32 x 128), each of which walks its XCD's tiles.
+// buffers take most of its LDS, two with 128 x 128, 128 x 256 and 64 x 256, three
+// or four with 32 x 128), each of which walks its XCD's tiles.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE>
 void launch_tiled(const Operands& p, hipStream_t st) {
     const int gm = (int)(MODE == kGrouped ? most_tiles(p.M, p.groups, 32 * WM * FM) : cdiv(p.M, 32 * WM * FM)), gn = (int)cdiv(p.N, 32 * WN * FN);
@@ -1072,37 +1073,41 @@ int launch_linear(const Operands& p, hipStream_t st) {
 // goes by their average, and by whether a row of 64 x 256 tiles of every group
 // that can have rows fills the CUs (`many`).  Measured, weights from HBM, rows
 // at random over 8 (few) and 64 groups (many), us:
-//                  2816 x 4096                              4096 x 1408
-//   rows a group   wide 16  wide 32  32x128  64x256  256^2  wide 16  wide 32  32x128  64x256  256^2
-//   INT4,  8,   1    10.9     11.8    17.6    25.3             8.7     11.2    11.1    14.8
-//               8    14.2     17.8    17.9    25.0             9.4     12.8    11.3    15.0
-//              16    14.6     18.3    17.9    25.4            11.6     13.0    11.4    15.1
-//              32    18.7     19.2    18.3    25.4            16.2     17.4    13.5    15.1
-//              64    28.5     30.0    22.3    25.7            25.1     25.8    14.3    16.1
-//             128                     36.2    27.0    54                       23.9    19.8    30
-//            1024                              112   120                               73     88
-//            2048                              218   193                              138    148
-//   INT4, 64,   1    47.7     61.6    56.2    50.0            31.5     56.8    30.7    33.8
-//               2    63.8     87.4    64.9    80.8            43.7     77.0    40.9    43.2
-//               4    73.8     96.9    71.3    78.8            51.4     90.7    51.7    45.7
-//              16    98.7    102.4    75.8    79.5            68.1     94.1    54.7    50.7
-//              64     197      207     136    97.4             162      198     103    67.9
-//             256                              248   267                              165    217
-//             512                              455   451                              304    313
-//            1024                              864   813                              572    576
-//                  wide 16  wide 32  128x128  256^2            wide 16  wide 32  128x128  256^2
+//                  2816 x 4096                               4096 x 1408
+//   rows a group   wide 16  wide 32  32x128  64x256  128x256  wide 16  wide 32  32x128  64x256  128x256
+//   INT4,  8,   1    10.9     11.8    17.6    25.3              8.7     11.2    11.1    14.8
+//               8    14.2     17.8    17.9    25.0              9.4     12.8    11.3    15.0
+//              16    14.6     18.3    17.9    25.4             11.6     13.0    11.4    15.1
+//              32    18.7     19.2    18.3    25.4             16.2     17.4    13.5    15.1
+//              64    28.5     30.0    22.3    25.7             25.1     25.8    14.3    16.1
+//             128                     36.2    27.0    39.9                      23.9    19.8
+//             512                             60.0    62.4                              45.2    48.0
+//            1024                              111     101                              71.8    74.5
+//            2048                              216     191                               136     129
+//   INT4, 64,   1    47.7     61.6    56.2    50.0             31.5     56.8    30.7    33.8
+//               2    63.8     87.4    64.9    80.8             43.7     77.0    40.9    43.2
+//               4    73.8     96.9    71.3    78.8             51.4     90.7    51.7    45.7
+//              16    98.7    102.4    75.8    79.5             68.1     94.1    54.7    50.7
+//              64     197      207     136    97.4     115      162      198     103    67.9
+//             256                              252     240                               163     158
+//            1024                              887     801                               568     528
+//                  wide 16  wide 32  128x128  128x256          wide 16  wide 32  128x128  128x256
 //   INT8,  8,   8    21.1     25.5    29.0                      13.4     15.6    16.4
 //              16    25.6     26.4    28.8                      15.3     15.9    17.1
-//              32    29.9     28.8    29.2                      20.4     20.5    16.7
+//              32    29.9     28.8    29.2     42.9             20.4     20.5    16.7
 //              64    41.0     37.6    30.8                      32.0     29.6    17.6
-//             128                     36.9    55.7                               22.6   29.2
-//            1024                      139     129                               86.1   89.4
+//             128                     36.5     49.3                               22.4     23.5
+//             256                     56.4     49.6                               31.6     30.9
+//            1024                      135      109                               83.0     78.0
 //   INT8, 64,   1    85.7     86.9    96.0                      49.1     65.0    56.2
 //               4     124      133     137                      90.9      113    85.9
 //              16     147      148     145                       116      122    89.7
-//             128                      235     215                                143    147
-//             256                      355     327                                216    214
-//            1024                     1179     865                                678    571
+//              32                      152      140                               94.0     93.0
+//             128                      237      216                                145      123
+//            1024                     1175      897                                683      570
+// 256 x 256 tiles, one work-group a CU, took 117 us (INT8 125) where the table
+// has 101 (109), and 836 (847) where it has 801 (897): they lead by 13 % at best,
+// INT8 with 8 groups of 512 rows, and lose by up to 30 %.
 // Where 32 x 128 tiles would leave a third of the CUs idle, the wide form with
 // 32 rows: INT8 10 groups of 60 rows, 1000 x 2901, 15.1 against 21.9 (128 x 128);
 // INT4 one group of 64 rows, 4096 x 4096, 8.1 against 16.8, 4096 x 12288 12.3
@@ -1110,13 +1115,14 @@ int launch_linear(const Operands& p, hipStream_t st) {
 // 13 groups of 78 rows, 823 x 3662 (104), 22.9 against 29.6; 8 of 128 rows, 2816 x
 // 4096 (176), 36.2 against 27.0.  A K below 1024 has fewer steps than the wide
 // form has waves: 16 groups of one row, 9668 x 120, 16.6 against 10.5 (64 x 256).
-int expert_form(int kind, int64_t rows, int64_t groups, int64_t N, int64_t K) {      // 1, 2 (wide, so many times 16 rows), 32, 64, 128 or 256
+int expert_form(int kind, int64_t rows, int64_t groups, int64_t N, int64_t K) {      // 1, 2 (wide), 32, 64, 128 or 256 (128 x 256)
     const int64_t met = rows < groups ? rows : groups, each = met ? cdiv(rows, met) : 0;
     const bool many = met * cdiv(N, 256) >= 256;
     if (each <= (!many ? 16 : K >= 1024 ? 2 : 0)) return 1;
     if (met * cdiv(each, 32) * cdiv(N, 128) < 170) return 2;
     if (kind == kInt4 && met * cdiv(each, 64) * cdiv(N, 256) <= 128) return 32;
-    if (many && each >= (kind == kInt8 ? 128 : 1024)) return 256;
+    const int64_t tiles = met * cdiv(each, 128) * cdiv(N, 256);
+    if (kind == kInt4 ? each >= 256 && tiles >= 512 : tiles >= (each >= 128 ? 170 : 512)) return 256;
     return kind == kInt8 ? 128 : 64;
 }
 
@@ -1124,7 +1130,7 @@ template <int KIND>
 int launch_experts(const Operands& p, hipStream_t st) {
     const int form = expert_form(KIND, p.M, p.groups, p.N, p.K);
     constexpr int BUF = KIND == kInt4 ? 3 : 4;
-    if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, BUF, kGrouped>(p, st);
+    if (form == 256) launch_tiled<KIND, 1, 4, 4, 2, BUF - 1, kGrouped>(p, st);
     else if (form >= 32) {
         if constexpr (KIND == kInt8) launch_tiled<KIND, 2, 2, 2, 2, BUF, kGrouped>(p, st);
         else if (form == 32) launch_tiled<KIND, 1, 2, 1, 2, BUF, kGrouped>(p, st);

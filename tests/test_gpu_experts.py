@@ -75,7 +75,7 @@ SIZES = [  # rows, top, E, N, K
     (900, 2, 3, 512, 100), (1200, 2, 2, 260, 1153), (2100, 1, 1, 1000, 64), (513, 3, 70, 96, 520), (1500, 2, 300, 24, 72),
     (1000, 2, 300, 40, 200), (9000, 4, 256, 130, 65), (70000, 4, 300, 17, 40), (1600, 1, 2, 33000, 128), (300, 2, 260, 72, 640),
     (100, 2, 8, 3000, 130), (900, 1, 6, 2000, 260), (2000, 4, 40, 700, 128), (560, 2, 20, 1500, 200), (70000, 2, 100, 700, 72), (20, 1, 54, 3900, 120),
-    (260, 1, 300, 200, 1100),
+    (260, 1, 300, 200, 1100), (9000, 4, 64, 260, 520), (4600, 4, 16, 1100, 1153),
 ]
 
 
@@ -102,7 +102,8 @@ def test_sizes_reach_every_form(gpu_dev):
     assert form(4) == {1, 2, 32, 64, 256} and form(8) == {1, 2, 128, 256}
 
 
-@pytest.mark.parametrize("rows,top,E,N,K", [(3, 2, 5, 40, 200), (90, 2, 4, 37, 130), (700, 2, 4, 260, 520), (1500, 2, 2, 264, 300), (1500, 2, 2, 261, 300)])
+@pytest.mark.parametrize("rows,top,E,N,K", [(3, 2, 5, 40, 200), (90, 2, 4, 37, 130), (700, 2, 4, 260, 520), (1500, 2, 2, 264, 300), (1500, 2, 2, 261, 300),
+                                            (4600, 2, 16, 1700, 300)])
 def test_output_types_and_the_experts_own_products(gpu_dev, rows, top, E, N, K):
     """16-bit results are the fp32 ones rounded once; each row has the bits of quantized_linear with its expert's weight."""
     import int_crush_converter_amd as icq
