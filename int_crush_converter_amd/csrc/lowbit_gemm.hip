@@ -400,9 +400,10 @@ __device__ __forceinline__ void meet() {
 // us where this one took 341 to 345 in turn on the same card.
 //
 // The 256 x 256 forms of INT4 and INT8 spill 16 and 4 registers (adapted 82 and
-// 93; the grouped ones of 128 x 256 20 and 3), at a tile's start and end, none in the K loop.  Spills are vector-memory operations like
-// those that meet() counts.  It lets the newest N stay outstanding; with spills
-// among these it waits for more copies than it needs, never for fewer.
+// 93; the grouped ones of 128 x 256 20 and 3), at a tile's start and end, none
+// in the K loop.  Spills are vector-memory operations like those that meet()
+// counts.  It lets the newest N stay outstanding; with spills among these it
+// waits for more copies than it needs, never for fewer.
 //
 // Grouped: tiles are numbered group by group, whatever their number of rows; a
 // work-group finds its tile's group by bisection in LDS.  8192 tokens x 4 of 32
@@ -1059,10 +1060,15 @@ int launch_linear(const Operands& p, hipStream_t st) {
         else if (p.M <= 32) launch_direct<KIND, 2>(p, st);
         else launch_direct<KIND, 4>(p, st);
     } else {
-        // (64 rows, INT4 12288 x 4096: 17.2 us with 2 x 2, 14.2 with 4 x 4; 4096 x 4096, 64 work-groups: 8.1 and 12.6)
+        // More than 32 rows: one work-group of 4 x 3 or 4 x 4 runs a CU, so the fewer rounds count, and 2 x 2 where they
+        // would leave a quarter of the CUs idle.  2 x 2 / 4 x 3 / 4 x 4, K = 4096, rank 16, INT4, us: 64 x 8192 17.8 / 19.6 /
+        // 22.1; 64 x 10240 23.9 / 20.0 / 22.5; 64 x 12288 25.3 / 20.9 / 24.6; 64 x 14336 24.8 / 33.0 / 22.9; 64 x 24576 38.3
+        // / 35.1 / 38.3; 128 x 4096 16.8 / 20.8 / 21.0; 192 x 4096 23.3 / 32.6 / 21.6; INT8 64 x 12288 28.5 / 24.8 / 29.9.
+        const int64_t high = cdiv(p.M, 64), threes = high * cdiv(p.N, 48), fours = high * cdiv(p.N, 64);
         if (p.M <= 16 && cdiv(p.N, 32) < 256) launch_wide<KIND, 1, 1, MODE>(p, st);
         else if (p.M <= 16) launch_wide<KIND, 1, 2, MODE>(p, st);
-        else if (p.M > 32 && cdiv(p.M, 64) * cdiv(p.N, 64) >= 128) launch_wide<KIND, 4, 4, MODE>(p, st);
+        else if (p.M > 32 && threes >= 200 && cdiv(threes, 256) <= cdiv(fours, 256)) launch_wide<KIND, 4, 3, MODE>(p, st);
+        else if (p.M > 32 && threes >= 200) launch_wide<KIND, 4, 4, MODE>(p, st);
         else launch_wide<KIND, 2, 2, MODE>(p, st);
     }
     IC_CHECK_LAUNCH();

@@ -81,6 +81,7 @@ SIZES = [  # M, N, K, adapters, rank
     (33, 48, 2901, 1000, 8), (64, 512, 256, 40, 16), (65, 300, 640, 2, 128), (300, 1000, 512, 7, 33), (1, 4096, 4096, 4, 16),
     (700, 1500, 65, 3, 16), (1100, 1000, 300, 30, 24), (2100, 2100, 260, 5, 64), (4200, 2304, 130, 300, 16), (2050, 4100, 64, 2, 128),
     (2050, 4100, 300, 3, 128), (2050, 4100, 4200, 3, 16), (2050, 4104, 4100, 40, 64), (1500, 1400, 193, 1000, 40), (900, 2000, 260, 70, 8), (4100, 2600, 520, 1, 16),
+    (70, 7000, 300, 3, 12), (40, 10111, 200, 5, 40), (9, 8200, 260, 4, 16),     # 64 rows x 64 and x 48 columns, 16 x 32
 ]
 
 
