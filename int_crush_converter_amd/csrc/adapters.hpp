@@ -40,7 +40,7 @@ typedef _Float16 lb_f16x8 __attribute__((ext_vector_type(8)));
 // The adapter's part of four consecutive outputs of row m from column n (a
 // multiple of 4), share k of n of its ranks: a dot product in fp32, for few rows,
 // which seldom share an adapter.  64 rows with 48 adapters of rank 16, INT4 12288
-// x 4096: 17.8 to 19.3 us traced, 11.8 without adapters; 19 MB of B are most of
+// x 4096: 16.0 to 16.8 us traced, 11.8 without adapters; 19 MB of B are most of
 // the difference.
 __device__ __forceinline__ lb_f32x4 adapter_dot4(const Adapted& ad, int64_t N, int64_t m, int64_t n, int share, int shares) {
     lb_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
