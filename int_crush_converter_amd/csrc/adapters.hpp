@@ -37,15 +37,16 @@ typedef float lb_f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 lb_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 lb_f16x8 __attribute__((ext_vector_type(8)));
 
-// The adapter's part of four consecutive outputs of row m from column n (a
-// multiple of 4), share k of n of its ranks: a dot product in fp32, for few rows,
-// which seldom share an adapter.  64 rows with 48 adapters of rank 16, INT4 12288
-// x 4096: 16.0 to 16.8 us traced, 11.8 without adapters; 19 MB of B are most of
-// the difference.
-__device__ __forceinline__ lb_f32x4 adapter_dot4(const Adapted& ad, int64_t N, int64_t m, int64_t n, int share, int shares) {
+__device__ __forceinline__ lb_f32x4 mma_ranks(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lb_bf16x8, w), __builtin_bit_cast(lb_bf16x8, x), acc, 0, 0, 0);
+}
+
+// Adapter id's part of four consecutive outputs of row m from column n (a multiple
+// of 4), share k of n of its ranks: a dot product in fp32, for rows that seldom share
+// an adapter.  64 rows with 48 adapters of rank 16, INT4 12288 x 4096: 16.0 to 16.8 us
+// traced, 11.8 without adapters; 19 MB of B are most of the difference.
+__device__ __forceinline__ lb_f32x4 adapter_dot4(const Adapted& ad, int64_t N, int64_t m, int id, int64_t n, int share, int shares) {
     lb_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int id = ad.ids[m];
-    if (id < 0 || id >= ad.adapters) return s;
     const int planes = up_planes(ad.f16);
     const lb_u32x4* t = reinterpret_cast<const lb_u32x4*>(ad.t + m * ad.parts * 64);
     const lb_u32x4* b = reinterpret_cast<const lb_u32x4*>(ad.up + (id * cdiv(N, 16) + n / 16) * (ad.parts * planes) * 1024) + n % 16;
@@ -63,6 +64,66 @@ __device__ __forceinline__ lb_f32x4 adapter_dot4(const Adapted& ad, int64_t N, i
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 s[i] = __builtin_fmaf(v[k], ad.f16 ? half_word<IC_DTYPE_F16>(u[k >> 1], k & 1) : half_word<IC_DTYPE_BF16>(u[k >> 1], k & 1), s[i]);
+        }
+    }
+    return s;
+}
+
+// The adapters' part of 16 rows x 16 columns, this lane's four outputs as above:
+// row m of `rows`, with adapter `id` (-1: none, or no row), columns nt * 16 + g * 4.
+// Where the rows share adapters, one adapter after another on the matrix cores,
+// rows of others with t of zeros; the loads for four tiles of B wait together.
+// Where few do, dot products: the matrix cores read a tile of B for each adapter
+// of the rows, a dot product its own row's part, and they meet at two or four
+// such tiles for 8 ranks (dots / matrix cores, 12288 x 4096 INT4 but for the
+// last, us; of the adapters, 64 rows drew at random):
+//   rank 16, bf16, 48: 23.5 / 26.5        rank 64, bf16, 12: 33.6 / 26.5, 48: 37.7 / 33.7
+//   rank 32, bf16, 48: 28.5 / 27.6, 8: 24.9 / 22.3        rank 64, fp16, 12: 33.5 / 33.9, 48: 37.4 / 44.4
+//   rank 128, 8, fp16: 48.5 / 44.5; bf16, 200 rows of 2816 x 4096: 46.3 / 31.2, 25 rows one after another 40.6 / 22.9
+__device__ __forceinline__ lb_f32x4 adapter_tile(const Adapted& ad, int64_t N, int rows, int m, int id, int nt, int share, int shares) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, n_tiles = (int)cdiv(N, 16);
+    lb_f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (nt >= n_tiles) return s;
+    if (id >= ad.adapters) id = -1;
+    unsigned left = (unsigned)__ballot(id >= 0) & 0xffffu;
+    int now = -1;
+    auto pick = [&]() {                                    // the next adapter, in the order of its first row
+        now = __builtin_amdgcn_readlane(id, __builtin_ctz(left));
+        left &= ~(unsigned)__ballot(id == now);
+    };
+    const unsigned all = left;
+    const int planes = up_planes(ad.f16), per = ad.parts * (ad.f16 ? 2 : 1), most = (ad.eights < 4 ? 2 : 4) * ad.eights;
+    int tiles = 0;
+    while (left && tiles <= most) {
+        pick();
+        tiles += per;
+    }
+    if (tiles > most) return id >= 0 && nt * 16 + g * 4 < N ? adapter_dot4(ad, N, m, id, nt * 16 + g * 4, share, shares) : s;
+    const int first = tiles * share / shares, last = tiles * (share + 1) / shares;
+    int at = first;                                        // the adapter's tile: part and plane
+    left = all;
+    if (left) pick();
+    for (; at >= per && left; at -= per) pick();
+    for (int p = first; p < last; p += 4) {
+        lb_u32x4 b[4], hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (p + k >= last) break;
+            const int part = ad.f16 ? at >> 1 : at;
+            const lb_u32x4* u = reinterpret_cast<const lb_u32x4*>(ad.up) + (((int64_t)now * n_tiles + nt) * ad.parts + part) * planes * 64 + lane;
+            const lb_u32x4* t = reinterpret_cast<const lb_u32x4*>(ad.t) + ((int64_t)(id == now ? m : rows) * ad.parts + part) * 8 + g;
+            b[k] = u[ad.f16 ? 64 + (at & 1) * 64 : 0];
+            hi[k] = t[0];
+            lo[k] = t[4];
+            if (++at == per && left) {
+                at = 0;
+                pick();
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (p + k >= last) break;
+            s = mma_ranks(b[k], lo[k], mma_ranks(b[k], hi[k], s));
         }
     }
     return s;

@@ -107,17 +107,19 @@ __device__ __forceinline__ GroupTile find_tile(const int32_t* offsets, int group
 
 // starts[g] = tiles of `height` rows of the groups before g, for g <= groups
 // (LDS; one wave).  Fewer than 2^16 for a height of 32 and more: 2^20 rows.
+// (Edges that are not in order could have more: what is past 2^16 is left out.)
 __device__ __forceinline__ void group_starts(const int32_t* offsets, int groups, int rows, int height, uint16_t* starts) {
     const int lane = threadIdx.x & 63;
+    auto held = [](int n) { return (uint16_t)(n < 0xffff ? n : 0xffff); };
     int before = 0;
     for (int g0 = 0; g0 < groups; g0 += 64) {
         const int g = g0 + lane;
         const int lo = g < groups ? group_edge(offsets, g, rows) : 0, hi = g < groups ? group_edge(offsets, g + 1, rows) : 0;
         const int own = hi > lo ? (hi - lo + height - 1) / height : 0, upto = wave_scan(own);
-        if (g < groups) starts[g] = (uint16_t)(before + upto - own);
+        if (g < groups) starts[g] = held(before + upto - own);
         before += __builtin_amdgcn_readlane(upto, 63);
     }
-    if (lane == 0) starts[groups] = (uint16_t)before;
+    if (lane == 0) starts[groups] = held(before);
 }
 
 // At most so many tiles of `height` rows, wherever the groups' edges lie.

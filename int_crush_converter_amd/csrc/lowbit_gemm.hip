@@ -295,17 +295,26 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
             x[i][1] = row[i][t * 8 + 4];
         }
     };
-    if (t0 < t1) load(t0);
     // the adapters' part of the wave's outputs, whose loads wait together with the first of the product
     // (with fewer tiles than waves a tile's ranks are shared among waves)
     constexpr int OWN = (MT * NT + WAVES - 1) / WAVES, SHARES = MT * NT < WAVES ? WAVES / (MT * NT) : 1;
     __shared__ lb_f32x4 shared[MODE == kAdapted && SHARES > 1 ? WAVES : 1][64];
     lb_f32x4 added[OWN];
+    const int own_wave = __builtin_amdgcn_readfirstlane(wave), u0 = own_wave % (MT * NT < WAVES ? MT * NT : WAVES);
+    int id[OWN];
     if constexpr (MODE == kAdapted) {
 #pragma unroll
         for (int k = 0; k < OWN; ++k) {
-            const int u = wave % (MT * NT < WAVES ? MT * NT : WAVES) + k * WAVES, m = m0 + u / NT * 16 + r, n = (nt0 + u % NT) * 16 + g * 4;
-            added[k] = m < m_end && n < p.N ? adapter_dot4(p.ad, p.N, m, n, SHARES > 1 ? wave / (MT * NT) : 0, SHARES) : lb_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const int u = u0 + k * WAVES, m = m0 + u / NT * 16 + r;
+            id[k] = u < MT * NT && m < m_end ? p.ad.ids[m] : -1;
+        }
+    }
+    if (t0 < t1) load(t0);
+    if constexpr (MODE == kAdapted) {
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            const int u = u0 + k * WAVES;
+            added[k] = adapter_tile(p.ad, p.N, m_end, m0 + u / NT * 16 + r, id[k], nt0 + u % NT, SHARES > 1 ? own_wave / (MT * NT) : 0, SHARES);
         }
         if (SHARES > 1) shared[wave][lane] = added[0];
     }
