@@ -1124,17 +1124,19 @@ int launch_linear(const Operands& p, hipStream_t st) {
 // has 101 (109), and 836 (847) where it has 801 (897): they lead by 13 % at best,
 // INT8 with 8 groups of 512 rows, and lose by up to 30 %.
 // Where 32 x 128 tiles would leave a third of the CUs idle, the wide form with
-// 32 rows: INT8 10 groups of 60 rows, 1000 x 2901, 15.1 against 21.9 (128 x 128);
-// INT4 one group of 64 rows, 4096 x 4096, 8.1 against 16.8, 4096 x 12288 12.3
-// against 35.5.  INT4 takes 32 x 128 tiles where there are up to 128 of 64 x 256:
-// 13 groups of 78 rows, 823 x 3662 (104), 22.9 against 29.6; 8 of 128 rows, 2816 x
-// 4096 (176), 36.2 against 27.0.  A K below 1024 has fewer steps than the wide
+// 32 rows, and for INT8, whose next are 128 x 128, up to 250 of them: 10 groups of
+// 70 rows, 1000 x 2901 (240), 16.7 against 21.7; 2 of 90, 4096 x 1024 (192), 10.8
+// and 13.2; 4 of 90, 2000 x 2000 (192), 17.7 and 17.6; 6 of 70, 2000 x 4096 (288),
+// 33.0 and 28.7; 2 of 128, 4096 x 1024 (256), 14.6 and 13.2.  INT4: one group of
+// 64 rows, 4096 x 4096, 8.1 against 16.8, 4096 x 12288 12.3 against 35.5; 32 x 128
+// tiles where there are up to 128 of 64 x 256: 13 groups of 78 rows, 823 x 3662
+// (104), 22.9 against 29.6; 8 of 128, 2816 x 4096 (176), 36.2 and 27.0.  A K below 1024 has fewer steps than the wide
 // form has waves: 16 groups of one row, 9668 x 120, 16.6 against 10.5 (64 x 256).
 int expert_form(int kind, int64_t rows, int64_t groups, int64_t N, int64_t K) {      // 1, 2 (wide), 32, 64, 128 or 256 (128 x 256)
     const int64_t met = rows < groups ? rows : groups, each = met ? cdiv(rows, met) : 0;
     const bool many = met * cdiv(N, 256) >= 256;
     if (each <= (!many ? 16 : K >= 1024 ? 2 : 0)) return 1;
-    if (met * cdiv(each, 32) * cdiv(N, 128) < 170) return 2;
+    if (met * cdiv(each, 32) * cdiv(N, 128) < (kind == kInt8 ? 250 : 170)) return 2;
     if (kind == kInt4 && met * cdiv(each, 64) * cdiv(N, 256) <= 128) return 32;
     const int64_t tiles = met * cdiv(each, 128) * cdiv(N, 256);
     if (kind == kInt4 ? each >= 256 && tiles >= 512 : tiles >= (each >= 128 ? 170 : 512)) return 256;
