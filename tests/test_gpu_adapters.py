@@ -95,6 +95,21 @@ def test_against_64_bits(gpu_dev, M, N, K, L, R, dtype, bits, asym):
     c.check(c.run(ids, c.bias, dtype), ids, c.bias)
 
 
+@pytest.mark.parametrize("R", [3, 8, 16, 24, 32, 40, 64, 100, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_that_share_adapters(gpu_dev, R, dtype):
+    """Few rows, from one adapter for all 16 of a tile to one for each, one after another and mixed, some with none."""
+    for M, N, L in ((3, 37, 2), (16, 200, 16), (33, 130, 5), (50, 3300, 9), (120, 68, 33)):
+        c = Case(gpu_dev, M, N, 150, L, R, 4, True, dtype, M + R)
+        for of in (1, 2, 4, L):                                   # so many adapters, of which neighbours are seldom the same
+            ids = torch.arange(M) % min(of, L)
+            c.check(c.run(ids), ids)
+            ids[torch.rand(M, generator=c.g) < 0.2] = -1
+            c.check(c.run(ids), ids)
+            ids = (torch.arange(M) * of // M).clamp(max=L - 1)    # and one after another
+            c.check(c.run(ids), ids)
+
+
 def test_sizes_reach_every_form(gpu_dev):
     """Tiles of 256 x 256 need K = 4096 here."""
     import int_crush_converter_amd._native as nat
