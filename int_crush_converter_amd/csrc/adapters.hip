@@ -90,7 +90,7 @@ __device__ __forceinline__ lb_f32x4 mma16(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc) 
 // the rows of a work-group are 32 or 48, whichever needs fewer rounds for its
 // height (32 rows left 6 of 262 work-groups for a second round: 56 us).  16 waves,
 // or two steps' loads in flight, made no difference.
-template <int DT, int MT, int RT, int WAVES>
+template <int DT, int MT, int RT, int WAVES, RankForm FORM>
 __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const int8_t* __restrict__ a, int64_t ld_a, const float* __restrict__ sa, int M,
                                                      const lb_u32x4* __restrict__ down, int64_t tiles, int rank, int adapters,
                                                      const float* __restrict__ scaling, const int32_t* __restrict__ offsets,
@@ -101,7 +101,8 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const int8_t* __rest
     // work-groups are dealt to the 8 XCDs in turn: each gets one run of rows, whose adapter its L2 keeps
     const int per = gridDim.x >> 3, extra = gridDim.x & 7, xcd = blockIdx.x & 7;
     const int at_run = xcd * per + (xcd < extra ? xcd : extra) + (blockIdx.x >> 3), rt0 = at_run % groups * RT;
-    if (blockIdx.x == 0 && threadIdx.x < parts * 64) t[(int64_t)M * parts * 64 + threadIdx.x] = 0;       // the row of zeros
+    constexpr int PITCH = FORM == kThree ? 128 : 64;   // of a row's part
+    if (blockIdx.x == 0 && threadIdx.x < parts * PITCH) t[(int64_t)M * parts * PITCH + threadIdx.x] = 0;       // the row of zeros
     const GroupTile tile = find_tile(offsets, adapters, M, 16 * MT, at_run / groups);
     if (tile.group < 0) return;
     auto row_of = [&](int i) {             // (rows past the last repeat the last)
@@ -149,35 +150,53 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const int8_t* __rest
         for (int k = 1; k < WAVES; ++k) s += part[k][u][lane];
         const int m = row_of(i);
         const float f = sa[m] * scaling[tile.group];
-        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+        const bool rest = rt == rts - 1 && rts % 2;    // of the last part: zeros
+        uint16_t* const row = t + ((int64_t)m * parts + rt / 2) * PITCH;
+        const int at = rt % 2 * 16 + g * 4;
+        lb_f32x4 v;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float v = rt * 16 + g * 4 + k < rank ? s[k] * f : 0.0f;
-            const uint32_t top = __float_as_uint(v) & 0xffff0000u, rest = pack_half_words<IC_DTYPE_BF16>(v - __uint_as_float(top), 0.0f);
-            hi[k >> 1] |= top >> (16 * (1 - (k & 1)));
-            lo[k >> 1] |= rest << (16 * (k & 1));
-        }
-        uint16_t* to = t + ((int64_t)m * parts + rt / 2) * 64 + rt % 2 * 16 + g * 4;
-        *reinterpret_cast<lb_u32x2*>(to) = lb_u32x2{hi[0], hi[1]};
-        *reinterpret_cast<lb_u32x2*>(to + kRankPart) = lb_u32x2{lo[0], lo[1]};
-        if (rt == rts - 1 && rts % 2) {                // the rest of the last part
-            *reinterpret_cast<lb_u32x2*>(to + 16) = lb_u32x2{0, 0};
-            *reinterpret_cast<lb_u32x2*>(to + kRankPart + 16) = lb_u32x2{0, 0};
+        for (int k = 0; k < 4; ++k) v[k] = rt * 16 + g * 4 + k < rank ? s[k] * f : 0.0f;
+        if constexpr (FORM == kWhole) {
+            lb_f32x4* to = reinterpret_cast<lb_f32x4*>(reinterpret_cast<float*>(row) + at);
+            to[0] = v;
+            if (rest) to[4] = lb_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        } else {
+            uint32_t value[4][2] = {};                 // hi, lo (kThree: the middle and the last 8 bits, zeros)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t hi = __float_as_uint(v[k]) & 0xffff0000u;
+                const float low = v[k] - __uint_as_float(hi);
+                const uint32_t mid = __float_as_uint(low) & 0xffff0000u, last = __float_as_uint(low - __uint_as_float(mid));
+                value[0][k >> 1] |= hi >> (16 * (1 - (k & 1)));
+                value[1][k >> 1] |= (FORM == kThree ? mid >> 16 : pack_half_words<IC_DTYPE_BF16>(low, 0.0f)) << (16 * (k & 1));
+                value[2][k >> 1] |= last >> 16 << (16 * (k & 1));
+            }
+#pragma unroll
+            for (int k = 0; k < PITCH / kRankPart; ++k) {
+                lb_u32x2* to = reinterpret_cast<lb_u32x2*>(row + k * kRankPart + at);
+                to[0] = lb_u32x2{value[k][0], value[k][1]};
+                if (rest) to[4] = lb_u32x2{0, 0};
+            }
         }
     }
 }
 
 }  // namespace
 
-int launch_shrink(const Adapted& ad, const int8_t* a, int64_t ld_a, const float* sa, int64_t M, int64_t K, const void* down, int rank,
+int launch_shrink(const Adapted& ad, RankForm form, const int8_t* a, int64_t ld_a, const float* sa, int64_t M, int64_t K, const void* down, int rank,
                   const float* scaling, const int32_t* offsets, const int32_t* order, hipStream_t st) {
     const lb_u32x4* d = static_cast<const lb_u32x4*>(down);
     const int64_t tiles = cdiv(K, kActPad) * 2;
-    auto go = [&](auto dt, auto mt, auto rt, auto waves) {
+    auto launch = [&](auto dt, auto mt, auto rt, auto waves, auto kept) {
         constexpr int MT = decltype(mt)::value, RT = decltype(rt)::value, WAVES = decltype(waves)::value;
         const dim3 grid((unsigned)(most_tiles(M, ad.adapters, 16 * MT) * cdiv(down_tiles(rank), RT)));
-        hipLaunchKernelGGL((shrink_kernel<decltype(dt)::value, MT, RT, WAVES>), grid, dim3(64 * WAVES), 0, st, a, ld_a, sa, (int)M, d, tiles, rank,
+        hipLaunchKernelGGL((shrink_kernel<decltype(dt)::value, MT, RT, WAVES, decltype(kept)::value>), grid, dim3(64 * WAVES), 0, st, a, ld_a, sa, (int)M, d, tiles, rank,
                            ad.adapters, scaling, offsets, order, ad.t);
+    };
+    auto go = [&](auto dt, auto mt, auto rt, auto waves) {
+        if (form == kTwo) launch(dt, mt, rt, waves, std::integral_constant<RankForm, kTwo>{});
+        else if (form == kWhole) launch(dt, mt, rt, waves, std::integral_constant<RankForm, kWhole>{});
+        else launch(dt, mt, rt, waves, std::integral_constant<RankForm, kThree>{});
     };
     auto shape = [&](auto dt) {
         typedef std::integral_constant<int, 1> c1;
@@ -215,7 +234,7 @@ extern "C" int64_t ic_adapter_up_bytes(int64_t adapters, int64_t N, int rank, in
 
 extern "C" int64_t ic_adapted_linear_workspace_bytes(int64_t M, int rank) {
     if (M < 0 || rank < 1 || rank > kMaxRank) return 0;
-    return (M + 1) * rank_parts(rank) * 128;
+    return (M + 1) * rank_parts(rank) * (M <= 64 ? 128 : 256);       // (tiles, which may ask for kThree, have more than 64 rows)
 }
 
 extern "C" int ic_adapter_pack(const void* a, const void* b, int dtype, int64_t adapters, int rank, int64_t N, int64_t K, void* down, void* up,

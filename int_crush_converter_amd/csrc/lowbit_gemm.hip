@@ -22,7 +22,8 @@ namespace icq {
 namespace {
 
 enum Kind { kInt8 = 0, kInt4 = 1, kMx = 2 };
-enum Mode { kPlain, kGrouped, kAdapted };
+enum Mode { kPlain, kGrouped, kAdapted, kAdaptedWhole };       // (kAdaptedWhole: t to its last bit, for fp32 results)
+constexpr bool adapted(int mode) { return mode == kAdapted || mode == kAdaptedWhole; }
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -298,11 +299,11 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
     // the adapters' part of the wave's outputs, whose loads wait together with the first of the product
     // (with fewer tiles than waves a tile's ranks are shared among waves)
     constexpr int OWN = (MT * NT + WAVES - 1) / WAVES, SHARES = MT * NT < WAVES ? WAVES / (MT * NT) : 1;
-    __shared__ lb_f32x4 shared[MODE == kAdapted && SHARES > 1 ? WAVES : 1][64];
+    __shared__ lb_f32x4 shared[adapted(MODE) && SHARES > 1 ? WAVES : 1][64];
     lb_f32x4 added[OWN];
     const int own_wave = __builtin_amdgcn_readfirstlane(wave), u0 = own_wave % (MT * NT < WAVES ? MT * NT : WAVES);
     int id[OWN];
-    if constexpr (MODE == kAdapted) {
+    if constexpr (adapted(MODE)) {
 #pragma unroll
         for (int k = 0; k < OWN; ++k) {
             const int u = u0 + k * WAVES, m = m0 + u / NT * 16 + r;
@@ -310,11 +311,11 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
         }
     }
     if (t0 < t1) load(t0);
-    if constexpr (MODE == kAdapted) {
+    if constexpr (adapted(MODE)) {
 #pragma unroll
         for (int k = 0; k < OWN; ++k) {
             const int u = u0 + k * WAVES;
-            added[k] = adapter_tile(p.ad, p.N, m_end, m0 + u / NT * 16 + r, id[k], nt0 + u % NT, SHARES > 1 ? own_wave / (MT * NT) : 0, SHARES);
+            added[k] = adapter_tile<MODE == kAdaptedWhole>(p.ad, p.N, m_end, m0 + u / NT * 16 + r, id[k], nt0 + u % NT, SHARES > 1 ? own_wave / (MT * NT) : 0, SHARES);
         }
         if (SHARES > 1) shared[wave][lane] = added[0];
     }
@@ -364,8 +365,8 @@ __global__ __launch_bounds__(512) void linear_wide_kernel(Operands p) {
         const int from = source_row<MODE>(p, m);
         const i32x4 s = {sum[u][0][lane], sum[u][1][lane], sum[u][2][lane], sum[u][3][lane]};
         lb_f32x4 y = cols.finish(s, p.sa[from], p.zp ? p.sums[from] : 0);
-        if constexpr (MODE == kAdapted && SHARES == 1) y += added[own];
-        else if constexpr (MODE == kAdapted) {
+        if constexpr (adapted(MODE) && SHARES == 1) y += added[own];
+        else if constexpr (adapted(MODE)) {
             lb_f32x4 a = shared[u][lane];
 #pragma unroll
             for (int k = 1; k < SHARES; ++k) a += shared[u + k * MT * NT][lane];
@@ -429,7 +430,7 @@ __device__ __forceinline__ void meet() {
 // adapters' products block by block behind the K loop, each waiting for its
 // operands from L2, took 437 us.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE = kPlain>
-__global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
+__global__ __launch_bounds__(64 * WM * WN, adapted(MODE) || FM == 4 ? 2 : 1) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
     typedef typename Acc32<KIND>::T acc_t;
     constexpr int WAVES = WM * WN, BM = 32 * WM * FM, BN = 32 * WN * FN;
     constexpr int X_KB = BM / 16 * (KIND == kInt4 ? 2 : 1), W_KB = BN / 16;      // a stage's KB
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
     // (and a group's first row of tiles)
     constexpr int SCALES = BUF * STAGE, COLS = SCALES + 2 * S_WORDS, ROWS = COLS + BN * 3 / 4, GROUPS = ROWS + (KIND == kMx ? 0 : BM / 2);
     // (kAdapted: each row's adapter, and which of the adapters the rows have, a bit each, for two tiles in turn)
-    __shared__ lb_u32x4 lds[GROUPS + (MODE == kGrouped ? kMaxGroups / 8 + 1 : MODE == kAdapted ? BM / 4 + kMaxGroups / 64 : 0)];
+    __shared__ lb_u32x4 lds[GROUPS + (MODE == kGrouped ? kMaxGroups / 8 + 1 : adapted(MODE) ? BM / 4 + kMaxGroups / 64 : 0)];
     int* const row_id = reinterpret_cast<int*>(lds + GROUPS);
     unsigned* const present = reinterpret_cast<unsigned*>(lds + GROUPS + BM / 4);
     float* const col = reinterpret_cast<float*>(lds + COLS);
@@ -550,10 +551,12 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
         __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, lane_off, off, 0, 0);
     };
     // kAdapted.  Behind the stages of K come those of each adapter that the tile's rows have: an operand of t lies like one
-    // of the activations (INT4: 32 ranks of hi and of lo in a stage, INT8: of one of them), one of B like one of the
+    // of the activations (INT4: 32 ranks of two of t's values in a stage, INT8: of one of them), one of B like one of the
     // weights.  Rows with another adapter or none take the row of zeros.  Fetched one after another: adapter `ad_now`,
     // its stage `ad_stage`.
-    const int ad_planes = p.ad.f16 ? 2 : 1, ad_stages = p.ad.parts * ad_planes * (KIND == kInt8 ? 2 : 1);
+    constexpr int T_BYTES = MODE == kAdaptedWhole ? 256 : 128;                    // of a row's part of t (kThree or kTwo), and its stages
+    constexpr int T_STAGES = KIND == kInt8 ? (MODE == kAdaptedWhole ? 3 : 2) : T_BYTES / 128;
+    const int ad_planes = p.ad.f16 ? 2 : 1, ad_stages = p.ad.parts * ad_planes * T_STAGES;
     int ad_now = -1, ad_stage = 0, ad_set = 0;
     auto next_adapter = [&]() {                            // the lowest in the set above ad_now (there is one)
         const unsigned* set = present + ad_set * (kMaxGroups / 32);
@@ -564,11 +567,12 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
         ad_now = first * 32 + __builtin_ctz((unsigned)__builtin_amdgcn_readlane((int)w, first));
     };
     auto fetch_adapter = [&](int buf) {
-        if constexpr (MODE == kAdapted) {
+        if constexpr (adapted(MODE)) {
             if (ad_stage == 0) next_adapter();
             lb_u32x4* to = lds + buf * STAGE + wave * 64;
-            const int half = KIND == kInt8 ? ad_stage & 1 : 0, tile_of = KIND == kInt8 ? ad_stage >> 1 : ad_stage;   // (tile_of: part and plane)
-            const int pitch = p.ad.parts * 128, part = tile_of / ad_planes, from = part * 128 + half * 64;
+            const int tile_of = ad_stage / T_STAGES;       // (part and plane)
+            const int pitch = p.ad.parts * T_BYTES, part = tile_of / ad_planes;
+            const int from = part * T_BYTES + (ad_stage - tile_of * T_STAGES) * (KIND == kInt8 ? 64 : 128);
             const int lane_row = KIND == kInt4 ? lane >> 3 : lane >> 2;
             const int chunk = KIND == kInt4 ? (lane & 7) ^ ((wave & 1) * 4 + (lane >> 4)) : (lane & 3) ^ (lane >> 4);
             const __amdgpu_buffer_rsrc_t t_buf = buffer(p.ad.t);
@@ -588,7 +592,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
         }
     };
     auto fetch = [&](int t, int buf) {
-        if (MODE == kAdapted && t >= k_stages) {
+        if (adapted(MODE) && t >= k_stages) {
             fetch_adapter(buf);
             return;
         }
@@ -662,7 +666,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
             }
         }
         if (p.bias) c_bias = load_as_f32(p.bias, p.bias_dtype, n);
-        if constexpr (MODE == kAdapted) {                  // (K has BUF - 1 stages at least; the set is read behind the next barrier)
+        if constexpr (adapted(MODE)) {                  // (K has BUF - 1 stages at least; the set is read behind the next barrier)
             int id = tid < BM && row0 + tid < row_end ? p.ad.ids[row0 + tid] : -1;
             if (id >= p.ad.adapters) id = -1;
             if (tid < BM) row_id[tid] = id;
@@ -733,14 +737,14 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
         }
     };
 
-    if constexpr (MODE == kAdapted) {
+    if constexpr (adapted(MODE)) {
         if (threadIdx.x < kMaxGroups / 16) present[threadIdx.x] = 0;
         lds_barrier();
     }
     start();
     meet<0>();
     for (;;) {
-        if constexpr (MODE == kAdapted) {
+        if constexpr (adapted(MODE)) {
             const int own = lane < 32 ? __builtin_popcount(present[ad_set * (kMaxGroups / 32) + lane]) : 0;
             stages = k_stages + __builtin_amdgcn_readlane(wave_scan(own), 63) * ad_stages;
             ad_now = -1;
@@ -802,7 +806,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
             stage(0, std::true_type{}, std::true_type{});
 #pragma unroll 1
             for (int t = 1; t < k_stages; ++t) stage(t, std::false_type{}, std::true_type{});
-            if constexpr (MODE == kAdapted) {
+            if constexpr (adapted(MODE)) {
                 whole_values();
 #pragma unroll 1
                 for (int t = k_stages; t < stages; ++t) stage(t, std::false_type{}, std::false_type{});
@@ -849,7 +853,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
             } else {
 #pragma unroll 1
                 for (int t = 1; t < k_stages; ++t) stage(t, std::integral_constant<int, 1>{}, std::false_type{}, std::true_type{});
-                if constexpr (MODE == kAdapted) {
+                if constexpr (adapted(MODE)) {
                     whole_values();
 #pragma unroll 1
                     for (int t = k_stages; t < stages; ++t) stage(t, std::integral_constant<int, 1>{}, std::false_type{}, std::false_type{});
@@ -896,13 +900,13 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
                             const int c = cw + j * 32 + q * 16 + h * 8 + k * 4;
                             const lb_f32x4 bias = *reinterpret_cast<const lb_f32x4*>(col + c);
                             lb_f32x4 sw = {}, zero = {};
-                            if (KIND != kMx && MODE != kAdapted) {
+                            if (KIND != kMx && !adapted(MODE)) {
                                 sw = *reinterpret_cast<const lb_f32x4*>(col + BN + c);
                                 zero = *reinterpret_cast<const lb_f32x4*>(col + 2 * BN + c);
                             }
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                if constexpr (MODE == kAdapted) v[k][e] = __int_as_float(acc[i][j][8 * q + 4 * k + e]);
+                                if constexpr (adapted(MODE)) v[k][e] = __int_as_float(acc[i][j][8 * q + 4 * k + e]);
                                 else v[k][e] = value(acc[i][j][8 * q + 4 * k + e], sw[e], zero[e], bias[e], sa, sum);
                             }
                         }
@@ -950,7 +954,7 @@ __global__ __launch_bounds__(64 * WM * WN, MODE == kAdapted || FM == 4 ? 2 : 1) 
                     if (n0 + n >= p.N) continue;
                     const sum_t s = area[m * PITCH + n];
                     const int c = wn * FN * 32 + n, o = wm * FM * 32 + i * 32 + m;
-                    const float v = MODE == kAdapted ? __builtin_bit_cast(float, s)
+                    const float v = adapted(MODE) ? __builtin_bit_cast(float, s)
                                     : KIND == kMx    ? value(s, 0.0f, 0.0f, col[c], 0.0f, 0.0f)
                                                      : value(s, col[BN + c], col[2 * BN + c], col[c], row[o], row[BM + o]);
                     store_from_f32(p.out, p.out_dtype, (m0 + i * 32 + m) * p.ld_out + n0 + n, v);
@@ -1048,20 +1052,26 @@ int linear_form(int kind, int64_t M, int64_t N) {      // 0, 128 or 256
     return tiles * 12 >= rounds * 256 * (kind == kInt4 ? 8 : 9) ? 256 : 128;
 }
 
+template <int KIND> constexpr int kBuffers = KIND == kInt4 ? 3 : 4;
+
+// The same for adapted products.  The end of a tile takes longer, which two
+// work-groups a CU hide: 256 x 256 from K = 4096 on, and where they fill three
+// quarters of their rounds.  128 against 256, INT4 / INT8, rank 16 where not said,
+// us: 8192 x 4096 x 1024 68 to 77 / 75 to 87; 2304 x 4096 x 2048 43 to 51 / 47 to
+// 58; 4096 x 4096 x 4096 90 to 89 / 100 to 99; 8192 x 4096 x 4096 rank 64 173 to
+// 165 / 189 to 184; 8192 x 4100 x 4096 (0.71) 192 to 242.
+int adapted_form(int kind, int64_t M, int64_t N, int64_t K) {
+    // (a tile's adapters are known when all but one of the buffers have been asked for)
+    if (cdiv(K, kind == kInt8 ? 64 : 128) < (kind == kInt8 ? kBuffers<kInt8> : kBuffers<kInt4>) - 1) return 0;
+    const int form = linear_form(kind, M, N);
+    const int64_t tiles = cdiv(M, 256) * cdiv(N, 256);
+    return form == 256 && (K < 4096 || (tiles > 256 && tiles * 12 < cdiv(tiles, 256) * 256 * 9)) ? 128 : form;
+}
+
 template <int KIND, int MODE = kPlain>
 int launch_linear(const Operands& p, hipStream_t st) {
-    constexpr int BUF = KIND == kInt4 ? 3 : 4;
-    int form = linear_form(KIND, p.M, p.N);
-    if constexpr (MODE == kAdapted) {
-        // The end of a tile takes longer, which two work-groups a CU hide: 256 x 256 from K = 4096 on, and where they fill
-        // three quarters of their rounds.  128 against 256, INT4 / INT8, rank 16 where not said, us: 8192 x 4096 x 1024 68
-        // to 77 / 75 to 87; 2304 x 4096 x 2048 43 to 51 / 47 to 58; 4096 x 4096 x 4096 90 to 89 / 100 to 99; 8192 x 4096
-        // x 4096 rank 64 173 to 165 / 189 to 184; 8192 x 4100 x 4096 (0.71) 192 to 242.
-        const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256);
-        if (form == 256 && (p.K < 4096 || (tiles > 256 && tiles * 12 < cdiv(tiles, 256) * 256 * 9))) form = 128;
-        // (a tile's adapters are known when BUF - 1 stages of it have been asked for)
-        if (cdiv(p.K, KIND == kInt8 ? 64 : 128) < BUF - 1) form = 0;
-    }
+    constexpr int BUF = kBuffers<KIND>;
+    const int form = adapted(MODE) ? adapted_form(KIND, p.M, p.N, p.K) : linear_form(KIND, p.M, p.N);
     if (form == 256) launch_tiled<KIND, 2, 4, 4, 2, BUF, MODE>(p, st);
     else if (form == 128) launch_tiled<KIND, 2, 2, 2, 2, BUF, MODE>(p, st);
     else if constexpr (MODE == kPlain) {
@@ -1146,7 +1156,7 @@ int expert_form(int kind, int64_t rows, int64_t groups, int64_t N, int64_t K) { 
 template <int KIND>
 int launch_experts(const Operands& p, hipStream_t st) {
     const int form = expert_form(KIND, p.M, p.groups, p.N, p.K);
-    constexpr int BUF = KIND == kInt4 ? 3 : 4;
+    constexpr int BUF = kBuffers<KIND>;
     if (form == 256) launch_tiled<KIND, 1, 4, 4, 2, BUF - 1, kGrouped>(p, st);
     else if (form >= 32) {
         if constexpr (KIND == kInt8) launch_tiled<KIND, 2, 2, 2, 2, BUF, kGrouped>(p, st);
@@ -1286,8 +1296,11 @@ extern "C" int ic_adapted_linear(const int8_t* a, int64_t ld_a, const float* sa,
     ProfScope prof(st, PT_OTHER, 2.0 * M * N * K + 2.0 * M * rank * (N + K), (double)M * K + (double)N * K * bits / 8);
     p.ad = Adapted{ids, static_cast<uint16_t*>(workspace), static_cast<const uint8_t*>(up), adapter_dtype == IC_DTYPE_F16, rank_parts(rank), (int)adapters,
                    (rank + 7) / 8};
-    if (const int rc = launch_shrink(p.ad, a, ld_a, sa, M, K, down, rank, scaling, offsets, order, st)) return rc;
-    return bits == 8 ? launch_linear<kInt8, kAdapted>(p, st) : launch_linear<kInt4, kAdapted>(p, st);
+    const bool whole = out_dtype == IC_DTYPE_F32;
+    const RankForm kept = !whole ? kTwo : adapted_form(bits == 8 ? kInt8 : kInt4, M, N, K) ? kThree : kWhole;
+    if (const int rc = launch_shrink(p.ad, kept, a, ld_a, sa, M, K, down, rank, scaling, offsets, order, st)) return rc;
+    if (bits == 8) return whole ? launch_linear<kInt8, kAdaptedWhole>(p, st) : launch_linear<kInt8, kAdapted>(p, st);
+    return whole ? launch_linear<kInt4, kAdaptedWhole>(p, st) : launch_linear<kInt4, kAdapted>(p, st);
 }
 
 extern "C" int ic_mxfp4_linear(const void* a, const void* a_scales, int64_t M, const void* w, const void* w_scales,

@@ -39,6 +39,11 @@ def _bias(bias: torch.Tensor | None, N: int):
     return b, nat.dtype_code(b)
 
 
+def _adapted_workspace(rows: int, rank: int) -> int:
+    """ic_adapted_linear_workspace_bytes without the call, in fp32 values."""
+    return (rows + 1) * -(-rank // 32) * (32 if rows <= 64 else 64)
+
+
 def _unpermuted(rows: torch.Tensor, permutation: torch.Tensor, bits: int, K: int) -> torch.Tensor:
     """Stored rows with their columns where they were before the converter permuted them: column j of the first
     len(permutation) goes to permutation[j]."""
@@ -124,7 +129,7 @@ def quantized_linear(x: QuantizedActivations, weight: QuantizedWeight, bias: tor
                          f"{rows} rows with one among {ad.count} adapters")
     nat.stream_for(ad.down, ad.up, ad.scaling, groups.data)
     out = torch.empty((*x.lead, N), dtype=out_dtype, device=data.device)
-    ws = torch.empty((rows + 1) * -(-ad.rank // 32) * 32, dtype=torch.float32, device=data.device)    # ic_adapted_linear_workspace_bytes
+    ws = torch.empty(_adapted_workspace(rows, ad.rank), dtype=torch.float32, device=data.device)
     ids, offsets, order, _ = groups.pointers()
     call("ic_adapted_linear", data.data_ptr(), data.shape[1], m, m + 4 * rows, rows, w.tiles.data_ptr(), w.bits,
          w.scales.data_ptr(), w.scale_kind, None if z is None else z.data_ptr(), None if b is None else b.data_ptr(),
