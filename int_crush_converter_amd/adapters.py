@@ -18,7 +18,7 @@ MAX_RANK = 128
 
 class LowRankAdapters:
     """The adapters of one layer: a [count, rank, in_features] and b [count, out_features, rank], both bfloat16 or both
-    float16, and their scaling (a number, or [count]).
+    float16, and their scaling (a number, or [count]); copies are kept.
 
     Beside a rotated weight the activations are rotated too: give ``rotate_weights(a, rot_size)`` there, whose rows are
     padded like the activations'.  Adapters of smaller rank are padded with zeros to the largest.  b has to be finite; Inf
@@ -42,7 +42,7 @@ class LowRankAdapters:
             if scaling.numel() not in (1, n):
                 raise ValueError(f"{scaling.numel()} scalings for {n} adapters")
             s = nat.on_gpu("scaling", scaling).float().reshape(-1)
-            self.scaling = s.expand(n).contiguous()
+            self.scaling = s.expand(n).clone(memory_format=torch.contiguous_format)
         else:
             self.scaling = torch.full((n,), float(scaling), dtype=torch.float32, device=a.device)
         self.count, self.rank, self.in_features, self.out_features = n, r, K, N
