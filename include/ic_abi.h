@@ -553,9 +553,10 @@ int ic_combine_rows(const void* y, int dtype, int64_t tokens, int64_t top, int64
 /* ic_quantized_linear with a weight for each group: row i of out, the place i
  * of an order by group, is the product of a row of the activations with the
  * weight of its group: of row i (top 0; a_rows = rows), or of row order[i] /
- * top (top > 0; a_rows * ld_a below 2^32).  tiles, sw, zp, bias [groups, N]:
- * those of all groups, one after another (tiles ic_linear_weight_bytes()
- * each).  Rows of out behind offsets[groups] are left as they were. */
+ * top (top > 0; a_rows * ld_a below 2^32; the last row where order names none of
+ * them).  tiles, sw, zp, bias [groups, N]: those of all groups, one after another
+ * (tiles ic_linear_weight_bytes() each).  Rows of out behind offsets[groups] are
+ * left as they were. */
 int ic_expert_linear(const int8_t* a, int64_t ld_a, const float* sa, const int32_t* sums, int64_t a_rows,
                      const int32_t* offsets, const int32_t* order, int top, int64_t groups, int64_t rows,
                      const void* tiles, int bits, const void* sw, int sw_kind, const int8_t* zp, const void* bias,

@@ -55,12 +55,13 @@ struct Operands {
     Adapted ad;              // kAdapted
 };
 
-// The row of activations that row m of y comes from.
+// The row of activations that row m of y comes from (the last, where the order
+// names none of them: -1 / 1 is past the last as an unsigned number too).
 template <int MODE>
 __device__ __forceinline__ int source_row(const Operands& p, int m) {
     if (MODE != kGrouped || !p.top) return m;
-    const int s = (int)((unsigned)p.order[m] / (unsigned)p.top);
-    return s < p.a_rows ? s : p.a_rows - 1;
+    const unsigned s = (unsigned)p.order[m] / (unsigned)p.top;
+    return s < (unsigned)p.a_rows ? (int)s : p.a_rows - 1;
 }
 
 template <int KIND> struct Acc { typedef i32x4 T; };
