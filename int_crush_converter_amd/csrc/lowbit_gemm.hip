@@ -710,7 +710,9 @@ __global__ __launch_bounds__(64 * WM * WN, adapted(MODE) || FM == 4 ? 2 : 1) voi
             return (float)(int)d * (sa * sw) + bias;
         }
     };
-    // kAdapted: whole values in place of the sums, before the adapters' stages
+    // kAdapted: whole values in place of the sums, before the adapters' stages.  (Each matrix instruction that follows
+    // rounds the value: four for 32 ranks, six or eight with t whole, twice as many with fp16 factors.  A sum of the
+    // adapters' part alone would take as many registers again as the sums have, and at 256 x 256 they have all.)
     auto whole_values = [&]() {
         // (two addresses, made here: the compiler would keep 80 of them over the K loop, spilled)
         const float* my_col = col + wn * FN * 32 + h * 8;

@@ -52,3 +52,60 @@ def test_t_has_all_its_bits(gpu_dev, M, N, K, L, R, used, bits, dtype):
 def test_sizes_reach_every_form(gpu_dev):
     import int_crush_converter_amd._native as nat
     assert {(nat.lib().ic_linear_form(k, m, n), d >= 4096) for m, n, d, _, _, _ in EXACT for k in (0, 1)} >= {(0, False), (128, False), (256, False), (256, True)}
+
+
+class Parts:
+    """A product and adapters whose base and added part are known in 64 bits, with the magnitudes of the part's sums."""
+
+    def __init__(self, dev, M, N, K, L, R, bits, dtype, a, b, scaling, weight, seed):
+        import int_crush_converter_amd as icq
+        g = torch.Generator().manual_seed(seed)
+        codes, sa = torch.randint(-128, 128, (M, K), generator=g).to(torch.int8), torch.rand(M, generator=g) * 0.01 + 1e-4
+        q = torch.randint(-8, 8, (N, K), generator=g).to(torch.int8) * weight
+        a, b = (torch.randn(L, R, K, generator=g) * a).to(dtype), (torch.randn(L, N, R, generator=g) * b).to(dtype)
+        s = (torch.rand(L, generator=g) + 0.5) * scaling
+        ids = torch.randint(-1, L, (M,), generator=g)
+        u = torch.nn.functional.pad(q, (0, K % 2)).view(torch.uint8) & 15
+        w = icq.QuantizedWeight((u[:, 0::2] | (u[:, 1::2] << 4) if bits == 4 else q).to(dev), torch.ones(N, device=dev), in_features=K)
+        act = icq.QuantizedActivations.from_codes(codes.to(dev), sa.to(dev))
+        y = icq.quantized_linear(act, w, adapters=icq.LowRankAdapters(a.to(dev), b.to(dev), s.to(dev)),
+                                 groups=icq.group_rows(ids.to(dev), L), out_dtype=F32)
+        self.y, x = y.cpu().double(), codes.double() * sa.double()[:, None]
+        self.base, self.added, self.room = x @ q.double().T, torch.zeros(M, N, dtype=torch.float64), torch.zeros(M, N, dtype=torch.float64)
+        for n in range(L):
+            at = (ids == n).nonzero()[:, 0]
+            self.added[at] = s[n].double() * (x[at] @ a[n].double().T) @ b[n].double().T
+            self.room[at] = s[n].double() * (x[at].abs() @ a[n].double().abs().T) @ b[n].double().abs().T
+        # t: K products and some joins and scalings; d: three values of t and two of b for each of the padded ranks, and joins
+        self.room *= (K + 8 + 6 * -(-R // 32) * 32 + 200) * 2.0 ** -23
+
+
+@pytest.mark.parametrize("M,N,K", [(20, 64, 200), (70, 1000, 200), (1500, 1400, 200), (2100, 4000, 4200)])
+@pytest.mark.parametrize("bits,dtype,a,b,scaling", [(8, BF16, 1.0, 1.0, 1e-30), (4, F16, 1.0, 1.0, 1e-30), (8, F16, 1e-3, 1.0, 1e-12), (4, BF16, 1e-3, 1.0, 1e-12),
+                                                    (4, F16, 1e-6, 1e-6, 1.0), (8, F16, 1e-6, 1e-6, 1e-6), (8, BF16, 1e-20, 1e-6, 1.0), (4, F16, 1.0, 1e3, 1e12)])
+def test_small_and_large_adapters_alone(gpu_dev, M, N, K, bits, dtype, a, b, scaling):
+    """The weight is of zeros, so that nothing but the adapters' own sums gives room: a part that is lost or flushed to zero
+    shows at any magnitude (1e-6 is below float16's normal numbers).  Products below fp32's smallest normal number 2^-126
+    count as lost: the values here are above 2^-126 by 2^24 and more, but for those far below their row's others."""
+    c = Parts(gpu_dev, M, N, K, 2, 16, bits, dtype, a, b, scaling, 0, M + bits)
+    assert (c.base == 0).all() and c.added.abs().max() > 0
+    assert ((c.y - c.added).abs() <= c.room).all()
+    assert (c.y[c.added == 0] == 0).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(20, 64, 200), (64, 14400, 136), (1500, 1400, 200), (2100, 4000, 4200)])
+@pytest.mark.parametrize("bits,dtype", [(4, BF16), (8, BF16), (4, F16), (8, F16)])
+@pytest.mark.parametrize("share", [1e-2, 1e-3])
+def test_small_adapters_beside_a_large_product(gpu_dev, M, N, K, bits, dtype, share):
+    """The forms for few rows add the adapters' part once.  The tiled ones add it to the value as the matrix instructions go:
+    at most one rounding or truncation of the value, 2^-23 of it, for each product: 16 ranks (padded to 32), three values of t
+    and a plane of zeros, and as many again for the second plane of float16 factors.  2^-21: the value's own roundings."""
+    R = 16
+    size = (share / (R * 200) ** 0.5 * 5) ** 0.5                    # base: sqrt(K) 5 sa |q|; part: sqrt(R K) a b sa |q|
+    c = Parts(gpu_dev, M, N, K, 2, R, bits, dtype, size, size, 1.0, 1, M)
+    planes = 32 * 4 * (1 if dtype == BF16 else 2)
+    tiled = M > 100
+    value = c.base.abs() + (c.added.abs() + c.room if tiled else 0)
+    room = c.room + value * (2.0 ** -21 + (planes * 2.0 ** -23 if tiled else 0)) + c.added.abs() * 2.0 ** -22
+    assert ((c.y - c.base - c.added).abs() <= room).all()
+    assert (c.added.abs() > 2 * room).any()                        # (a part that is lost would show)
