@@ -164,7 +164,11 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(const int8_t* __rest
             uint32_t value[4][2] = {};                 // hi, lo (kThree: the middle and the last 8 bits, zeros)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint32_t hi = __float_as_uint(v[k]) & 0xffff0000u;
+                uint32_t hi = __float_as_uint(v[k]) & 0xffff0000u;
+                if (FORM == kTwo) {                    // the nearest, if it is finite: half the rest, with a sign, for lo
+                    const uint32_t near = pack_half_words<IC_DTYPE_BF16>(0.0f, v[k]) & 0xffff0000u;
+                    hi = (near & 0x7fffffffu) == 0x7f800000u ? hi : near;
+                }
                 const float low = v[k] - __uint_as_float(hi);
                 const uint32_t mid = __float_as_uint(low) & 0xffff0000u, last = __float_as_uint(low - __uint_as_float(mid));
                 value[0][k >> 1] |= hi >> (16 * (1 - (k & 1)));

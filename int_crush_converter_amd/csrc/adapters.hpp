@@ -11,8 +11,9 @@ constexpr int kRankPart = 32;           // ranks are padded to parts of 32 with 
 __host__ __device__ inline int rank_parts(int rank) { return (rank + kRankPart - 1) / kRankPart; }
 
 // How t is kept goes by the result.  A 16-bit result has 8 or 11 bits: t as two
-// bf16 values, hi + lo (hi by truncation, which cannot overflow), within 2^-16 of
-// it, is what the matrix cores take as it lies.  An fp32 result has t whole: in
+// bf16 values, each the nearest to what is left (the first by truncation where the
+// nearest is infinite), within 2^-18 of it, is what the matrix cores take as it
+// lies.  An fp32 result has t whole: in
 // fp32 for the forms for few rows, which split it in registers, and for the tiled
 // ones, whose stages go straight to LDS, as three bf16 values of 8 bits each.
 // They are exact where the last is one (|t| >= 2^-110).

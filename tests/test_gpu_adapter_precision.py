@@ -49,6 +49,59 @@ def test_t_has_all_its_bits(gpu_dev, M, N, K, L, R, used, bits, dtype):
     assert torch.equal(y.cpu().double(), want)
 
 
+@pytest.mark.parametrize("M,N,K,L,R,used", [c[:2] + (140,) + c[3:] for c in EXACT if c[2] < 4096])
+@pytest.mark.parametrize("bits,dtype", [(4, BF16), (8, BF16), (4, F16), (8, F16)])
+def test_t_of_sixteen_bit_results(gpu_dev, M, N, K, L, R, used, bits, dtype):
+    """t as two bfloat16 values, each the nearest, has whole numbers below 2^17: the first leaves at most 2^8.  The product
+    beside it is -t and at most two codes, so that the result is a whole number up to 254, which bfloat16 has too; a t that
+    is off by one shows."""
+    import int_crush_converter_amd as icq
+    g = torch.Generator().manual_seed(M + N + R)
+    codes = torch.randint(100, 128, (M, K), generator=g).to(torch.int8)
+    rows = torch.randint(5, 8, (R, K), generator=g)                        # t: 140 x 100 x 5 = 2^16.1 to 140 x 127 x 7 < 2^17
+    q = -rows[torch.arange(N) % R]
+    q[torch.arange(N)[:, None], torch.randint(0, K, (N, 1), generator=g)] += 1
+    q[torch.arange(N), torch.randint(0, K, (N,), generator=g)] += 1
+    q = q.to(torch.int8)
+    place = torch.stack([torch.randperm(R, generator=g) for _ in range(L)])   # adapter l has row r at place[l, r]
+    a = torch.zeros(L, R, K).scatter_(1, place[:, :, None].expand(L, R, K), rows.float()[None].expand(L, R, K).contiguous()).to(dtype)
+    b = torch.zeros(L, N, R).scatter_(2, place[:, torch.arange(N) % R][:, :, None], 1.0).to(dtype)
+    ids = torch.randint(-1, used, (M,), generator=g)
+    u = q.view(torch.uint8) & 15
+    w = icq.QuantizedWeight((u[:, 0::2] | (u[:, 1::2] << 4) if bits == 4 else q).to(gpu_dev), torch.ones(N, device=gpu_dev), in_features=K)
+    act = icq.QuantizedActivations.from_codes(codes.to(gpu_dev), torch.ones(M, device=gpu_dev))
+    want = codes.double() @ q.double().T
+    t = codes.double() @ rows.double().T
+    assert (t < 2 ** 17).all() and (t >= 2 ** 16).all()
+    want[ids >= 0] += t[ids >= 0][:, torch.arange(N) % R]
+    assert (want[ids >= 0].abs() <= 254).all()
+    ad, groups = icq.LowRankAdapters(a.to(gpu_dev), b.to(gpu_dev)), icq.group_rows(ids.to(gpu_dev), L)
+    for out in (BF16, F16):
+        y = icq.quantized_linear(act, w, adapters=ad, groups=groups, out_dtype=out)
+        assert torch.equal(y.cpu(), want.float().to(out))
+
+
+def test_the_largest_t(gpu_dev):
+    """t within 2^-9 of fp32's largest value, whose nearest bfloat16 value is infinite."""
+    import int_crush_converter_amd as icq
+    K, N = 128, 32
+    w = icq.QuantizedWeight(torch.zeros(N, K, dtype=torch.int8, device=gpu_dev), torch.ones(N, device=gpu_dev))
+    a, b = torch.zeros(1, 1, K, dtype=BF16), torch.full((1, N, 1), 2.0 ** -40, dtype=BF16)
+    a[0, 0, 0] = 1.0
+    top = torch.finfo(F32).max
+    for scale in (top, -top, top * (1 - 2.0 ** -10), top * (1 - 2.0 ** -8)):
+        ad = icq.LowRankAdapters(a.to(gpu_dev), b.to(gpu_dev), scale)
+        for M in (3, 700):
+            codes = torch.zeros(M, K, dtype=torch.int8)
+            codes[:, 0] = 1
+            act = icq.QuantizedActivations.from_codes(codes.to(gpu_dev), torch.ones(M, device=gpu_dev))
+            groups = icq.group_rows(torch.zeros(M, dtype=torch.int32, device=gpu_dev), 1)
+            want = torch.tensor(scale, dtype=F32).double() * 2.0 ** -40
+            for out, room in ((F32, 2.0 ** -22), (BF16, 2.0 ** -8 + 2.0 ** -15)):
+                y = icq.quantized_linear(act, w, adapters=ad, groups=groups, out_dtype=out)
+                assert ((y.cpu().double() - want).abs() <= want.abs() * room).all(), (scale, M, out)
+
+
 def test_sizes_reach_every_form(gpu_dev):
     import int_crush_converter_amd._native as nat
     assert {(nat.lib().ic_linear_form(k, m, n), d >= 4096) for m, n, d, _, _, _ in EXACT for k in (0, 1)} >= {(0, False), (128, False), (256, False), (256, True)}
