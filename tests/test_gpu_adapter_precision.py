@@ -162,3 +162,24 @@ def test_small_adapters_beside_a_large_product(gpu_dev, M, N, K, bits, dtype, sh
     room = c.room + value * (2.0 ** -21 + (planes * 2.0 ** -23 if tiled else 0)) + c.added.abs() * 2.0 ** -22
     assert ((c.y - c.base - c.added).abs() <= room).all()
     assert (c.added.abs() > 2 * room).any()                        # (a part that is lost would show)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_as_many_rows_as_there_may_be(gpu_dev, bits):
+    """The largest batch and rank, t whole: a workspace of 1 GB, and whole numbers as above."""
+    import int_crush_converter_amd as icq
+    g = torch.Generator(device=gpu_dev).manual_seed(bits)
+    M, N, K, L, R = 1048560, 16, 136, 3, 128
+    codes = torch.randint(-127, 128, (M, K), generator=g, device=gpu_dev, dtype=torch.int32).to(torch.int8)
+    a = torch.randint(-100, 101, (L, R, K), generator=g, device=gpu_dev).to(BF16)
+    rank_of = torch.randint(0, R, (L, N), generator=g, device=gpu_dev)
+    b = torch.zeros(L, N, R, device=gpu_dev).scatter_(2, rank_of[:, :, None], 1.0).to(BF16)
+    ids = torch.randint(-1, L, (M // 8,), generator=g, device=gpu_dev).repeat_interleave(8)
+    w = icq.QuantizedWeight(torch.zeros(N, K // (1 if bits == 8 else 2), dtype=torch.int8 if bits == 8 else torch.uint8, device=gpu_dev), torch.ones(N, device=gpu_dev))
+    act = icq.QuantizedActivations.from_codes(codes, torch.ones(M, device=gpu_dev))
+    y = icq.quantized_linear(act, w, adapters=icq.LowRankAdapters(a, b), groups=icq.group_rows(ids, L), out_dtype=F32)
+    x = codes.float()
+    for n in range(-1, L):
+        at = (ids == n).nonzero()[:, 0]
+        want = torch.zeros(at.shape[0], N, device=gpu_dev) if n < 0 else (x[at].double() @ a[n, rank_of[n]].double().T.contiguous()).float()
+        assert torch.equal(y[at], want)
