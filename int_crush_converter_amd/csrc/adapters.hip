@@ -82,10 +82,10 @@ __device__ __forceinline__ lb_f32x4 mma16(lb_u32x4 w, lb_u32x4 x, lb_f32x4 acc) 
 // are exact in 16 bits, the products are summed in fp32.  A work-group's waves
 // take a share of K each; the sums are joined in LDS in a fixed order.
 //
-// Few rows: 48 adapters of 64 rows, rank 16, K = 4096 4.7 to 5.2 us traced, the
+// Few rows: 48 adapters of 64 rows, rank 16, K = 4096 5.3 to 5.5 us traced, the
 // launch and three loads that wait for one another (6.3 MB of A).  Many: 8192 x
-// 12288, rank 64 39 us traced (codes from HBM: 20 us), 8192 x 4096 15 us.  There a
-// CU's work bounds it: 28 us of it with no loads at all, 2.5 operations a code for
+// 12288, rank 64 38 to 40 us traced (codes from HBM: 20 us), 8192 x 4096 15 us.
+// There a CU's work bounds it: 28 us of it with no loads at all, 2.5 operations a code for
 // its value and as many matrix instructions; a round of CUs is what counts, so
 // the rows of a work-group are 32 or 48, whichever needs fewer rounds for its
 // height (32 rows left 6 of 262 work-groups for a second round: 56 us).  16 waves,

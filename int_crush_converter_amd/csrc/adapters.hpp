@@ -55,7 +55,7 @@ __device__ __forceinline__ lb_f32x4 mma_ranks(lb_u32x4 w, lb_u32x4 x, lb_f32x4 a
 
 // Adapter id's part of four consecutive outputs of row m from column n (a multiple
 // of 4), share k of n of its ranks: a dot product in fp32, for rows that seldom share
-// an adapter (t: kTwo or, where WHOLE, kWhole).  64 rows with 48 adapters of rank 16, INT4 12288 x 4096: 16.0 to 16.8 us
+// an adapter (t: kTwo or, where WHOLE, kWhole).  64 rows with 48 adapters of rank 16, INT4 12288 x 4096: 16.6 to 17.3 us
 // traced, 11.8 without adapters; 19 MB of B are most of the difference.
 template <bool WHOLE>
 __device__ __forceinline__ lb_f32x4 adapter_dot4(const Adapted& ad, int64_t N, int64_t m, int id, int64_t n, int share, int shares) {

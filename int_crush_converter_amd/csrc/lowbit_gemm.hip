@@ -250,7 +250,7 @@ __global__ __launch_bounds__(512) void linear_direct_kernel(Operands p) {
 // loads are on their way during a step's products.  Sums are integers: waves
 // add theirs in LDS in any order.
 //
-// One token's four experts of 64, INT4 2816 x 4096: traced 6.6 to 7.4 us, 9.0 to
+// One token's four experts of 64, INT4 2816 x 4096: traced 7.1 to 7.7 us, 9.0 to
 // 9.6 a launch in a graph with weights from HBM (23 MB: 2.5 TB/s); 8 experts 10.9
 // us (4.2 TB/s).  Latency bounds it: the launch, the tile's place, then 4 steps of
 // a wave.  With two or four steps' loads in flight it was slower (12 and 22 %
@@ -410,7 +410,7 @@ __device__ __forceinline__ void meet() {
 // kernel with 16 x 16 instructions, a work-group a tile, was faster: 318 to 323
 // us where this one took 341 to 345 in turn on the same card.
 //
-// The 256 x 256 forms of INT4 and INT8 spill 16 and 4 registers (adapted 82 and
+// The 256 x 256 forms of INT4 and INT8 spill 16 and 4 registers (adapted 81 to
 // 93; the grouped ones of 128 x 256 20 and 3), at a tile's start and end, none
 // in the K loop.  Spills are vector-memory operations like those that meet()
 // counts.  It lets the newest N stay outstanding; with spills among these it
@@ -418,18 +418,22 @@ __device__ __forceinline__ void meet() {
 //
 // Grouped: tiles are numbered group by group, whatever their number of rows; a
 // work-group finds its tile's group by bisection in LDS.  8192 tokens x 4 of 32
-// experts 2816 x 4096 INT4 370 to 383 us, 2.0 POP/s (K = 4096 gives 2.2 in whole tiles;
-// a group's last tile is half empty on average): 128 x 256 by two work-groups of
-// 4 waves a CU, one at its products while the other is at a tile's end.  64 x 256
+// experts 2816 x 4096 INT4 370 to 383 us a call (traced, medians on three cards
+// 403 to 421, least 378), 2.0 POP/s (K = 4096 gives 2.2 in whole tiles; a group's
+// last tile is half empty on average): 128 x 256 by two work-groups of 4 waves a
+// CU, one at its products while the other is at a tile's end.  64 x 256
 // took 409, 256 x 256 414.  Running only the blocks of 32 rows that a last tile
 // has took as long (425 against 424, 256 x 256): rows that repeat cost little of
 // the power that bounds the rest.  512 tokens x 4 of 64 experts, 32 rows each, 64 x
 // 256 tiles: 83 to 87 us, 4.3 to 4.5 TB/s of weights (a large copy: 4.7 to 5.1).
 //
-// Adapted: 8192 x 4096 x 12288 INT4 with rank 64 traced 367 to 374 us where the
-// plain product takes 343 to 349, 8192 x 4096 x 4096 149 and 124.  Adding the
-// adapters' products block by block behind the K loop, each waiting for its
-// operands from L2, took 437 us.
+// Adapted: 8192 x 4096 x 12288 INT4 with rank 64 traced 358 to 372 us (medians on
+// three cards, least 347) where the plain product takes 343 to 349, 8192 x 4096 x
+// 4096 149 and 124.  That is with one adapter or two a tile: each that its rows
+// have costs the stages of its ranks over the whole tile.  8192 x 4096 x 4096, rank
+// 64, a call: 172 us with 64 adapters' rows one after another, 480 with each row
+// one of them at random.  Adding the adapters' products block by block behind the
+// K loop, each waiting for its operands from L2, took 437 us.
 template <int KIND, int WM, int WN, int FM, int FN, int BUF, int MODE = kPlain>
 __global__ __launch_bounds__(64 * WM * WN, adapted(MODE) || FM == 4 ? 2 : 1) void linear_tiled_kernel(Operands p, int grid_m, int grid_n) {
     typedef typename Acc32<KIND>::T acc_t;
@@ -1067,7 +1071,10 @@ template <int KIND> constexpr int kBuffers = KIND == kInt4 ? 3 : 4;
 // quarters of their rounds.  128 against 256, INT4 / INT8, rank 16 where not said,
 // us: 8192 x 4096 x 1024 68 to 77 / 75 to 87; 2304 x 4096 x 2048 43 to 51 / 47 to
 // 58; 4096 x 4096 x 4096 90 to 89 / 100 to 99; 8192 x 4096 x 4096 rank 64 173 to
-// 165 / 189 to 184; 8192 x 4100 x 4096 (0.71) 192 to 242.
+// 165 / 189 to 184; 8192 x 4100 x 4096 (0.71) 192 to 242.  The rule sees neither
+// the number of adapters nor the rank, nor which rows share one: 512 x 4096 x 4096
+// INT4 takes 22 us plain, 39 with 48 adapters of rank 16 in order and 58 mixed,
+// 126 with 512 adapters, 245 with 512 of rank 64.
 int adapted_form(int kind, int64_t M, int64_t N, int64_t K) {
     // (a tile's adapters are known when all but one of the buffers have been asked for)
     if (cdiv(K, kind == kInt8 ? 64 : 128) < (kind == kInt8 ? kBuffers<kInt8> : kBuffers<kInt4>) - 1) return 0;
